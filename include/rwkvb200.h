@@ -343,12 +343,67 @@ int rwkvb200_wkv7_select_path(int path);
  * they do not depend on how many units a call has.
  * Process-wide; no counterpart in the reference. */
 int rwkvb200_wkv7_select_form(int form);
+/* ---------------------------------------------------------------------------------
+ * Gated linear recurrence: the token mixer of the layers that decoders of several layer types put between others.  No
+ * counterpart in the reference.
+ *   x, gx, ga, y, dy, dx, dgx, dga (B,T,C) in `dtype`; s, ds (C), h0, hT, dhT, dh0 (B,C) fp32; first (B,T) bytes.
+ *   L = s[c] sigmoid(ga)    a = exp(-L)    beta = sqrt(1 - a^2)    h_t = a h_{t-1} + beta sigmoid(gx) x    y_t = h_t
+ *   Where first != 0 a document begins: a = 0 and beta = 1, and nothing of the tokens before (infinities and NaN too) reaches it.
+ *   s >= 0 (softplus of a parameter, times a constant, by the caller).  Where L = 0 the gradient through beta is taken as 0.
+ *   h0 (zeros), hT, first, saved, dhT (zeros) and dh0 may be NULL; hT may be h0.
+ * The forward of a training step leaves states in `saved` (rwkvb200_gated_scan_saved_bytes(B,T,C) bytes) for the backward, which
+ * needs `work` (rwkvb200_gated_scan_work_bytes(B,T,C) bytes; free after the call); ds is summed in a fixed order.
+ */
+size_t rwkvb200_gated_scan_saved_bytes(int B, int T, int C);
+size_t rwkvb200_gated_scan_work_bytes(int B, int T, int C);
+int rwkvb200_gated_scan_forward(int dtype, int B, int T, int C, const float* h0, const void* x, const void* gx,
+                                const void* ga, const float* s, const unsigned char* first, void* y, float* hT,
+                                void* saved, void* stream);
+int rwkvb200_gated_scan_backward(int dtype, int B, int T, int C, const void* x, const void* gx, const void* ga,
+                                 const float* s, const unsigned char* first, const void* saved, const void* dy,
+                                 const float* dhT, float* dh0, void* dx, void* dgx, void* dga, float* ds, void* work,
+                                 void* stream);
+/* One new token per row: x, gx, ga, y (B,C), state (pool,C) fp32 advanced in place.  slots (B): which state a row has (NULL: row b
+ * has state b).  A negative slot is a row that only pads the batch: its y stays as it was.  Rows with one slot are tokens of
+ * one sequence in the order of the rows.  A slot >= pool is not touched: y of the row becomes NaN and rwkvb200_device_status 121. */
+int rwkvb200_gated_scan_update(int dtype, int B, int C, int pool, float* state, const int* slots, const void* x,
+                               const void* gx, const void* ga, const float* s, void* y, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * Paged key-value cache.  No counterpart in the reference.
+ *   k_pages, v_pages (pages,Hkv,page,N) in `dtype`: `page` tokens of one head lie behind one another.
+ *   table (B,width) int32: the token at position j of sequence b is in page table[b][j / page], at place j % page.
+ * A page number outside of 0..pages-1 is never followed (the token is left out, rwkvb200_device_status says 131 or 141), nor is
+ * a position beyond width * page (132, 142).
+ *
+ * rwkvb200_paged_append: the new tokens of B sequences go behind the lengths[b] tokens that sequence b has.  k, v (M,Hkv,N) and,
+ * if not NULL, q, q_out (M,Hq,N; may be the same): cu_seqlens NULL: one token per sequence (M = B); else (B+1) int32, the tokens
+ * cu[b] .. cu[b+1]-1 are those of sequence b, rows in front of the first and behind the last are left alone.  A negative length
+ * is a row that only pads the batch: nothing is written for it.  The first R elements of every head of q and k are rotated by
+ * position * inv_freq[j] (inv_freq (R/2) fp32), pairs (j, j+R/2) or, interleaved != 0, (2j, 2j+1); cos and sin are multiplied by
+ * `factor`.  Pages that are written belong to one sequence only. */
+int rwkvb200_paged_append(int dtype, int M, int B, int Hq, int Hkv, int N, int R, int pages, int page, int width,
+                          const void* q, const void* k, const void* v, void* q_out, void* k_pages, void* v_pages,
+                          const int* table, const int* lengths, const int* cu_seqlens, const float* inv_freq,
+                          int interleaved, float factor, void* stream);
+/* rwkvb200_paged_attention: one new token per sequence, q and out (B,Hq,N), Hq a multiple of Hkv (query heads h*Hq/Hkv .. share
+ * key-value head h).  lengths[b] counts the tokens in the cache, the new one among them; those of the last `window` (0: all) count:
+ *   z_j = scale q.k_j    z_j = cap tanh(z_j / cap) if cap > 0    z_j += slopes[h] (j - (len - 1)) if slopes (Hq) is given
+ *   out = softmax(z) v    lse (B,Hq; may be NULL) = log sum exp(z)
+ * No token, or scores of -infinity only: out = 0, lse = -infinity.  A negative length is a row that only pads the batch: its out
+ * and lse stay as they were.  Nothing is read beyond a sequence's tokens.  `work`: rwkvb200_paged_attention_work_bytes bytes,
+ * free after the call; two calls that may run at the same time need one each. */
+size_t rwkvb200_paged_attention_work_bytes(int dtype, int Hq, int Hkv, int N);
+int rwkvb200_paged_attention(int dtype, int B, int Hq, int Hkv, int N, int pages, int page, int width, const void* q,
+                             const void* k_pages, const void* v_pages, const int* table, const int* lengths, float scale,
+                             float cap, int window, const float* slopes, void* out, float* lse, void* work, void* stream);
+
 /* Synchronous read of the current device's sticky status word: 0, or 10 + n / 20 + n when the n-th
  * bounded wait of the tensor-core forward / backward ran out in some thread block (30.. / 40..: the
  * front / back warp group of the two-stage backward, 50.. / 55.. / 60..: loader / matrix / chain group of the
  * staged forward; 70.. / 75.. / 80..: the same groups of the staged RWKV-6 / RWKV-5 forward; 91..: their tcgen05 backward;
  * 101..: the RWKV-7 kernels with the chunks in parallel) (the outputs of
- * that call are then invalid); negative on a CUDA error.  Per device; stays set until cleared. */
+ * that call are then invalid), or 121, 131, 132, 141, 142 as the gated recurrence and the paged cache say; negative on a CUDA error.  Per device; stays set until cleared. */
 int rwkvb200_device_status(void);
 /* Resets the current device's status word.  No counterpart in the reference. */
 int rwkvb200_device_status_clear(void);

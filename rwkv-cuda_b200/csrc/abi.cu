@@ -3,6 +3,7 @@
 #include "common.cuh"
 #include "wkv7_dispatch.cuh"
 #include "wkv6_chunked.cuh"
+#include "paged.cuh"
 #include <atomic>
 #include <initializer_list>
 
@@ -123,8 +124,8 @@ extern "C" int rwkvb200_device_status(void) {
         return RWKVB200_ECUDA;
     }
     const int p = wkv7_l32_bwdp_error(0), q = wkv7_l32_fwdp_error(0), r6 = wkv6_l32_error(0), b6 = wkv6_l32_bwd_error(0);
-    const int v7s = wkv7_scan_error(0);
-    if (p < 0 || q < 0 || r6 < 0 || b6 < 0 || v7s < 0) {
+    const int v7s = wkv7_scan_error(0), gs = gated_scan_error(0), append = paged_append_error(0), attend = paged_attention_error(0);
+    if (p < 0 || q < 0 || r6 < 0 || b6 < 0 || v7s < 0 || gs < 0 || append < 0 || attend < 0) {
         set_error("device_status: reading the status words failed");
         return RWKVB200_ECUDA;
     }
@@ -134,11 +135,14 @@ extern "C" int rwkvb200_device_status(void) {
     if (q) return q + 20;       // the staged RWKV-7 forward 50.. / 55.. / 60..
     if (r6) return r6 + 40;     // the staged RWKV-6 / RWKV-5 forward 70.. / 75.. / 80..
     if (b6) return b6 + 90;     // the tcgen05 RWKV-6 / RWKV-5 backward 91..
-    return v7s ? v7s + 100 : 0; // the RWKV-7 kernels with the chunks in parallel 101..
+    if (v7s) return v7s + 100;  // the RWKV-7 kernels with the chunks in parallel 101..
+    if (gs) return gs + 120;    // indices that point nowhere: a slot of gated_scan_update 121
+    if (append) return append + 130;        // paged_append 131, 132
+    return attend ? attend + 140 : 0;       // paged_attention 141, 142
 }
 
 extern "C" int rwkvb200_device_status_clear(void) {
-    RWKV_REQUIRE(wkv7_l32_clear_errors() == 0 && wkv7_l32_bwdp_error(1) == 0 && wkv7_l32_fwdp_error(1) == 0 && wkv6_l32_error(1) == 0 && wkv6_l32_bwd_error(1) == 0 && wkv7_scan_error(1) == 0, RWKVB200_ECUDA, "device_status_clear: writing the status words failed");
+    RWKV_REQUIRE(wkv7_l32_clear_errors() == 0 && wkv7_l32_bwdp_error(1) == 0 && wkv7_l32_fwdp_error(1) == 0 && wkv6_l32_error(1) == 0 && wkv6_l32_bwd_error(1) == 0 && wkv7_scan_error(1) == 0 && gated_scan_error(1) == 0 && paged_append_error(1) == 0 && paged_attention_error(1) == 0, RWKVB200_ECUDA, "device_status_clear: writing the status words failed");
     return RWKVB200_OK;
 }
 

@@ -1,4 +1,5 @@
-// The host side of the training classes (functions.py) and of RWKV-7 inference (ops.wkv7_state_update) in native code.
+// The host side of the training classes (functions.py), of RWKV-7 inference (ops.wkv7_state_update), of the gated recurrence and
+// of the paged cache (ops.gated_scan_*, ops.paged_*) in native code.
 //
 // A small problem keeps the GPU busy for 5 to 50 us, and the same work in Python (the checks of eight tensors, the stream,
 // the ctypes call, an autograd.Function written in Python and its re-entry from the autograd thread) took 15 us for a
@@ -161,6 +162,7 @@ bool ordinary(const Tensor& x) {
     constexpr c10::DispatchKeySet special({c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::Python});
     return !x.key_set().has_any(special) && !x._fw_grad(0).defined();
 }
+bool ordinary(const std::optional<Tensor>& x) { return !x || ordinary(*x); }
 template <typename T>
 bool ordinary(const T&) { return true; }   // (a number)
 
@@ -169,12 +171,12 @@ void record(const Made& m) {
     const auto& inputs = m.inputs;
     const Saved& s = m.s;
     bool any = false;
-    for (const Tensor& x : inputs) any |= x.requires_grad();
+    for (const Tensor& x : inputs) any |= x.defined() && x.requires_grad();
     if (!any || !at::GradMode::is_enabled()) return;
     auto node = std::shared_ptr<OpNode>(new OpNode(), torch::autograd::deleteNode);
     torch::autograd::edge_list edges;
     edges.reserve(inputs.size());
-    for (const Tensor& x : inputs) edges.push_back(torch::autograd::impl::gradient_edge(x));
+    for (const Tensor& x : inputs) edges.push_back(x.defined() ? torch::autograd::impl::gradient_edge(x) : torch::autograd::Edge());
     node->set_next_edges(std::move(edges));
     node->fn = m.backward;
     node->op = m.op;
@@ -419,6 +421,183 @@ static Made wkv7_statepassing(const Tensor& s0, const Tensor& r, const Tensor& w
     return wkv7_forward(&s0, r, w, k, v, a, b, true);
 }
 
+// ---- gated linear recurrence ------------------------------------------------------------------------------------
+// every tensor of a call is on the device of the first
+struct OnDevice {
+    c10::Device device;
+    const Tensor& operator()(const Tensor& t, const char* name) const {
+        on_device(t, name);
+        TORCH_CHECK(t.device() == device, name, ": tensor is on ", t.device(), ", expected ", device);
+        return t;
+    }
+};
+static void shape(const Tensor& t, at::IntArrayRef sizes, const char* name) {
+    TORCH_CHECK(t.sizes() == sizes, name, ": expected shape ", sizes, ", got ", t.sizes());
+}
+static int whole(int64_t n, const char* name) {   // the C ABI counts in int
+    TORCH_CHECK_VALUE(n <= INT_MAX, name, " = ", n, " is too large");
+    return (int)n;
+}
+static const unsigned char* document_starts(const Tensor& first, int64_t B, int64_t T, const OnDevice& here) {
+    if (!first.defined()) return nullptr;
+    shape(here(first, "first"), {B, T}, "first");
+    TORCH_CHECK(first.is_contiguous(), "first: tensor must be contiguous");
+    TORCH_CHECK_TYPE(first.scalar_type() == at::kBool || first.scalar_type() == at::kByte, "first: expected bool or uint8, got ", first.scalar_type());
+    return static_cast<const unsigned char*>(first.data_ptr());
+}
+struct ScanCall {   // the checks that forward, training forward and backward share
+    int dtype, B, T, C;
+    at::ScalarType d;
+    OnDevice here;
+    ScanCall(const Tensor& x, const Tensor& gx, const Tensor& ga, const Tensor& s) : here{x.device()} {
+        TORCH_CHECK_VALUE(x.dim() == 3, "x: expected (B,T,C), got ", x.sizes());
+        B = whole(x.size(0), "B"), T = whole(x.size(1), "T"), C = whole(x.size(2), "C");
+        d = x.scalar_type();
+        dtype = dt(x, "x");
+        shape(here(gx, "gx"), x.sizes(), "gx");
+        shape(here(ga, "ga"), x.sizes(), "ga");
+        shape(here(s, "s"), {C}, "s");
+    }
+};
+static void gated_scan_forward(const Tensor& x, const Tensor& gx, const Tensor& ga, const Tensor& s, const Tensor& y, const std::optional<Tensor>& h0,
+                               const std::optional<Tensor>& hT, const std::optional<Tensor>& first) {
+    on_device(x, "x");
+    const c10::cuda::CUDAGuard guard(x.device());
+    const ScanCall c(x, gx, ga, s);
+    const auto f = at::kFloat;
+    shape(c.here(y, "y"), x.sizes(), "y");
+    if (h0) shape(c.here(*h0, "h0"), {c.B, c.C}, "h0");
+    if (hT) shape(c.here(*hT, "hT"), {c.B, c.C}, "hT");
+    check_rc(rwkvb200_gated_scan_forward(c.dtype, c.B, c.T, c.C, h0 ? f32(ptr(*h0, "h0", f)) : nullptr, ptr(x, "x", c.d), ptr(gx, "gx", c.d),
+                                         ptr(ga, "ga", c.d), f32(ptr(s, "s", f)), document_starts(first ? *first : Tensor(), c.B, c.T, c.here),
+                                         ptr(y, "y", c.d), hT ? f32(ptr(*hT, "hT", f)) : nullptr, nullptr, stream()),
+             "rwkvb200_gated_scan_forward");
+}
+// (s.in: x, gx, ga, s, first; the initial state is the first of the states that the forward keeps)
+static variable_list gated_scan_backward(const Saved& s, const variable_list& g) {
+    const auto [B, T, C, state, d4, d5] = s.dims;
+    const c10::cuda::CUDAGuard guard(s.in[0].device());
+    const auto d = s.in[0].scalar_type(), f = at::kFloat;
+    const Tensor &dy = g[0], &dhT = g[1];
+    numel(dy, B * T * C, "dy");
+    numel(dhT, B * C, "dhT");
+    Outputs o(3 * B * T * C, 3, d, dy);
+    Tensor dx = o.next({B, T, C}, dy), dgx = o.next({B, T, C}, dy), dga = o.next({B, T, C}, dy);
+    Tensor ds = empty({C}, f, dy), dh0 = state ? empty({B, C}, f, dy) : Tensor();
+    const Tensor work = bytes(rwkvb200_gated_scan_work_bytes(B, T, C), dy);
+    check_rc(rwkvb200_gated_scan_backward(dt(s.in[0], "x"), B, T, C, s.in[0].data_ptr(), s.in[1].data_ptr(), s.in[2].data_ptr(),
+                                          f32(s.in[3].data_ptr()), s.in[4].defined() ? static_cast<const unsigned char*>(s.in[4].data_ptr()) : nullptr,
+                                          s.own.data_ptr(), ptr(dy, "dy", d), f32(ptr(dhT, "dhT", f)), state ? f32(dh0.data_ptr()) : nullptr,
+                                          dx.data_ptr(), dgx.data_ptr(), dga.data_ptr(), f32(ds.data_ptr()), work.data_ptr(), stream()),
+             "rwkvb200_gated_scan_backward", true);
+    return {std::move(dx), std::move(dgx), std::move(dga), std::move(ds), Tensor(), std::move(dh0)};
+}
+static Made gated_scan(const Tensor& x, const Tensor& gx, const Tensor& ga, const Tensor& s, const std::optional<Tensor>& h0,
+                       const std::optional<Tensor>& first) {
+    on_device(x, "x");
+    const c10::cuda::CUDAGuard guard(x.device());
+    const ScanCall c(x, gx, ga, s);
+    const auto f = at::kFloat;
+    Saved k{{dense(x), dense(gx), dense(ga), dense(s), first ? dense(*first) : Tensor()}, {}, {c.B, c.T, c.C, h0.has_value()}};
+    const Tensor start = h0 ? dense(*h0) : Tensor();
+    if (h0) shape(c.here(start, "h0"), {c.B, c.C}, "h0");
+    Tensor y = empty({c.B, c.T, c.C}, c.d, x), hT = empty({c.B, c.C}, f, x);
+    k.own = bytes(rwkvb200_gated_scan_saved_bytes(c.B, c.T, c.C), x);
+    check_rc(rwkvb200_gated_scan_forward(c.dtype, c.B, c.T, c.C, f32(opt(start, "h0", f)), ptr(k.in[0], "x", c.d), ptr(k.in[1], "gx", c.d),
+                                         ptr(k.in[2], "ga", c.d), f32(ptr(k.in[3], "s", f)), document_starts(k.in[4], c.B, c.T, c.here), y.data_ptr(),
+                                         f32(hT.data_ptr()), k.own.data_ptr(), stream()),
+             "rwkvb200_gated_scan_forward");
+    return {"GATED_SCANBackward", gated_scan_backward, {y, hT}, {x, gx, ga, s, first ? *first : Tensor(), h0 ? *h0 : Tensor()}, std::move(k)};
+}
+static void gated_scan_update(const Tensor& state, const Tensor& x, const Tensor& gx, const Tensor& ga, const Tensor& s, const Tensor& y,
+                              const std::optional<Tensor>& slots) {
+    on_device(x, "x");
+    const c10::cuda::CUDAGuard guard(x.device());
+    const OnDevice here{x.device()};
+    TORCH_CHECK_VALUE(x.dim() == 2, "x: expected (B,C), got ", x.sizes());
+    const int B = whole(x.size(0), "B"), C = whole(x.size(1), "C"), dtype = dt(x, "x");
+    TORCH_CHECK_VALUE(here(state, "state").dim() == 2 && state.size(1) == C, "state: expected (pool,", C, "), got ", state.sizes());
+    shape(here(gx, "gx"), x.sizes(), "gx");
+    shape(here(ga, "ga"), x.sizes(), "ga");
+    shape(here(y, "y"), x.sizes(), "y");
+    shape(here(s, "s"), {C}, "s");
+    if (slots) shape(here(*slots, "slots"), {B}, "slots");
+    const auto d = x.scalar_type(), f = at::kFloat;
+    check_rc(rwkvb200_gated_scan_update(dtype, B, C, whole(state.size(0), "pool"), f32(ptr(state, "state", f)),
+                                        slots ? static_cast<const int*>(ptr(*slots, "slots", at::kInt)) : nullptr, ptr(x, "x", d), ptr(gx, "gx", d),
+                                        ptr(ga, "ga", d), f32(ptr(s, "s", f)), ptr(y, "y", d), stream()),
+             "rwkvb200_gated_scan_update");
+}
+
+// ---- paged cache ------------------------------------------------------------------------------------------------
+static const int* i32(const Tensor& t, const char* name) { return static_cast<const int*>(ptr(t, name, at::kInt)); }
+struct Pools {
+    int pages, Hkv, page, N, B, width;
+    Pools(const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths, const OnDevice& here) {
+        TORCH_CHECK_VALUE(here(k_pages, "k_pages").dim() == 4, "k_pages: expected (pages,Hkv,page,N), got ", k_pages.sizes());
+        shape(here(v_pages, "v_pages"), k_pages.sizes(), "v_pages");
+        TORCH_CHECK_VALUE(here(table, "table").dim() == 2, "table: expected (B,width), got ", table.sizes());
+        pages = whole(k_pages.size(0), "pages"), Hkv = whole(k_pages.size(1), "Hkv"), page = whole(k_pages.size(2), "page");
+        N = whole(k_pages.size(3), "N"), B = whole(table.size(0), "B"), width = whole(table.size(1), "width");
+        shape(here(lengths, "lengths"), {B}, "lengths");
+    }
+};
+static void paged_append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
+                         const std::optional<Tensor>& cu_seqlens, const std::optional<Tensor>& q, const std::optional<Tensor>& q_out,
+                         const std::optional<Tensor>& inv_freq, bool interleaved, double factor) {
+    on_device(k, "k");
+    const c10::cuda::CUDAGuard guard(k.device());
+    const OnDevice here{k.device()};
+    const Pools p(k_pages, v_pages, table, lengths, here);
+    TORCH_CHECK_VALUE(k.dim() == 3, "k: expected (M,Hkv,N), got ", k.sizes());
+    const int M = whole(k.size(0), "M"), dtype = dt(k, "k");
+    const auto d = k.scalar_type();
+    shape(k, {M, p.Hkv, p.N}, "k");
+    shape(here(v, "v"), k.sizes(), "v");
+    TORCH_CHECK_VALUE(q.has_value() == q_out.has_value(), "q and q_out come together");
+    int Hq = 0, R = 0;
+    if (q) {
+        TORCH_CHECK_VALUE(here(*q, "q").dim() == 3, "q: expected (M,Hq,N), got ", q->sizes());
+        Hq = whole(q->size(1), "Hq");
+        shape(*q, {M, Hq, p.N}, "q");
+        shape(here(*q_out, "q_out"), q->sizes(), "q_out");
+    }
+    if (inv_freq) {
+        TORCH_CHECK_VALUE(here(*inv_freq, "inv_freq").dim() == 1, "inv_freq: expected (R/2), got ", inv_freq->sizes());
+        TORCH_CHECK_VALUE(inv_freq->size(0) <= p.N / 2, "inv_freq: ", inv_freq->size(0), " pairs in heads of ", p.N);
+        R = 2 * (int)inv_freq->size(0);
+    }
+    if (cu_seqlens) shape(here(*cu_seqlens, "cu_seqlens"), {p.B + 1}, "cu_seqlens");
+    check_rc(rwkvb200_paged_append(dtype, M, p.B, Hq, p.Hkv, p.N, R, p.pages, p.page, p.width, q ? ptr(*q, "q", d) : nullptr, ptr(k, "k", d),
+                                   ptr(v, "v", d), q ? ptr(*q_out, "q_out", d) : nullptr, ptr(k_pages, "k_pages", d), ptr(v_pages, "v_pages", d),
+                                   i32(table, "table"), i32(lengths, "lengths"), cu_seqlens ? i32(*cu_seqlens, "cu_seqlens") : nullptr,
+                                   R ? f32(ptr(*inv_freq, "inv_freq", at::kFloat)) : nullptr, interleaved, (float)factor, stream()),
+             "rwkvb200_paged_append");
+}
+static void paged_attention(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages, const Tensor& table, const Tensor& lengths,
+                            const Tensor& out, const std::optional<Tensor>& lse, std::optional<double> scale, double cap, int64_t window,
+                            const std::optional<Tensor>& slopes) {
+    on_device(q, "q");
+    const c10::cuda::CUDAGuard guard(q.device());
+    const OnDevice here{q.device()};
+    const Pools p(k_pages, v_pages, table, lengths, here);
+    TORCH_CHECK_VALUE(q.dim() == 3, "q: expected (B,Hq,N), got ", q.sizes());
+    const int Hq = whole(q.size(1), "Hq"), dtype = dt(q, "q");
+    const auto d = q.scalar_type(), f = at::kFloat;
+    shape(q, {p.B, Hq, p.N}, "q");
+    shape(here(out, "out"), q.sizes(), "out");
+    if (lse) shape(here(*lse, "lse"), {p.B, Hq}, "lse");
+    if (slopes) shape(here(*slopes, "slopes"), {Hq}, "slopes");
+    TORCH_CHECK_VALUE(window >= 0, "window: ", window, " is negative");
+    const Tensor work = bytes(rwkvb200_paged_attention_work_bytes(dtype, Hq, p.Hkv, p.N), q);
+    check_rc(rwkvb200_paged_attention(dtype, p.B, Hq, p.Hkv, p.N, p.pages, p.page, p.width, ptr(q, "q", d), ptr(k_pages, "k_pages", d),
+                                      ptr(v_pages, "v_pages", d), i32(table, "table"), i32(lengths, "lengths"),
+                                      (float)(scale ? *scale : 1.0 / std::sqrt((double)p.N)), (float)cap,
+                                      (int)std::min<int64_t>(window, INT_MAX), slopes ? f32(ptr(*slopes, "slopes", f)) : nullptr, ptr(out, "out", d),
+                                      lse ? f32(ptr(*lse, "lse", f)) : nullptr, work.data_ptr(), stream()),
+             "rwkvb200_paged_attention");
+}
+
 // ---- bindings -----------------------------------------------------------------------------------------------
 // A launch may wait for room in the GPU's queue: other Python threads run meanwhile.
 template <typename F>
@@ -467,6 +646,11 @@ static void define(py::module_& m, const char* op_name, Made (*op)(A...), Backwa
 PYBIND11_MODULE(_native, m) {
     m.def("set_error_class", [](py::object cls) { g_error_class = cls.inc_ref().ptr(); });
     m.def("wkv7_state_update", &wkv7_state_update, py::call_guard<py::gil_scoped_release>());
+    m.def("gated_scan_run", &gated_scan_forward, py::call_guard<py::gil_scoped_release>());
+    m.def("gated_scan_update", &gated_scan_update, py::call_guard<py::gil_scoped_release>());
+    m.def("paged_append", &paged_append, py::call_guard<py::gil_scoped_release>());
+    m.def("paged_attention", &paged_attention, py::call_guard<py::gil_scoped_release>());
+    define(m, "gated_scan", &gated_scan, gated_scan_backward);
     define(m, "wkv4", &wkv4, wkv4_backward);
     define(m, "timex", &timex, timex_backward);
     define(m, "wkv5", &wkv5, wkv5_backward);

@@ -185,6 +185,28 @@ class WKV_6STATE_EX(torch.autograd.Function):
         return tuple(_gradients(ctx, native().wkv6_state_backward, gy, dsT))
 
 
+class GATED_SCAN(torch.autograd.Function):
+    """Gated linear recurrence with an fp32 state in and out, (x, gx, ga, s, h0, first) -> (y, hT); no counterpart in the reference.
+
+    x, gx, ga, y (B,T,C) in bf16 or fp32, s (C) and h0, hT (B,C) fp32, first (B,T) bool or uint8; h0 and first may be None:
+        a = exp(-s sigmoid(ga))    h_t = a h_{t-1} + sqrt(1 - a^2) sigmoid(gx) x    y_t = h_t
+    and at a document's first token (first != 0) h_t = sigmoid(gx) x, whatever was before."""
+
+    @classmethod
+    def apply(cls, x, gx, ga, s, h0=None, first=None):
+        out = native().gated_scan(x, gx, ga, s, h0, first) if cls is GATED_SCAN else None
+        return out if out is not None else super().apply(x, gx, ga, s, h0, first)
+
+    @staticmethod
+    def forward(ctx, x, gx, ga, s, h0, first):
+        return _keep(ctx, native().gated_scan_forward(x, gx, ga, s, h0, first))
+
+    @staticmethod
+    def backward(ctx, dy, dhT):
+        *grads, _, dh0 = _gradients(ctx, native().gated_scan_backward, dy, dhT)
+        return *grads, dh0, None
+
+
 class RWKV7_CLAMPW_CUDA_OP(torch.autograd.Function):
     """rwkv7_fast_fused/rwkv7_cuda_benchmark.py:76-96; inputs (B,T,H,N)."""
 

@@ -394,3 +394,40 @@ def wkv7_backward(r, w, k, v, a, b, dy, dsT, s, sa, ds0, dr, dw, dk, dv, da, db)
         call("rwkvb200_wkv7_backward", _dt(r, "r"), B, T, H, N, chunk, *_ptrs(d, r=r, w=w, k=k, v=v, a=a, b=b, dy=dy),
              _ptr(dsT, "dsT", f), _ptr(s, "s", f), _ptr(sa, "sa", f), _ptr(ds0, "ds0", f),
              *_ptrs(d, dr=dr, dw=dw, dk=dk, dv=dv, da=da, db=db), _stream(r))
+
+
+# ---- gated linear recurrence (no counterpart in the reference) --------------------------
+def gated_scan_forward(x, gx, ga, s, y, h0=None, hT=None, first=None):
+    """Inference over T >= 1 tokens: y (B,T,C) and the state hT (B,C) after the last of them; functions.GATED_SCAN has the formulas
+    and trains.  hT may be h0."""
+    _lib.native().gated_scan_run(x, gx, ga, s, y, h0, hT, first)
+
+
+def gated_scan_update(state, x, gx, ga, s, y, slots=None):
+    """One new token per row, x, gx, ga, y (B,C): advances `state` (pool,C) fp32 in place.  slots (B) int32: the state of each row
+    (None: row b has state b); a negative one is a row that only pads the batch (its y is left alone), rows with the same
+    slot are taken in their order, and one >= pool makes the row's y NaN and sets the device status (121)."""
+    _lib.native().gated_scan_update(state, x, gx, ga, s, y, slots)
+
+
+# ---- paged key-value cache (no counterpart in the reference) ----------------------------
+def paged_append(k, v, k_pages, v_pages, table, lengths, cu_seqlens=None, q=None, q_out=None, inv_freq=None, interleaved=False,
+                 rotary_scale=1.0):
+    """Writes new tokens k, v (M,Hkv,N) into the pages (pages,Hkv,page,N) behind the lengths[b] tokens that sequence b has, k
+    rotated by position, and the rotated q (M,Hq,N) into q_out (which may be q).  table (B,width), lengths (B), cu_seqlens (B+1) int32.
+
+    cu_seqlens None: token b is sequence b's; else the tokens cu[b] .. cu[b+1]-1 are, and other rows are left alone.  inv_freq (R/2)
+    fp32: the first R elements of each head turn by position * inv_freq[j], pairs (j, j+R/2) or, interleaved, (2j, 2j+1); cos and
+    sin are multiplied by rotary_scale.  None: nothing turns.  A negative length: nothing is written for that row.  Page numbers
+    outside of the pool and positions beyond the table are left out and set the device status (131, 132).  `lengths` is only
+    read: add the new tokens to it before paged_attention."""
+    _lib.native().paged_append(k, v, k_pages, v_pages, table, lengths, cu_seqlens, q, q_out, inv_freq, interleaved, rotary_scale)
+
+
+def paged_attention(q, k_pages, v_pages, table, lengths, out, lse=None, scale=None, cap=0.0, window=0, slopes=None):
+    """Attention of one new token per sequence, q and out (B,Hq,N), over the lengths[b] tokens (the new one among them) that the
+    cache has of it; query heads share key-value heads in groups of Hq / Hkv.  scale: 1 / sqrt(N) if None.  cap > 0: scores become
+    cap * tanh(score / cap).  window > 0: only the last `window` tokens count.  slopes (Hq) fp32: slope * (j - (len - 1)) is added
+    to the score of token j.  lse (B,Hq) fp32: log of the sum of exp(score).  A length of 0 gives out 0, lse -inf; a negative one
+    leaves the row alone.  Tokens on pages outside of the pool are left out and set the device status (141)."""
+    _lib.native().paged_attention(q, k_pages, v_pages, table, lengths, out, lse, scale, cap, window, slopes)

@@ -1,0 +1,303 @@
+"""GPU tests of the gated linear recurrence against its fp64 form: lengths around the tokens of a warp (8, 16), of a round (64, 128)
+and of several, channels that fill no warp, odd ones, documents, states in and out; gradients against the formulas and against
+differences; values that are not finite; the single-token update and its slots."""
+import pytest
+import torch
+
+from oracle import mixer_oracle as M
+from tests import helpers as Hh
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def inputs(B, T, C, dtype, seed, docs=False, h0=True, scale=1.0):
+    g = Hh.gen(seed)
+    d = dict(x=Hh.randn(g, B, T, C).to(dtype), gx=Hh.randn(g, B, T, C).to(dtype), ga=(scale * Hh.randn(g, B, T, C)).to(dtype),
+             s=-8 * torch.log(Hh.rand(g, C, lo=0.9, hi=0.999)), h0=Hh.randn(g, B, C) if h0 else None,
+             first=Hh.rand(g, B, T) < 0.1 if docs else None, dy=Hh.randn(g, B, T, C).to(dtype), dhT=Hh.randn(g, B, C))
+    return {n: t.cuda() if t is not None else None for n, t in d.items()}
+
+
+def within(got, want, bound, what):
+    off = (got.double() - want).abs()
+    assert (off <= bound).all(), f"{what}: off by {(off / bound).nan_to_num(nan=9e9).max().item():.3g} of the bound"
+
+
+def forward(d):
+    import rwkv_cuda_b200 as R
+    y = torch.full_like(d["x"], float("nan"))
+    hT = torch.full((d["x"].shape[0], d["x"].shape[2]), float("nan"), device="cuda")
+    R.ops.gated_scan_forward(d["x"], d["gx"], d["ga"], d["s"], y, h0=d["h0"], hT=hT, first=d["first"])
+    return y, hT
+
+
+LEAVES = ("x", "gx", "ga", "s", "h0")
+
+
+def train(d, retain=False):
+    import rwkv_cuda_b200 as R
+    leaves = [d[n].detach().requires_grad_(True) for n in LEAVES if d[n] is not None]
+    out = R.functions.GATED_SCAN.apply(*leaves[:4], leaves[4] if d["h0"] is not None else None, d["first"])
+    return out, torch.autograd.grad(out, leaves, (d["dy"], d["dhT"]), retain_graph=retain), leaves
+
+
+def check(d):
+    T, dtype = d["x"].shape[1], d["x"].dtype
+    ins = [d[n] for n in ("x", "gx", "ga", "s", "h0", "first")]
+    y64, hT64 = M.gated_scan(*ins)
+    ybar, hbar = M.gated_scan(*ins, bar=True)
+    for y, hT in (forward(d), train(d)[0]):
+        within(y, y64, M.scan_bound(T, ybar, y64, dtype), "y")
+        within(hT, hT64, M.scan_bound(T, hbar, hT64, F32), "hT")
+    grads = train(d)[1]
+    want, bars = M.gated_scan_gradients(*ins, d["dy"], d["dhT"])
+    for got, w, bar, name in zip(grads, want, bars, ("dx", "dgx", "dga", "ds", "dh0")):
+        within(got, w, M.scan_bound(T, bar, w, got.dtype), name)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,T,C", [(1, 1, 64), (2, 7, 64), (1, 8, 2), (1, 9, 66), (2, 16, 1), (1, 17, 63), (2, 63, 130), (3, 64, 64), (1, 65, 31),
+                                   (1, 127, 96), (2, 128, 64), (1, 129, 65), (2, 300, 192), (1, 1025, 64)])
+def test_lengths_and_channels(dtype, B, T, C):
+    check(inputs(B, T, C, dtype, seed=T, docs=T % 2 == 0, h0=T % 3 != 0))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("scale", [8.0, 15.0])
+def test_gates_that_saturate(dtype, scale):
+    """Gates from sigmoid(-60) to sigmoid(60): decays of 1 - 1e-27 to exp(-s)."""
+    d = inputs(2, 70, 64, dtype, seed=5, scale=scale)
+    d["gx"] = d["ga"].flip(1).contiguous()
+    check(d)
+
+
+def test_documents_at_every_token_and_none():
+    for fill in (0, 1):
+        d = inputs(1, 150, 64, F32, seed=2)
+        d["first"] = torch.full((1, 150), fill, dtype=torch.uint8, device="cuda")
+        check(d)
+
+
+def test_gradients_against_differences():
+    """Central differences of the fp64 form along one direction per input; the third derivative leaves about step^2 = 1e-8 relative."""
+    d = inputs(2, 90, 64, F32, seed=7, docs=True)
+    grads = train(d)[1]
+    ins = {n: d[n].double() for n in LEAVES}
+    value = lambda z: sum((a * b.double()).sum() for a, b in zip(M.gated_scan(*(z[n] for n in LEAVES), d["first"]), (d["dy"], d["dhT"])))
+    for n, got in zip(LEAVES, grads):
+        way = torch.randn(ins[n].shape, dtype=torch.float64, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) * (0.1 if n == "s" else 1)
+        up, down = ({**ins, n: ins[n] + h * way} for h in (1e-4, -1e-4))
+        want, have = (value(up) - value(down)) / 2e-4, (got.double() * way).sum()
+        size = (got.double() * way).abs().sum()
+        assert abs(want - have) <= 1e-5 * size, n   # rounding of the sum's terms to fp32 and the difference's own error are far below
+
+
+def test_unaligned_and_strided():
+    """Tensors that start at an odd element take the one-channel kernels; strided ones are made contiguous by the training class."""
+    for dtype in (BF, F32):
+        d = inputs(2, 40, 64, dtype, seed=3)
+        y, hT = forward(d)
+        out, grads, _ = train(d)
+        moved = dict(d)
+        for n in ("x", "gx", "ga", "dy"):
+            base = torch.empty(d[n].numel() + 1, dtype=dtype, device="cuda")
+            moved[n] = base[1:].view(d[n].shape).copy_(d[n])
+        out2, grads2, _ = train(moved)
+        for a, b in zip((*out, *grads), (*out2, *grads2)):
+            assert torch.equal(a, b)
+        for n in ("x", "gx", "ga", "dy"):
+            moved[n] = d[n].transpose(0, 1).contiguous().transpose(0, 1)
+        moved["first"] = None
+        out3, grads3, _ = train(moved)
+        for a, b in zip((*out, *grads), (*out3, *grads3)):
+            assert torch.equal(a, b)
+        assert torch.equal(out[0], y) and torch.equal(out[1], hT)
+
+
+def test_pieces_are_the_whole():
+    """A prompt in pieces of any length through the state (in place) is the prompt at once, to rounding."""
+    d = inputs(2, 333, 64, F32, seed=4, docs=True)
+    y, hT = forward(d)
+    import rwkv_cuda_b200 as R
+    state, at = d["h0"].clone(), 0
+    for n in (1, 100, 64, 128, 40):
+        cut = {k: d[k][:, at:at + n].contiguous() for k in ("x", "gx", "ga", "first")}
+        part = torch.empty_like(cut["x"])
+        R.ops.gated_scan_forward(cut["x"], cut["gx"], cut["ga"], d["s"], part, h0=state, hT=state, first=cut["first"])
+        torch.testing.assert_close(part, y[:, at:at + n], rtol=1e-5, atol=1e-5)
+        at += n
+    assert at == 333
+    torch.testing.assert_close(state, hT, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_values_that_are_not_finite(bad):
+    """An infinity stays one as long as its document lasts, and neither it nor a NaN reaches another document, another channel or an earlier token;
+    backward, none of dy's reaches later tokens or the document before."""
+    d = inputs(1, 400, 64, F32, seed=6)
+    first = torch.zeros(1, 400, dtype=torch.bool, device="cuda")
+    first[:, 250] = True
+    d["first"] = first
+    clean = forward(d)
+    _, clean_grads, _ = train(d)
+    x = d["x"].clone()
+    x[0, 77, 5] = bad
+    y, hT = forward({**d, "x": x})
+    assert torch.equal(y[:, :77], clean[0][:, :77]) and torch.equal(y[:, 250:], clean[0][:, 250:]) and torch.equal(hT, clean[1])
+    others = [c for c in range(64) if c != 5]
+    assert torch.equal(y[:, :, others], clean[0][:, :, others])
+    seen = y[0, 77:250, 5]
+    assert (seen.isnan() if bad != bad else seen == bad).all()
+    h0 = d["h0"].clone()
+    h0[0, 9] = bad
+    y, hT = forward({**d, "h0": h0})
+    seen = y[0, :250, 9]
+    assert (seen.isnan() if bad != bad else seen == bad).all() and torch.equal(y[:, 250:], clean[0][:, 250:])
+    dy = d["dy"].clone()
+    dy[0, 300, 5] = bad
+    grads = train({**d, "dy": dy})[1]
+    for g, c in zip(grads[:3], clean_grads[:3]):
+        assert torch.equal(g[:, 301:], c[:, 301:]) and torch.equal(g[:, :250], c[:, :250]) and torch.equal(g[:, :, others], c[:, :, others])
+    assert not torch.isfinite(grads[0][0, 251:301, 5]).any()
+    assert torch.equal(grads[4], clean_grads[4])
+
+
+def test_autograd():
+    """Walked twice; only one output used; no state; through torch.autograd.Function."""
+    import rwkv_cuda_b200 as R
+    d = inputs(2, 70, 64, BF, seed=8, docs=True)
+    out, grads, leaves = train(d, retain=True)
+    again = torch.autograd.grad(out, leaves, (d["dy"], d["dhT"]))
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(out, leaves, (d["dy"], d["dhT"]))
+
+    class Sub(R.functions.GATED_SCAN):
+        pass
+    for h0 in (leaves[4], None):
+        outs = []
+        for cls in (R.functions.GATED_SCAN, Sub):
+            y, hT = cls.apply(*leaves[:4], h0, d["first"])
+            one = torch.autograd.grad(y, leaves[:4], d["dy"], retain_graph=True)
+            two = torch.autograd.grad(hT, leaves[:4], d["dhT"])
+            outs.append((y, hT, *one, *two))
+        assert all(torch.equal(a, b) for a, b in zip(*outs))
+    # first as uint8; s alone wants a gradient
+    s = d["s"].clone().requires_grad_(True)
+    y, _ = R.functions.GATED_SCAN.apply(d["x"], d["gx"], d["ga"], s, None, d["first"].to(torch.uint8))
+    assert torch.equal(torch.autograd.grad(y, s, d["dy"])[0], outs[0][5])
+    assert not R.functions.GATED_SCAN.apply(d["x"], d["gx"], d["ga"], d["s"])[0].requires_grad
+
+
+def test_captured_training_step():
+    d = inputs(2, 200, 64, BF, seed=9)
+    want_out, want, _ = train(d)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        train(d)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, grads, _ = train(d)
+    for t in (*out, *grads):
+        t.zero_()
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((*out, *grads), (*want_out, *want)))
+
+
+# ---- one token -----------------------------------------------------------------------------------------------------
+def step(state, x, gx, ga, s, slots):
+    """fp64, row after row"""
+    state, out = state.double().clone(), {}
+    for b, slot in enumerate(slots):
+        if 0 <= slot < state.shape[0]:
+            y, h = M.gated_scan(x[b][None, None], gx[b][None, None], ga[b][None, None], s, state[slot][None])
+            state[slot] = h[0]
+            out[b] = y[0, 0]
+    return state, out
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,C,pool", [(1, 64, 1), (3, 33, 3), (5, 130, 9), (200, 65, 300)])
+def test_update(dtype, B, C, pool):
+    import rwkv_cuda_b200 as R
+    d = inputs(B, 1, C, dtype, seed=B)
+    x, gx, ga = (d[n][:, 0].contiguous() for n in ("x", "gx", "ga"))
+    g = Hh.gen(1)
+    state = Hh.randn(g, pool, C).cuda()
+    for slots in ([int(i) for i in torch.randperm(pool, generator=g)[:B]], None):
+        mine, y = state.clone(), torch.full((B, C), float("nan"), dtype=dtype, device="cuda")
+        R.ops.gated_scan_update(mine, x, gx, ga, d["s"], y, slots=torch.tensor(slots, dtype=torch.int32, device="cuda") if slots else None)
+        want, rows = step(state, x, gx, ga, d["s"], slots or list(range(B)))
+        size = state.abs().double().max() + 8
+        within(mine, want, M.scan_bound(1, size, want, F32), "state")
+        y64 = torch.stack([rows[b] for b in range(B)])
+        within(y, y64, M.scan_bound(1, size, y64, dtype), "y")
+
+
+def test_update_slots():
+    """Padding rows, a slot that is there three times, and one behind the pool."""
+    import rwkv_cuda_b200 as R
+    from rwkv_cuda_b200 import _lib
+    B, C, pool = 300, 70, 40
+    d = inputs(B, 1, C, F32, seed=3)
+    x, gx, ga = (d[n][:, 0].contiguous() for n in ("x", "gx", "ga"))
+    state = Hh.randn(Hh.gen(2), pool, C).cuda()
+    slots = [-1] * B
+    slots[0], slots[7], slots[150], slots[299], slots[20], slots[21] = 5, 5, 11, 5, 0, pool - 1
+    L = _lib.lib()
+    L.rwkvb200_device_status_clear()
+    mine, y = state.clone(), torch.full((B, C), 7.0, device="cuda")
+    R.ops.gated_scan_update(mine, x, gx, ga, d["s"], y, slots=torch.tensor(slots, dtype=torch.int32, device="cuda"))
+    assert L.rwkvb200_device_status() == 0
+    want, rows = step(state, x, gx, ga, d["s"], slots)
+    within(mine, want, M.scan_bound(3, torch.tensor(16.0, device="cuda"), want, F32), "state")
+    for b in range(B):
+        if b in rows:
+            within(y[b], rows[b], M.scan_bound(3, torch.tensor(16.0, device="cuda"), rows[b], F32), "y")
+        else:
+            assert (y[b] == 7.0).all()
+    slots[40], slots[41] = pool, 2 ** 31 - 1
+    again, y2 = state.clone(), torch.full((B, C), 7.0, device="cuda")
+    R.ops.gated_scan_update(again, x, gx, ga, d["s"], y2, slots=torch.tensor(slots, dtype=torch.int32, device="cuda"))
+    assert L.rwkvb200_device_status() == 121
+    assert L.rwkvb200_device_status_clear() == 0 and L.rwkvb200_device_status() == 0
+    assert y2[40].isnan().all() and y2[41].isnan().all() and torch.equal(again, mine)
+    y2[40:42] = 7.0
+    assert torch.equal(y, y2)
+
+
+def test_update_is_the_scan():
+    """Tokens one at a time, bit by bit what the scan makes of them where its sums have the same order (one token a call)."""
+    import rwkv_cuda_b200 as R
+    d = inputs(2, 9, 64, BF, seed=12)
+    a, b = d["h0"].clone(), d["h0"].clone()
+    for t in range(9):
+        x, gx, ga = (d[n][:, t].contiguous() for n in ("x", "gx", "ga"))
+        y, z = torch.empty_like(x), torch.empty_like(x[:, None])
+        R.ops.gated_scan_update(a, x, gx, ga, d["s"], y)
+        R.ops.gated_scan_forward(x[:, None], gx[:, None], ga[:, None], d["s"], z, h0=b, hT=b)
+        torch.testing.assert_close(a, b, rtol=1e-6, atol=1e-6)
+        torch.testing.assert_close(y, z[:, 0], rtol=2 ** -7, atol=1e-6)
+
+
+def test_refusals():
+    import rwkv_cuda_b200 as R
+    d = inputs(2, 5, 64, F32, seed=1, docs=True)
+    y = torch.empty_like(d["x"])
+    call = lambda **k: R.ops.gated_scan_forward(**{**dict(x=d["x"], gx=d["gx"], ga=d["ga"], s=d["s"], y=y, h0=d["h0"], first=d["first"]), **k})
+    for k, error, word in ((dict(gx=d["gx"][:, :4]), RuntimeError, "gx: expected shape"), (dict(s=d["s"][:5]), RuntimeError, "s: expected shape"),
+                           (dict(ga=d["ga"].to(BF)), TypeError, "ga: expected"), (dict(h0=d["h0"][:1]), RuntimeError, "h0: expected shape"),
+                           (dict(first=d["first"].int()), TypeError, "first: expected bool"), (dict(y=y.cpu()), RuntimeError, "CUDA device"),
+                           (dict(x=d["x"].transpose(0, 1).contiguous().transpose(0, 1)), RuntimeError, "contiguous"),
+                           (dict(x=d["x"][0]), ValueError, "expected \\(B,T,C\\)"), (dict(x=d["x"].half()), TypeError, "not supported")):
+        with pytest.raises(error, match=word):
+            call(**k)
+    with pytest.raises(TypeError, match="not supported"):
+        R.functions.GATED_SCAN.apply(d["x"].double(), d["gx"], d["ga"], d["s"])
+    with pytest.raises(R.RwkvB200Error, match="states for 2 rows"):
+        R.ops.gated_scan_update(d["h0"][:1], *(d[n][:, 0].contiguous() for n in ("x", "gx", "ga")), d["s"], y[:, 0].contiguous())
