@@ -6,23 +6,33 @@
 // At the first token of a document a_t = 0 and beta_t = 1.  Gradients, with e_t = a_{t+1} G_{t+1} and e_{T-1} = dhT:
 //
 //   G_t = dy_t + e_t       dx = G beta sigmoid(gx)      dgx = G beta u (1 - sigmoid(gx))
-//   dL = G (u a^2 / beta - a h_{t-1})                   dga = dL L (1 - sigmoid(ga))     ds = sum dL sigmoid(ga)     dh0 = e_{-1}
+//   dL = G a (u a / beta - h_{t-1})                     dga = dL L (1 - sigmoid(ga))     ds = sum dL sigmoid(ga)     dh0 = e_{-1}
 //
 // (dL = 0 at a document's first token; where L = 0 the term through beta is taken as 0.)
 //
-// A block owns 32 lanes x VEC channels of one sequence and goes through it in rounds of kWarps x L tokens, a warp owns L of
-// them: it makes the gates of its tokens in registers, reduces them to (P, H) (the product of the decays and the end state from
-// a zero start), all warps fold those of the warps before theirs onto the block's state, and each walks its tokens once more
-// from its own start state.  Every input is read once, y is written once.
-#include "common.cuh"
+// A block owns 32 lanes x 2 channels of one sequence and goes through it in rounds of kWarps x kTokens tokens, a warp owns
+// kTokens of them: it makes the gates of its tokens in registers, reduces them to (P, H) (the product of the decays and the end
+// state from a zero start), all warps fold those of the warps before theirs onto the block's state, and each walks its tokens
+// once more from its own start state.  Every input is read once, y is written once.  Where there are few (sequence, channel)
+// blocks, a cluster of blocks shares the rounds: block k of K takes rounds k, k + K, ..., and the (P, H) of their rounds go
+// through distributed shared memory, one cluster barrier for K rounds.
+//
+// Every warp copies its own tokens to shared memory (cp.async), one or two rounds ahead: that keeps enough bytes in flight and
+// needs no barrier.  What bounds the kernels is in front of each.
+#include "packed.cuh"
+#include <cooperative_groups.h>
+#include <type_traits>
 
 namespace rwkvb200 {
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int kWarps = 8;
-constexpr int kFwdTokens = 16;                    // per warp and round
-constexpr int kBwdTokens = 8;
-constexpr int kSaved = kWarps * kBwdTokens;       // the forward saves the state before every 64th token: a round of the backward
+constexpr int kTokens = 8;                   // per warp and round
+constexpr int kRound = kWarps * kTokens;     // the forward saves the state before every round for the backward
+constexpr int kTile = 64;                    // channels of a block
+constexpr int kMaxCluster = 8;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -40,86 +50,118 @@ __device__ __forceinline__ float rsqrt_fast(float x) {
     return y;
 }
 
-// Gates of one channel at one token.  For bf16 tensors by the hardware approximations (2e-7 relative: 2^-14 of a step of bf16),
-// for fp32 by CUDA's functions.  1 - a^2 by its series where L is small: the difference would lose its digits there.  A square
-// below the normal numbers counts as 0, and its root and inverse root are 0 (below 0, which only a negative s makes, NaN).
-template <typename E> struct Gates;
-template <> struct Gates<bf16> {
+// The functions behind the gates: for bf16 tensors the hardware approximations (2e-7 relative: 2^-14 of a step of bf16), for fp32
+// CUDA's exponential and one step of Newton's method behind the others.
+template <typename E> struct Fn;
+template <> struct Fn<bf16> {
     static __device__ __forceinline__ float exp_minus(float x) { return ex2(-1.4426950408889634f * x); }
     static __device__ __forceinline__ float inverse(float x) { return rcp(x); }
-    // 1 - exp(-2L): five terms leave z^5/720 = 7e-6 at z = 0.35
-    static __device__ __forceinline__ float square(float L, float a) {
-        const float z = 2.f * L;
-        const float p = z * fmaf(-z, fmaf(-z, fmaf(-z, fmaf(-z, 1.f / 120.f, 1.f / 24.f), 1.f / 6.f), 0.5f), 1.f);
-        return z < 0.35f ? p : fmaf(-a, a, 1.f);
-    }
-    static __device__ __forceinline__ float inverse_root(float v) { return fabsf(v) < 1.2e-38f ? 0.f : rsqrt_fast(v); }
-    static __device__ __forceinline__ float root(float v) { return v * inverse_root(v); }
+    static __device__ __forceinline__ float inverse_root(float v) { return rsqrt_fast(v); }
 };
-template <> struct Gates<float> {
+template <> struct Fn<float> {
     static __device__ __forceinline__ float exp_minus(float x) { return expf(-x); }
-    static __device__ __forceinline__ float inverse(float x) { return 1.f / x; }
-    static __device__ __forceinline__ float square(float L, float a) {   // eight terms: z^8/9! = 6e-10
-        const float z = 2.f * L;
-        float p = 1.f / 40320.f;
-        p = fmaf(-z, p, 1.f / 5040.f);
-        p = fmaf(-z, p, 1.f / 720.f);
-        p = fmaf(-z, p, 1.f / 120.f);
-        p = fmaf(-z, p, 1.f / 24.f);
-        p = fmaf(-z, p, 1.f / 6.f);
-        p = fmaf(-z, p, 0.5f);
-        p = z * fmaf(-z, p, 1.f);
-        return z < 0.35f ? p : fmaf(-a, a, 1.f);
+    static __device__ __forceinline__ float inverse(float x) {   // (of 1 to 4)
+        const float r = rcp(x);
+        return fmaf(r, fmaf(-x, r, 1.f), r);
     }
-    static __device__ __forceinline__ float inverse_root(float v) { return fabsf(v) < 1.2e-38f ? 0.f : 1.f / sqrtf(v); }
-    static __device__ __forceinline__ float root(float v) { return fabsf(v) < 1.2e-38f ? 0.f : sqrtf(v); }
+    static __device__ __forceinline__ float inverse_root(float v) {
+        const float r = rsqrt_fast(v);
+        return fmaf(0.5f * r, fmaf(-v * r, r, 1.f), r);
+    }
 };
-template <typename E> __device__ __forceinline__ float sigmoid(float x) { return Gates<E>::inverse(1.f + Gates<E>::exp_minus(x)); }
-// A sigmoid that keeps the digits of 1 - sigmoid(x) too: the smaller of the two, negative where that is 1 - sigmoid(x).
-template <typename E> __device__ __forceinline__ float sigmoid_pair(float x) {
-    const float q = Gates<E>::exp_minus(fabsf(x)), m = q * Gates<E>::inverse(1.f + q);
-    return x > 0.f ? -m : m;
-}
-__device__ __forceinline__ float of_pair(float v) { return __float_as_int(v) < 0 ? 1.f + v : v; }
-__device__ __forceinline__ float rest_of_pair(float v) { return __float_as_int(v) < 0 ? -v : 1.f - v; }
 
-// VEC neighbouring channels of one token as they lie in memory
-template <typename E, int VEC> struct Pack;
-template <> struct Pack<bf16, 2> {
-    uint32_t w;
-    __device__ __forceinline__ float get(int i) const { return __uint_as_float(i ? w & 0xffff0000u : w << 16); }
-    __device__ __forceinline__ void set(const float* v) {
-        const __nv_bfloat162 t = __floats2bfloat162_rn(v[0], v[1]);
-        w = *reinterpret_cast<const uint32_t*>(&t);
+__device__ __forceinline__ f2 both(float x) { return pack2(x, x); }
+__device__ __forceinline__ float lo(f2 v) {
+    float a, b;
+    unpack2(v, a, b);
+    return a;
+}
+__device__ __forceinline__ float hi(f2 v) {
+    float a, b;
+    unpack2(v, a, b);
+    return b;
+}
+template <typename F> __device__ __forceinline__ f2 each(f2 a, F f) { return pack2(f(lo(a)), f(hi(a))); }
+template <typename F> __device__ __forceinline__ f2 each(f2 a, f2 b, F f) { return pack2(f(lo(a), lo(b)), f(hi(a), hi(b))); }
+
+// 1 - exp(-L) of two channels, with all its digits where L is small: by its series for L / 8 (five terms leave (1/8)^5/720 = 4e-8),
+// doubled three times, 1 - a^2 = (1 - a) (2 - (1 - a)).  That serves L < 1 and takes no special function; beyond it the exponential.
+template <typename E>
+__device__ __forceinline__ f2 fall(f2 L, bool small) {
+    const f2 r = mul2(L, both(0.125f)), two = both(2.f), minus = both(-1.f);
+    f2 q = fma2(r, both(1.f / 120.f), both(-1.f / 24.f));
+    q = fma2(q, r, both(1.f / 6.f));
+    q = fma2(q, r, both(-0.5f));
+    q = fma2(q, r, both(1.f));
+    q = mul2(q, r);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) q = mul2(q, fma2(q, minus, two));
+    if (small) return q;   // (s <= 1 in all channels of the warp)
+    return each(L, q, [](float l, float p) { return l < 1.f ? p : 1.f - Fn<E>::exp_minus(l); });
+}
+__device__ __forceinline__ f2 square(f2 q) { return mul2(q, fma2(q, both(-1.f), both(2.f))); }
+__device__ __forceinline__ f2 decay(f2 q) { return fma2(q, both(-1.f), both(1.f)); }
+// 1 / sqrt(1 - a^2); 0 below the normal numbers, where beta counts as 0 (and NaN below 0, which only a negative s makes)
+template <typename E>
+__device__ __forceinline__ f2 inverse_root(f2 v) {
+    return each(v, [](float x) { return fabsf(x) < 1.2e-38f ? 0.f : Fn<E>::inverse_root(x); });
+}
+
+// sigmoid(x) and 1 - sigmoid(x) without loss of either: m is the smaller of the two, with the sign of x in front of it
+__device__ __forceinline__ float of_pair(float m) { return __float_as_int(m) < 0 ? 1.f + m : m; }
+__device__ __forceinline__ float rest_of_pair(float m) { return __float_as_int(m) < 0 ? -m : 1.f - m; }
+// Both gates of two channels from one division: exp(-|x|) <= 1, so that no product overflows.
+template <typename E>
+__device__ __forceinline__ void gates(f2 ga, f2 gx, f2& ea, f2& ex, f2& ra, f2& rx) {
+    const f2 one = both(1.f);
+    ea = each(ga, [](float v) { return Fn<E>::exp_minus(fabsf(v)); });
+    ex = each(gx, [](float v) { return Fn<E>::exp_minus(fabsf(v)); });
+    const f2 da = add2(ea, one), dx = add2(ex, one);
+    const f2 r = each(mul2(da, dx), [](float v) { return Fn<E>::inverse(v); });
+    ra = mul2(r, dx);   // 1 / (1 + exp(-|ga|))
+    rx = mul2(r, da);
+}
+__device__ __forceinline__ f2 sigmoid(f2 x, f2 e, f2 r) {
+    const f2 m = mul2(e, r);
+    return pack2(lo(x) > 0.f ? lo(r) : lo(m), hi(x) > 0.f ? hi(r) : hi(m));
+}
+__device__ __forceinline__ f2 sigmoid_pair(f2 x, f2 e, f2 r) {
+    const f2 m = mul2(e, r);
+    return pack2(lo(x) > 0.f ? -lo(m) : lo(m), hi(x) > 0.f ? -hi(m) : hi(m));
+}
+
+// two neighbouring channels in shared memory, and back
+__device__ __forceinline__ f2 get2(const bf16* p) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+    return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ f2 get2(const float* p) {
+    const float2 w = *reinterpret_cast<const float2*>(p);
+    return pack2(w.x, w.y);
+}
+// ... to global memory: as one word, or one after the other where C is odd or a tensor starts between two words
+template <bool PAIRS>
+__device__ __forceinline__ void put2(bf16* p, f2 v, bool second) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(lo(v), hi(v));
+    if (PAIRS) {
+        *reinterpret_cast<__nv_bfloat162*>(p) = t;
+    } else {
+        p[0] = t.x;
+        if (second) p[1] = t.y;
     }
-};
-template <> struct Pack<bf16, 1> {
-    bf16 w;
-    __device__ __forceinline__ float get(int) const { return __bfloat162float(w); }
-    __device__ __forceinline__ void set(const float* v) { w = __float2bfloat16_rn(v[0]); }
-};
-template <> struct alignas(8) Pack<float, 2> {
-    float2 w;
-    __device__ __forceinline__ float get(int i) const { return i ? w.y : w.x; }
-    __device__ __forceinline__ void set(const float* v) { w = make_float2(v[0], v[1]); }
-};
-template <> struct Pack<float, 1> {
-    float w;
-    __device__ __forceinline__ float get(int) const { return w; }
-    __device__ __forceinline__ void set(const float* v) { w = v[0]; }
-};
-template <typename E, int VEC>
-__device__ __forceinline__ Pack<E, VEC> load(const E* p) { return *reinterpret_cast<const Pack<E, VEC>*>(p); }
-template <typename E, int VEC>
-__device__ __forceinline__ Pack<E, VEC> zero() {
-    Pack<E, VEC> z;
-    const float v[2] = {0.f, 0.f};
-    z.set(v);
-    return z;
+}
+template <bool PAIRS>
+__device__ __forceinline__ void put2(float* p, f2 v, bool second) {
+    if (PAIRS) {
+        *reinterpret_cast<float2*>(p) = make_float2(lo(v), hi(v));
+    } else {
+        p[0] = lo(v);
+        if (second) p[1] = hi(v);
+    }
 }
 
 struct Args {
-    int T, C, tiles, rounds_saved;
+    int T, C, tiles, rounds;   // channel tiles, rounds of kRound tokens
     const float* h0;
     const void *x, *gx, *ga;
     const float* s;
@@ -136,241 +178,346 @@ struct Args {
 };
 
 // which of a warp's tokens from t on begin a document, a bit each
-template <int L>
 __device__ __forceinline__ uint32_t firsts(const uint8_t* first, int t, int T, int lane) {
     if (first == nullptr) return 0;
-    const bool f = lane < L && t + lane < T && first[t + lane] != 0;
+    const bool f = lane < kTokens && t + lane < T && first[t + lane] != 0;
     return __ballot_sync(0xffffffffu, f);
 }
 
-// A warp's share of a round reduced to one step: h -> P h + H, or H alone where a document begins in it (whatever h is: one
-// document's infinities do not reach the next).  A product that underflows must not make an infinite state NaN.
-__device__ __forceinline__ float fold(bool cut, float P, float H, float h) { return cut ? H : fmaf(fmaxf(P, 1e-45f), h, H); }
+// The [kTokens][kTile] tile of a tensor from token t on: to shared memory, without waiting.  WIDE: every row of C starts on a 16-byte
+// boundary, and a piece of 16 bytes is asked for at a time; else element by element, at once.  What lies outside is left alone.
+template <typename E, bool WIDE>
+__device__ __forceinline__ void fetch(E* tile, const E* from, int t, int T, int C, int c_tile, int lane) {
+    if (WIDE) {
+        constexpr int n = 16 / sizeof(E), row = kTile / n;   // pieces of a row
+#pragma unroll
+        for (int i = 0; i < kTokens * row / 32; ++i) {
+            const int piece = i * 32 + lane, j = piece / row, c = piece % row * n;
+            if (t + j < T && c_tile + c < C) {
+                const uint32_t to = (uint32_t)__cvta_generic_to_shared(tile + j * kTile + c);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from + (i64)(t + j) * C + c) : "memory");
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kTokens; ++j) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int c = i * 32 + lane;
+                if (t + j < T && c_tile + c < C) tile[j * kTile + c] = from[(i64)(t + j) * C + c];
+            }
+        }
+    }
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_group() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <typename E, int VEC>
-__global__ void __launch_bounds__(32 * kWarps) scan_forward_kernel(const Args p) {
-    constexpr int L = kFwdTokens;
-    __shared__ float sP[2][kWarps][32 * VEC], sH[2][kWarps][32 * VEC];
-    __shared__ int sCut[2][kWarps];
+// Shares of a round reduced to one step each: h -> P h + H, or H alone where a document begins in it (P = 0; whatever h is: one document's
+// infinities and NaN do not reach the next).  A product of decays that underflows is kept above 0: it must not make an infinite
+// state NaN, and 0 means a document.
+constexpr float kTiny = 1e-45f;
+__device__ __forceinline__ f2 clamp(f2 P) {
+    return each(P, [](float v) { return v < kTiny ? kTiny : v; });   // (a NaN stays one)
+}
+__device__ __forceinline__ f2 step(f2 P, f2 H, f2 h) {
+    const f2 n = fma2(P, h, H);
+    return pack2(lo(P) == 0.f ? lo(H) : lo(n), hi(P) == 0.f ? hi(H) : hi(n));
+}
+__device__ __forceinline__ f2 behind(f2 P, f2 before) {   // the product of two shares: 0 if one of them is a document's
+    const f2 n = clamp(mul2(P, before));
+    return pack2(lo(P) == 0.f || lo(before) == 0.f ? 0.f : lo(n), hi(P) == 0.f || hi(before) == 0.f ? 0.f : hi(n));
+}
+struct Share {
+    f2 P, H;
+};
+// All shares of the block in the order of time (backward: `reversed`): those before warp `warp` in `mine`, all of them in `all`.
+template <bool REVERSED>
+__device__ __forceinline__ void fold(const ulonglong2 (*shares)[32], int warp, int lane, bool cuts, Share& mine, Share& all) {
+    Share a{both(1.f), both(0.f)};
+    if (!cuts) {
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+            const int q = REVERSED ? kWarps - 1 - i : i;
+            if (q == warp) mine = a;
+            const ulonglong2 v = shares[q][lane];
+            a.H = fma2(v.x, a.H, v.y);
+            a.P = mul2(a.P, v.x);
+        }
+        mine.P = clamp(mine.P);
+        a.P = clamp(a.P);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+            const int q = REVERSED ? kWarps - 1 - i : i;
+            if (q == warp) mine = a;
+            const ulonglong2 v = shares[q][lane];
+            a.H = step(v.x, v.y, a.H);
+            a.P = behind(v.x, a.P);
+        }
+    }
+    all = a;
+}
+// The state before this block's round and the one behind the rounds of all blocks of the cluster, from the state before them.
+template <bool REVERSED>
+__device__ __forceinline__ f2 through_cluster(cg::cluster_group& cluster, int K, int rank, ulonglong2 (*peers)[32], const Share& all, int warp, int lane, f2& carry) {
+    if (K == 1) {
+        const f2 start = carry;
+        carry = step(all.P, all.H, carry);
+        return start;
+    }
+    if (warp < K) *cluster.map_shared_rank(&peers[rank][lane], warp) = make_ulonglong2(all.P, all.H);
+    cluster.sync();
+    f2 start = carry;
+    for (int i = 0; i < K; ++i) {
+        const int q = REVERSED ? K - 1 - i : i;
+        if (q == rank) start = carry;
+        const ulonglong2 v = peers[q][lane];
+        carry = step(v.x, v.y, carry);
+    }
+    return start;
+}
+
+template <typename E> constexpr int kFwdStages = sizeof(E) == 2 ? 3 : 2;
+constexpr int kBwdStages = 2;
+template <typename E> constexpr int fwd_smem() { return kFwdStages<E> * kWarps * 3 * kTokens * kTile * (int)sizeof(E); }
+template <typename E> constexpr int bwd_smem() { return kBwdStages * kWarps * 4 * kTokens * kTile * (int)sizeof(E); }
+
+template <typename E, bool WIDE, bool PAIRS>
+__global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args p) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    __shared__ ulonglong2 shares[2][kWarps][32], peers[2][kMaxCluster][32];
+    constexpr int S = kFwdStages<E>, kPart = kTokens * kTile;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int b = blockIdx.x / p.tiles, c0 = (blockIdx.x % p.tiles) * 32 * VEC + lane * VEC;
-    const bool live = c0 < p.C;
-    const i64 base = (i64)b * p.T * p.C + c0;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int K = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), unit = blockIdx.x / K;
+    const int b = unit / p.tiles, c_tile = unit % p.tiles * kTile, c0 = c_tile + lane * 2;
+    const bool live = c0 < p.C, second = c0 + 1 < p.C;
+    const i64 base = (i64)b * p.T * p.C + c_tile;
     const E *x = static_cast<const E*>(p.x) + base, *gx = static_cast<const E*>(p.gx) + base, *ga = static_cast<const E*>(p.ga) + base;
-    E* y = static_cast<E*>(p.y) + base;
+    E* y = static_cast<E*>(p.y) + base + lane * 2;
+    E* mine = reinterpret_cast<E*>(raw) + warp * 3 * kPart;
     const uint8_t* first = p.first ? p.first + (i64)b * p.T : nullptr;
-    float s[VEC], carry[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        s[i] = live ? p.s[c0 + i] : 0.f;
-        carry[i] = live && p.h0 ? p.h0[(i64)b * p.C + c0 + i] : 0.f;
-    }
-    for (int t0 = 0, buf = 0; t0 < p.T; t0 += kWarps * L, buf ^= 1) {
-        const int t = t0 + warp * L;
-        const uint32_t docs = firsts<L>(first, t, p.T, lane);
-        Pack<E, VEC> px[L], pgx[L], pga[L];
-#pragma unroll
-        for (int j = 0; j < L; ++j) {
-            const bool in = live && t + j < p.T;
-            const i64 at = (i64)(t + j) * p.C;
-            px[j] = in ? load<E, VEC>(x + at) : zero<E, VEC>();
-            pgx[j] = in ? load<E, VEC>(gx + at) : zero<E, VEC>();
-            pga[j] = in ? load<E, VEC>(ga + at) : zero<E, VEC>();
+    const f2 s = pack2(live ? p.s[c0] : 0.f, second ? p.s[c0 + 1] : 0.f);
+    const i64 row = (i64)b * p.C + c0;
+    f2 carry = pack2(live && p.h0 ? p.h0[row] : 0.f, second && p.h0 ? p.h0[row + 1] : 0.f);
+    const bool small = __all_sync(0xffffffffu, lo(s) <= 1.f && hi(s) <= 1.f);
+
+    auto ask = [&](int round, int stage) {
+        const int t = round * kRound + warp * kTokens;
+        E* to = mine + stage * kWarps * 3 * kPart;
+        if (t < p.T) {
+            fetch<E, WIDE>(to, x, t, p.T, p.C, c_tile, lane);
+            fetch<E, WIDE>(to + kPart, gx, t, p.T, p.C, c_tile, lane);
+            fetch<E, WIDE>(to + 2 * kPart, ga, t, p.T, p.C, c_tile, lane);
         }
-        float a[L][VEC], w[L][VEC], P[VEC], H[VEC];
+        commit();
+    };
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) P[i] = 1.f, H[i] = 0.f;
+    for (int i = 0; i < S - 1; ++i) ask(rank + i * K, i);
+    if (K > 1) cluster.sync();   // (a block's shared memory is written by others once it has begun)
+    int stage = 0, buf = 0;
+    for (int r0 = 0; r0 < p.rounds; r0 += K, buf ^= 1) {   // (all blocks of a cluster go through the same barriers)
+        const int round = r0 + rank, t = round * kRound + warp * kTokens;
+        ask(round + (S - 1) * K, stage == 0 ? S - 1 : stage - 1);
+        wait_group<S - 1>();
+        __syncwarp();
+        const E* in = mine + stage * kWarps * 3 * kPart + lane * 2;
+        const uint32_t docs = firsts(first, t, p.T, lane);
+        f2 a[kTokens], w[kTokens];
+        Share mine_share{both(1.f), both(0.f)};
+        auto make = [&](auto plain) {   // plain: all tokens are there, and none begins a document
+            constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
-        for (int j = 0; j < L; ++j) {
-            const bool doc = docs >> j & 1, past = t + j >= p.T;
+            for (int j = 0; j < kTokens; ++j) {
+                const f2 vx = get2(in + j * kTile), vgx = get2(in + kPart + j * kTile), vga = get2(in + 2 * kPart + j * kTile);
+                f2 ea, ex, ra, rx;
+                gates<E>(vga, vgx, ea, ex, ra, rx);
+                const f2 q = fall<E>(mul2(s, sigmoid(vga, ea, ra)), small), v = square(q), u = mul2(sigmoid(vgx, ex, rx), vx);
+                f2 aj = decay(q), wj = mul2(mul2(v, inverse_root<E>(v)), u);
+                if (!kPlain) {
+                    if (docs >> j & 1) aj = both(0.f), wj = u;
+                    if (t + j >= p.T) aj = both(1.f), wj = both(0.f);
+                }
+                a[j] = aj;
+                w[j] = wj;
+                if (kPlain) {
+                    mine_share.H = fma2(aj, mine_share.H, wj);
+                    mine_share.P = mul2(mine_share.P, aj);
+                } else {
+                    mine_share.H = docs >> j & 1 ? wj : fma2(aj, mine_share.H, wj);
+                    mine_share.P = mul2(mine_share.P, aj);
+                }
+            }
+            mine_share.P = !kPlain && docs ? both(0.f) : clamp(mine_share.P);
+        };
+        if (docs == 0 && t + kTokens <= p.T) make(std::true_type{}); else make(std::false_type{});
+        shares[buf][warp][lane] = make_ulonglong2(mine_share.P, mine_share.H);
+        const bool cuts = __syncthreads_or(docs != 0);   // (a buffer is written again two rounds on, behind the next barrier)
+        Share before, all;
+        fold<false>(shares[buf], warp, lane, cuts, before, all);
+        f2 h = through_cluster<false>(cluster, K, rank, peers[buf], all, warp, lane, carry);
+        h = step(before.P, before.H, h);
+        if (live && t < p.T) {
+            if (p.saved != nullptr && warp == 0) {
+                float* to = p.saved + ((i64)b * p.rounds + round) * p.C + c0;
+                to[0] = lo(h);
+                if (second) to[1] = hi(h);
+            }
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float len = s[i] * sigmoid<E>(pga[j].get(i));
-                const float d = Gates<E>::exp_minus(len), beta = doc ? 1.f : Gates<E>::root(Gates<E>::square(len, d));
-                a[j][i] = past ? 1.f : d;
-                w[j][i] = past ? 0.f : beta * (sigmoid<E>(pgx[j].get(i)) * px[j].get(i));
-                H[i] = doc ? w[j][i] : fmaf(a[j][i], H[i], w[j][i]);
-                P[i] *= a[j][i];
+            for (int j = 0; j < kTokens; ++j) {
+                if (t + j >= p.T) break;
+                h = docs >> j & 1 ? w[j] : fma2(a[j], h, w[j]);
+                put2<PAIRS>(y + (i64)(t + j) * p.C, h, second);
             }
         }
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            sP[buf][warp][lane * VEC + i] = P[i];
-            sH[buf][warp][lane * VEC + i] = H[i];
-        }
-        if (lane == 0) sCut[buf][warp] = docs != 0;
-        __syncthreads();   // (a buffer is written again two rounds on, behind the next round's barrier)
-        float h[VEC];
-#pragma unroll
-        for (int q = 0; q < kWarps; ++q) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                if (q == warp) h[i] = carry[i];
-                carry[i] = fold(sCut[buf][q], sP[buf][q][lane * VEC + i], sH[buf][q][lane * VEC + i], carry[i]);
-            }
-        }
-        if (!live) continue;
-        if (p.saved != nullptr && t % kSaved == 0 && t < p.T) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) p.saved[((i64)b * p.rounds_saved + t / kSaved) * p.C + c0 + i] = h[i];
-        }
-#pragma unroll
-        for (int j = 0; j < L; ++j) {
-            if (t + j >= p.T) break;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) h[i] = docs >> j & 1 ? w[j][i] : fmaf(a[j][i], h[i], w[j][i]);
-            Pack<E, VEC> o;
-            o.set(h);
-            *reinterpret_cast<Pack<E, VEC>*>(y + (i64)(t + j) * p.C) = o;
-        }
+        stage = stage == S - 1 ? 0 : stage + 1;
+        __syncwarp();
     }
-    if (p.hT != nullptr && warp == 0 && live) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) p.hT[(i64)b * p.C + c0 + i] = carry[i];
+    if (p.hT != nullptr && rank == 0 && warp == 0 && live) {
+        p.hT[row] = lo(carry);
+        if (second) p.hT[row + 1] = hi(carry);
     }
 }
 
 // Rounds from the last to the first; e (the gradient that comes into a token from the later ones) goes the same way as h does in
 // the forward, with the same products of decays.  h before each token is made again from the saved states.
-template <typename E, int VEC>
-__global__ void __launch_bounds__(32 * kWarps) scan_backward_kernel(const Args p) {
-    constexpr int L = kBwdTokens;
-    __shared__ float sP[2][kWarps][32 * VEC], sH[2][kWarps][32 * VEC], sQ[2][kWarps][32 * VEC];
-    __shared__ int sCut[2][kWarps];
+template <typename E, bool WIDE, bool PAIRS>
+__global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_backward_kernel(const Args p) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    __shared__ ulonglong2 shares[2][kWarps][32], forward[2][kWarps][32], peers[2][kMaxCluster][32];
+    constexpr int S = kBwdStages, kPart = kTokens * kTile;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int b = blockIdx.x / p.tiles, c0 = (blockIdx.x % p.tiles) * 32 * VEC + lane * VEC;
-    const bool live = c0 < p.C;
-    const i64 base = (i64)b * p.T * p.C + c0;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int K = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), unit = blockIdx.x / K;
+    const int b = unit / p.tiles, c_tile = unit % p.tiles * kTile, c0 = c_tile + lane * 2;
+    const bool live = c0 < p.C, second = c0 + 1 < p.C;
+    const i64 base = (i64)b * p.T * p.C + c_tile;
     const E *x = static_cast<const E*>(p.x) + base, *gx = static_cast<const E*>(p.gx) + base, *ga = static_cast<const E*>(p.ga) + base,
             *dy = static_cast<const E*>(p.dy) + base;
-    E *dx = static_cast<E*>(p.dx) + base, *dgx = static_cast<E*>(p.dgx) + base, *dga = static_cast<E*>(p.dga) + base;
+    E *dx = static_cast<E*>(p.dx) + base + lane * 2, *dgx = static_cast<E*>(p.dgx) + base + lane * 2, *dga = static_cast<E*>(p.dga) + base + lane * 2;
+    E* mine = reinterpret_cast<E*>(raw) + warp * 4 * kPart;
     const uint8_t* first = p.first ? p.first + (i64)b * p.T : nullptr;
-    float s[VEC], carry[VEC], ds[VEC];
+    const f2 s = pack2(live ? p.s[c0] : 0.f, second ? p.s[c0 + 1] : 0.f);
+    const i64 row = (i64)b * p.C + c0;
+    f2 carry = pack2(live && p.dhT ? p.dhT[row] : 0.f, second && p.dhT ? p.dhT[row + 1] : 0.f), ds = both(0.f);
+    const bool small = __all_sync(0xffffffffu, lo(s) <= 1.f && hi(s) <= 1.f);
+
+    auto ask = [&](int round, int stage) {
+        const int t = round * kRound + warp * kTokens;
+        E* to = mine + stage * kWarps * 4 * kPart;
+        if (round >= 0 && t < p.T) {
+            fetch<E, WIDE>(to, x, t, p.T, p.C, c_tile, lane);
+            fetch<E, WIDE>(to + kPart, gx, t, p.T, p.C, c_tile, lane);
+            fetch<E, WIDE>(to + 2 * kPart, ga, t, p.T, p.C, c_tile, lane);
+            fetch<E, WIDE>(to + 3 * kPart, dy, t, p.T, p.C, c_tile, lane);
+        }
+        commit();
+    };
+    const int turns = (p.rounds + K - 1) / K;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-        s[i] = live ? p.s[c0 + i] : 0.f;
-        carry[i] = live && p.dhT ? p.dhT[(i64)b * p.C + c0 + i] : 0.f;
-        ds[i] = 0.f;
-    }
-    int buf = 0;
-    for (int round = p.rounds_saved - 1; round >= 0; --round, buf ^= 1) {
-        const int t = round * kSaved + warp * L;
-        const uint32_t docs = firsts<L>(first, t, p.T, lane);
-        Pack<E, VEC> px[L], pdy[L];
-        float r[L][VEC], g[L][VEC], a[L][VEC], P[VEC], H[VEC], Q[VEC], hs[VEC], e[VEC];
-        {
-            Pack<E, VEC> pgx[L], pga[L];
+    for (int i = 0; i < S - 1; ++i) ask((turns - 1 - i) * K + rank, i);
+    if (K > 1) cluster.sync();
+    int stage = 0, buf = 0;
+    for (int turn = turns - 1; turn >= 0; --turn, buf ^= 1) {
+        const int round = turn * K + rank, t = round * kRound + warp * kTokens;
+        ask(round - (S - 1) * K, stage == 0 ? S - 1 : stage - 1);
+        f2 h = both(0.f);
+        if (live && round < p.rounds) {
+            const float* from = p.saved + ((i64)b * p.rounds + round) * p.C + c0;
+            h = pack2(from[0], second ? from[1] : 0.f);
+        }
+        wait_group<S - 1>();
+        __syncwarp();
+        const E* in = mine + stage * kWarps * 4 * kPart + lane * 2;
+        const uint32_t docs = firsts(first, t, p.T, lane);
+        // per token: 1 - a, the gates as pairs, 1 / beta, and w = beta u, which makes room for h before the token
+        f2 q[kTokens], r[kTokens], g[kTokens], inv[kTokens], w[kTokens], P = both(1.f), H = both(0.f), Q = both(0.f);
+        auto make = [&](auto plain) {
+            constexpr bool kPlain = decltype(plain)::value;
 #pragma unroll
-            for (int j = 0; j < L; ++j) {
-                const bool in = live && t + j < p.T;
-                const i64 at = (i64)(t + j) * p.C;
-                px[j] = in ? load<E, VEC>(x + at) : zero<E, VEC>();
-                pgx[j] = in ? load<E, VEC>(gx + at) : zero<E, VEC>();
-                pga[j] = in ? load<E, VEC>(ga + at) : zero<E, VEC>();
-                pdy[j] = in ? load<E, VEC>(dy + at) : zero<E, VEC>();
+            for (int j = 0; j < kTokens; ++j) {
+                const f2 vx = get2(in + j * kTile), vgx = get2(in + kPart + j * kTile), vga = get2(in + 2 * kPart + j * kTile);
+                f2 ea, ex, ra, rx;
+                gates<E>(vga, vgx, ea, ex, ra, rx);
+                r[j] = sigmoid_pair(vga, ea, ra);
+                g[j] = sigmoid_pair(vgx, ex, rx);
+                q[j] = fall<E>(mul2(s, sigmoid(vga, ea, ra)), small);
+                const f2 v = square(q[j]), u = mul2(sigmoid(vgx, ex, rx), vx);
+                inv[j] = inverse_root<E>(v);
+                w[j] = mul2(mul2(v, inv[j]), u);
+                if (!kPlain) {
+                    if (docs >> j & 1) q[j] = both(1.f), inv[j] = both(0.f), w[j] = u;
+                    if (t + j >= p.T) q[j] = both(0.f), w[j] = both(0.f);
+                }
+                const f2 a = decay(q[j]);
+                H = !kPlain && docs >> j & 1 ? w[j] : fma2(a, H, w[j]);
+                P = mul2(P, a);
             }
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                P[i] = 1.f, H[i] = 0.f, Q[i] = 0.f;
-                hs[i] = live ? p.saved[((i64)b * p.rounds_saved + round) * p.C + c0 + i] : 0.f;
-            }
-#pragma unroll
-            for (int j = 0; j < L; ++j) {
-                const bool doc = docs >> j & 1, past = t + j >= p.T;
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    r[j][i] = sigmoid_pair<E>(pga[j].get(i));
-                    g[j][i] = sigmoid_pair<E>(pgx[j].get(i));
-                    const float len = s[i] * of_pair(r[j][i]), d = Gates<E>::exp_minus(len);
-                    const float w = (doc ? 1.f : Gates<E>::root(Gates<E>::square(len, d))) * (of_pair(g[j][i]) * px[j].get(i));
-                    a[j][i] = past ? 1.f : d;
-                    H[i] = doc ? w : fmaf(a[j][i], H[i], past ? 0.f : w);
-                    P[i] *= a[j][i];
+            for (int j = kTokens - 1; j >= 0; --j) {
+                if (kPlain) {
+                    Q = mul2(decay(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
+                } else if (t + j < p.T) {
+                    Q = docs >> j & 1 ? both(0.f) : mul2(decay(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
                 }
             }
+            P = !kPlain && docs ? both(0.f) : clamp(P);
+        };
+        if (docs == 0 && t + kTokens <= p.T) make(std::true_type{}); else make(std::false_type{});
+        shares[buf][warp][lane] = make_ulonglong2(P, Q);
+        forward[buf][warp][lane] = make_ulonglong2(P, H);
+        const bool cuts = __syncthreads_or(docs != 0);
+        Share after, all;
+        fold<true>(shares[buf], warp, lane, cuts, after, all);
+        f2 e = through_cluster<true>(cluster, K, rank, peers[buf], all, warp, lane, carry);
+        e = step(after.P, after.H, e);
+        for (int i = 0; i < warp; ++i) {
+            const ulonglong2 v = forward[buf][i][lane];
+            h = step(v.x, v.y, h);
         }
+        if (live && t < p.T) {
 #pragma unroll
-        for (int j = L - 1; j >= 0; --j)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) Q[i] = docs >> j & 1 ? 0.f : a[j][i] * (pdy[j].get(i) + Q[i]);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            sP[buf][warp][lane * VEC + i] = P[i];
-            sH[buf][warp][lane * VEC + i] = H[i];
-            sQ[buf][warp][lane * VEC + i] = Q[i];
-        }
-        if (lane == 0) sCut[buf][warp] = docs != 0;
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < kWarps; ++q) {
-            if (q < warp) {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) hs[i] = fold(sCut[buf][q], sP[buf][q][lane * VEC + i], sH[buf][q][lane * VEC + i], hs[i]);
+            for (int j = 0; j < kTokens; ++j) {
+                const f2 before = h;
+                h = docs >> j & 1 ? w[j] : fma2(decay(q[j]), h, w[j]);
+                w[j] = before;
             }
-        }
 #pragma unroll
-        for (int q = kWarps - 1; q >= 0; --q) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                if (q == warp) e[i] = carry[i];
-                carry[i] = fold(sCut[buf][q], sP[buf][q][lane * VEC + i], sQ[buf][q][lane * VEC + i], carry[i]);
-            }
-        }
-        if (!live) continue;
-        float before[L][VEC];
-#pragma unroll
-        for (int j = 0; j < L; ++j) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                before[j][i] = hs[i];
+            for (int j = kTokens - 1; j >= 0; --j) {
+                if (t + j >= p.T) continue;
                 const bool doc = docs >> j & 1;
-                const float w = (doc ? 1.f : Gates<E>::root(Gates<E>::square(s[i] * of_pair(r[j][i]), a[j][i]))) * (of_pair(g[j][i]) * px[j].get(i));
-                hs[i] = doc ? w : fmaf(a[j][i], hs[i], w);
+                const f2 vx = get2(in + j * kTile), a = decay(q[j]), G = add2(get2(in + 3 * kPart + j * kTile), e);
+                const f2 sr = each(r[j], of_pair), sg = each(g[j], of_pair), beta = doc ? both(1.f) : mul2(square(q[j]), inv[j]);
+                const f2 ox = mul2(mul2(G, beta), sg), og = mul2(mul2(ox, vx), each(g[j], rest_of_pair));
+                const f2 slope = fma2(w[j], both(-1.f), mul2(mul2(mul2(sg, vx), a), inv[j]));
+                const f2 dL = doc ? both(0.f) : mul2(mul2(G, a), slope);
+                const f2 oa = mul2(mul2(dL, mul2(s, sr)), each(r[j], rest_of_pair));
+                ds = fma2(dL, sr, ds);
+                e = doc ? both(0.f) : mul2(a, G);
+                const i64 at = (i64)(t + j) * p.C;
+                put2<PAIRS>(dx + at, ox, second);
+                put2<PAIRS>(dgx + at, og, second);
+                put2<PAIRS>(dga + at, oa, second);
             }
         }
-#pragma unroll
-        for (int j = L - 1; j >= 0; --j) {
-            if (t + j >= p.T) continue;
-            const bool doc = docs >> j & 1;
-            float ox[VEC], og[VEC], oa[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float sr = of_pair(r[j][i]), sg = of_pair(g[j][i]), len = s[i] * sr, v = Gates<E>::square(len, a[j][i]);
-                const float G = pdy[j].get(i) + e[i], u = sg * px[j].get(i), beta = doc ? 1.f : Gates<E>::root(v);
-                ox[i] = G * beta * sg;
-                og[i] = G * beta * u * rest_of_pair(g[j][i]);
-                const float dlen = doc ? 0.f : G * (u * (a[j][i] * a[j][i]) * Gates<E>::inverse_root(v) - a[j][i] * before[j][i]);
-                oa[i] = dlen * len * rest_of_pair(r[j][i]);
-                ds[i] += dlen * sr;
-                e[i] = doc ? 0.f : a[j][i] * G;
-            }
-            Pack<E, VEC> o;
-            const i64 at = (i64)(t + j) * p.C;
-            o.set(ox);
-            *reinterpret_cast<Pack<E, VEC>*>(dx + at) = o;
-            o.set(og);
-            *reinterpret_cast<Pack<E, VEC>*>(dgx + at) = o;
-            o.set(oa);
-            *reinterpret_cast<Pack<E, VEC>*>(dga + at) = o;
-        }
+        stage = stage == S - 1 ? 0 : stage + 1;
+        __syncwarp();
     }
-    if (p.dh0 != nullptr && warp == 0 && live) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) p.dh0[(i64)b * p.C + c0 + i] = carry[i];
+    if (p.dh0 != nullptr && rank == 0 && warp == 0 && live) {
+        p.dh0[row] = lo(carry);
+        if (second) p.dh0[row + 1] = hi(carry);
     }
     // the warps' shares of ds, in their order
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) sP[0][warp][lane * VEC + i] = ds[i];
+    shares[0][warp][lane] = make_ulonglong2(ds, 0);
     __syncthreads();
     if (warp == 0 && live) {
+        f2 sum = both(0.f);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            float sum = 0.f;
-#pragma unroll
-            for (int q = 0; q < kWarps; ++q) sum += sP[0][q][lane * VEC + i];
-            p.ds[(i64)b * p.C + c0 + i] = sum;
-        }
+        for (int q = 0; q < kWarps; ++q) sum = add2(sum, shares[0][q][lane].x);
+        float* to = p.ds + ((i64)b * K + rank) * p.C + c0;
+        to[0] = lo(sum);
+        if (second) to[1] = hi(sum);
     }
 }
 
@@ -411,8 +558,11 @@ __global__ void __launch_bounds__(128) scan_update_kernel(int B, int C, int pool
     for (int q = b; q < B; ++q) {
         if (q == b || slots[q] == slot) {
             const i64 i = (i64)q * C + c;
-            const float len = sc * sigmoid<E>(to_f(ga[i])), a = Gates<E>::exp_minus(len);
-            h = fmaf(a, h, Gates<E>::root(Gates<E>::square(len, a)) * (sigmoid<E>(to_f(gx[i])) * to_f(x[i])));
+            const f2 vga = both(to_f(ga[i])), vgx = both(to_f(gx[i]));
+            f2 ea, ex, ra, rx;
+            gates<E>(vga, vgx, ea, ex, ra, rx);
+            const f2 fallen = fall<E>(mul2(both(sc), sigmoid(vga, ea, ra)), false), v = square(fallen);
+            h = fmaf(lo(decay(fallen)), h, lo(mul2(v, inverse_root<E>(v))) * (lo(sigmoid(vgx, ex, rx)) * to_f(x[i])));
             y[i] = from_f<E>(h);
         }
         if (!later) break;
@@ -420,34 +570,63 @@ __global__ void __launch_bounds__(128) scan_update_kernel(int B, int C, int pool
     *at = h;
 }
 
-bool aligned(const void* p, int n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
-// Two channels a thread where a pair can be read as one word: C even and pointers aligned to it.
-bool pairs(const Args& p, int element) {
-    const int n = 2 * element;
-    return p.C % 2 == 0 && aligned(p.x, n) && aligned(p.gx, n) && aligned(p.ga, n) && aligned(p.y, n) && aligned(p.dy, n) && aligned(p.dx, n) &&
-           aligned(p.dgx, n) && aligned(p.dga, n);
-}
+bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 int check(const char* what, int dtype, int B, int T, int C) {
     RWKV_REQUIRE(dtype == RWKVB200_F32 || dtype == RWKVB200_BF16, RWKVB200_EINVAL, "%s: unknown dtype %d", what, dtype);
     RWKV_REQUIRE(B > 0 && T > 0 && C > 0, RWKVB200_EINVAL, "%s: B=%d T=%d C=%d must be positive", what, B, T, C);
-    RWKV_REQUIRE((i64)B * ((C + 31) / 32) <= 0x7fffffff, RWKVB200_EINVAL, "%s: B=%d C=%d: too many blocks", what, B, C);
-    RWKV_REQUIRE(T <= 0x7fffffff - 1024, RWKVB200_EINVAL, "%s: T=%d is too long", what, T);
+    RWKV_REQUIRE((i64)B * ((C + kTile - 1) / kTile) <= 0x7fffffff / kMaxCluster, RWKVB200_EINVAL, "%s: B=%d C=%d: too many blocks", what, B, C);
+    RWKV_REQUIRE(T <= 0x7fffffff - 65536, RWKVB200_EINVAL, "%s: T=%d is too long", what, T);
     return RWKVB200_OK;
 }
 
-template <typename E, int VEC>
-int run_forward(Args& p, int B, cudaStream_t st) {
-    p.tiles = (p.C + 32 * VEC - 1) / (32 * VEC);
-    scan_forward_kernel<E, VEC><<<(unsigned)(B * p.tiles), 32 * kWarps, 0, st>>>(p);
-    return check_launch("gated_scan_forward");
+// How many blocks share a (sequence, channel tile): the K for which the rounds that an SM's places go through one after the other are
+// fewest, a barrier of a cluster counting as a quarter of a round.
+int cluster_size(int units, int rounds, int places) {
+    int best = 1;
+    double least = 0;
+    for (int K = 1; K <= kMaxCluster; K *= 2) {
+        if (K > 1 && K > rounds) break;
+        const double cost = (double)(((i64)units * K + places - 1) / places) * ((rounds + K - 1) / K) * (K > 1 ? 1.25 : 1.0);
+        if (K == 1 || cost < least) best = K, least = cost;
+    }
+    return best;
 }
-template <typename E, int VEC>
-int run_backward(Args& p, int B, cudaStream_t st) {
-    p.tiles = (p.C + 32 * VEC - 1) / (32 * VEC);
-    scan_backward_kernel<E, VEC><<<(unsigned)(B * p.tiles), 32 * kWarps, 0, st>>>(p);
-    return check_launch("gated_scan_backward");
+
+template <auto Kernel>
+int launch(const char* what, const Args& p, int B, int K, int smem, cudaStream_t st) {
+    if (allow_smem<Kernel>(smem) != cudaSuccess) return check_launch(what);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((unsigned)(B * p.tiles * K));
+    config.blockDim = dim3(32 * kWarps);
+    config.dynamicSmemBytes = smem;
+    config.stream = st;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = K;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    cudaLaunchKernelEx(&config, Kernel, p);
+    return check_launch(what);
+}
+template <typename E>
+int run_forward(const Args& p, int B, int K, cudaStream_t st) {
+    const char* what = "gated_scan_forward";
+    const bool wide = p.C % (16 / sizeof(E)) == 0 && aligned(p.x, 16) && aligned(p.gx, 16) && aligned(p.ga, 16);
+    const bool pairs = p.C % 2 == 0 && aligned(p.y, 2 * sizeof(E));
+    constexpr int smem = fwd_smem<E>();
+    if (wide && pairs) return launch<scan_forward_kernel<E, true, true>>(what, p, B, K, smem, st);
+    return launch<scan_forward_kernel<E, false, false>>(what, p, B, K, smem, st);
+}
+template <typename E>
+int run_backward(const Args& p, int B, int K, cudaStream_t st) {
+    const char* what = "gated_scan_backward";
+    const bool wide = p.C % (16 / sizeof(E)) == 0 && aligned(p.x, 16) && aligned(p.gx, 16) && aligned(p.ga, 16) && aligned(p.dy, 16);
+    const bool pairs = p.C % 2 == 0 && aligned(p.dx, 2 * sizeof(E)) && aligned(p.dgx, 2 * sizeof(E)) && aligned(p.dga, 2 * sizeof(E));
+    constexpr int smem = bwd_smem<E>();
+    if (wide && pairs) return launch<scan_backward_kernel<E, true, true>>(what, p, B, K, smem, st);
+    return launch<scan_backward_kernel<E, false, false>>(what, p, B, K, smem, st);
 }
 
 }  // namespace
@@ -464,11 +643,11 @@ using namespace rwkvb200;
 
 extern "C" size_t rwkvb200_gated_scan_saved_bytes(int B, int T, int C) {
     if (B <= 0 || T <= 0 || C <= 0) return 0;
-    return (size_t)B * ((T + kSaved - 1) / kSaved) * C * sizeof(float);
+    return (size_t)B * ((T + kRound - 1) / kRound) * C * sizeof(float);
 }
 extern "C" size_t rwkvb200_gated_scan_work_bytes(int B, int T, int C) {
     if (B <= 0 || T <= 0 || C <= 0) return 0;
-    return (size_t)B * C * sizeof(float);
+    return (size_t)B * kMaxCluster * C * sizeof(float);
 }
 
 extern "C" int rwkvb200_gated_scan_forward(int dtype, int B, int T, int C, const float* h0, const void* x, const void* gx, const void* ga,
@@ -476,11 +655,11 @@ extern "C" int rwkvb200_gated_scan_forward(int dtype, int B, int T, int C, const
     if (int e = check("gated_scan_forward", dtype, B, T, C)) return e;
     RWKV_NOTNULL(x); RWKV_NOTNULL(gx); RWKV_NOTNULL(ga); RWKV_NOTNULL(s); RWKV_NOTNULL(y);
     Args p{};
-    p.T = T; p.C = C; p.rounds_saved = (T + kSaved - 1) / kSaved;
+    p.T = T; p.C = C; p.tiles = (C + kTile - 1) / kTile; p.rounds = (T + kRound - 1) / kRound;
     p.h0 = h0; p.x = x; p.gx = gx; p.ga = ga; p.s = s; p.first = first; p.y = y; p.hT = hT; p.saved = static_cast<float*>(saved);
     const cudaStream_t st = as_stream(stream);
-    if (dtype == RWKVB200_BF16) return pairs(p, 2) ? run_forward<bf16, 2>(p, B, st) : run_forward<bf16, 1>(p, B, st);
-    return pairs(p, 4) ? run_forward<float, 2>(p, B, st) : run_forward<float, 1>(p, B, st);
+    const int K = cluster_size(B * p.tiles, p.rounds, 2 * sm_count());
+    return dtype == RWKVB200_BF16 ? run_forward<bf16>(p, B, K, st) : run_forward<float>(p, B, K, st);
 }
 
 extern "C" int rwkvb200_gated_scan_backward(int dtype, int B, int T, int C, const void* x, const void* gx, const void* ga, const float* s,
@@ -490,15 +669,13 @@ extern "C" int rwkvb200_gated_scan_backward(int dtype, int B, int T, int C, cons
     RWKV_NOTNULL(x); RWKV_NOTNULL(gx); RWKV_NOTNULL(ga); RWKV_NOTNULL(s); RWKV_NOTNULL(saved); RWKV_NOTNULL(dy);
     RWKV_NOTNULL(dx); RWKV_NOTNULL(dgx); RWKV_NOTNULL(dga); RWKV_NOTNULL(ds); RWKV_NOTNULL(work);
     Args p{};
-    p.T = T; p.C = C; p.rounds_saved = (T + kSaved - 1) / kSaved;
+    p.T = T; p.C = C; p.tiles = (C + kTile - 1) / kTile; p.rounds = (T + kRound - 1) / kRound;
     p.x = x; p.gx = gx; p.ga = ga; p.s = s; p.first = first; p.saved = static_cast<float*>(const_cast<void*>(saved));
     p.dy = dy; p.dhT = dhT; p.dh0 = dh0; p.dx = dx; p.dgx = dgx; p.dga = dga; p.ds = static_cast<float*>(work);
     const cudaStream_t st = as_stream(stream);
-    int rc;
-    if (dtype == RWKVB200_BF16) rc = pairs(p, 2) ? run_backward<bf16, 2>(p, B, st) : run_backward<bf16, 1>(p, B, st);
-    else rc = pairs(p, 4) ? run_backward<float, 2>(p, B, st) : run_backward<float, 1>(p, B, st);
-    if (rc != RWKVB200_OK) return rc;
-    return sum_rows(RWKVB200_F32, B, C, p.ds, ds, st);
+    const int K = cluster_size(B * p.tiles, p.rounds, (dtype == RWKVB200_BF16 ? 2 : 1) * sm_count());
+    const int rc = dtype == RWKVB200_BF16 ? run_backward<bf16>(p, B, K, st) : run_backward<float>(p, B, K, st);
+    return rc != RWKVB200_OK ? rc : sum_rows(RWKVB200_F32, (i64)B * K, C, p.ds, ds, st);
 }
 
 extern "C" int rwkvb200_gated_scan_update(int dtype, int B, int C, int pool, float* state, const int* slots, const void* x, const void* gx,
