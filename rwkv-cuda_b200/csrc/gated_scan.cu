@@ -21,6 +21,7 @@
 // needs no barrier.  What bounds the kernels is in front of each.
 #include "packed.cuh"
 #include <cooperative_groups.h>
+#include <initializer_list>
 #include <type_traits>
 
 namespace rwkvb200 {
@@ -52,18 +53,31 @@ __device__ __forceinline__ float rsqrt_fast(float x) {
 
 // The functions behind the gates: for bf16 tensors the hardware approximations (2e-7 relative: 2^-14 of a step of bf16), for fp32
 // CUDA's exponential and one step of Newton's method behind the others.
+constexpr float kLog2e = 1.4426950408889634f;
 template <typename E> struct Fn;
 template <> struct Fn<bf16> {
-    static __device__ __forceinline__ float exp_minus(float x) { return ex2(-1.4426950408889634f * x); }
+    static __device__ __forceinline__ float exp_minus(float x) { return ex2(-kLog2e * x); }
+    static __device__ __forceinline__ f2 exp_minus(f2 x) {
+        float a, b;
+        unpack2(mul2(x, pack2(-kLog2e, -kLog2e)), a, b);
+        return pack2(ex2(a), ex2(b));
+    }
     static __device__ __forceinline__ float inverse(float x) { return rcp(x); }
+    static __device__ __forceinline__ float inverse_any(float x) { return rcp(x); }
     static __device__ __forceinline__ float inverse_root(float v) { return rsqrt_fast(v); }
 };
 template <> struct Fn<float> {
     static __device__ __forceinline__ float exp_minus(float x) { return expf(-x); }
-    static __device__ __forceinline__ float inverse(float x) {   // (of 1 to 4)
+    static __device__ __forceinline__ f2 exp_minus(f2 x) {
+        float a, b;
+        unpack2(x, a, b);
+        return pack2(expf(-a), expf(-b));
+    }
+    static __device__ __forceinline__ float inverse(float x) {   // (of finite values from 1 on)
         const float r = rcp(x);
         return fmaf(r, fmaf(-x, r, 1.f), r);
     }
+    static __device__ __forceinline__ float inverse_any(float x) { return 1.f / x; }
     static __device__ __forceinline__ float inverse_root(float v) {
         const float r = rsqrt_fast(v);
         return fmaf(0.5f * r, fmaf(-v * r, r, 1.f), r);
@@ -84,21 +98,22 @@ __device__ __forceinline__ float hi(f2 v) {
 template <typename F> __device__ __forceinline__ f2 each(f2 a, F f) { return pack2(f(lo(a)), f(hi(a))); }
 template <typename F> __device__ __forceinline__ f2 each(f2 a, f2 b, F f) { return pack2(f(lo(a), lo(b)), f(hi(a), hi(b))); }
 
-// 1 - exp(-L) of two channels, with all its digits where L is small: by its series for L / 8 (five terms leave (1/8)^5/720 = 4e-8),
-// doubled three times, 1 - a^2 = (1 - a) (2 - (1 - a)).  That serves L < 1 and takes no special function; beyond it the exponential.
-template <typename E>
-__device__ __forceinline__ f2 fall(f2 L, bool small) {
-    const f2 r = mul2(L, both(0.125f)), two = both(2.f), minus = both(-1.f);
-    f2 q = fma2(r, both(1.f / 120.f), both(-1.f / 24.f));
-    q = fma2(q, r, both(1.f / 6.f));
-    q = fma2(q, r, both(-0.5f));
-    q = fma2(q, r, both(1.f));
-    q = mul2(q, r);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) q = mul2(q, fma2(q, minus, two));
-    if (small) return q;   // (s <= 1 in all channels of the warp)
-    return each(L, q, [](float l, float p) { return l < 1.f ? p : 1.f - Fn<E>::exp_minus(l); });
+// 1 - exp(-L) of two channels, with all its digits where L is small: for L <= 1 as L times a polynomial (interpolation of
+// (1 - exp(-L)) / L at the Chebyshev points of [0, 1]: off by 3e-9, and by one unit of fp32 as it is evaluated), which takes no
+// special function; beyond by the exponential.  SMALL: s <= 1 in all channels of the warp.
+template <typename E, bool SMALL>
+__device__ __forceinline__ f2 fall(f2 L) {
+    f2 q = fma2(L, both(0.0001290763f), both(-0.001300775f));
+    q = fma2(q, L, both(0.008275505f));
+    q = fma2(q, L, both(-0.04164685f));
+    q = fma2(q, L, both(0.16666341f));
+    q = fma2(q, L, both(-0.4999998f));
+    q = fma2(q, L, both(1.f));
+    q = mul2(q, L);
+    if (SMALL) return q;
+    return each(L, q, [](float l, float p) { return l <= 1.f ? p : 1.f - Fn<E>::exp_minus(l); });
 }
+// 1 - a^2 = (1 - a) (2 - (1 - a))
 __device__ __forceinline__ f2 square(f2 q) { return mul2(q, fma2(q, both(-1.f), both(2.f))); }
 __device__ __forceinline__ f2 decay(f2 q) { return fma2(q, both(-1.f), both(1.f)); }
 // 1 / sqrt(1 - a^2); 0 below the normal numbers, where beta counts as 0 (and NaN below 0, which only a negative s makes)
@@ -107,52 +122,70 @@ __device__ __forceinline__ f2 inverse_root(f2 v) {
     return each(v, [](float x) { return fabsf(x) < 1.2e-38f ? 0.f : Fn<E>::inverse_root(x); });
 }
 
-// sigmoid(x) and 1 - sigmoid(x) without loss of either: m is the smaller of the two, with the sign of x in front of it
-__device__ __forceinline__ float of_pair(float m) { return __float_as_int(m) < 0 ? 1.f + m : m; }
-__device__ __forceinline__ float rest_of_pair(float m) { return __float_as_int(m) < 0 ? -m : 1.f - m; }
-// Both gates of two channels from one division: exp(-|x|) <= 1, so that no product overflows.
-template <typename E>
-__device__ __forceinline__ void gates(f2 ga, f2 gx, f2& ea, f2& ex, f2& ra, f2& rx) {
-    const f2 one = both(1.f);
-    ea = each(ga, [](float v) { return Fn<E>::exp_minus(fabsf(v)); });
-    ex = each(gx, [](float v) { return Fn<E>::exp_minus(fabsf(v)); });
-    const f2 da = add2(ea, one), dx = add2(ex, one);
-    const f2 r = each(mul2(da, dx), [](float v) { return Fn<E>::inverse(v); });
-    ra = mul2(r, dx);   // 1 / (1 + exp(-|ga|))
-    rx = mul2(r, da);
-}
-__device__ __forceinline__ f2 sigmoid(f2 x, f2 e, f2 r) {
-    const f2 m = mul2(e, r);
-    return pack2(lo(x) > 0.f ? lo(r) : lo(m), hi(x) > 0.f ? hi(r) : hi(m));
-}
-__device__ __forceinline__ f2 sigmoid_pair(f2 x, f2 e, f2 r) {
-    const f2 m = mul2(e, r);
-    return pack2(lo(x) > 0.f ? -lo(m) : lo(m), hi(x) > 0.f ? -hi(m) : hi(m));
-}
+// sigmoid(ga), sigmoid(gx) and what they lack of 1, without loss of either.  Two forms: as long as no gate is below kFast, so that
+// exp(-ga) exp(-gx) does not overflow, both come from one division; tiles with a gate that is (EXTREME) take one each.
+constexpr float kFast = -41.f;
+template <typename E, bool EXTREME>
+struct Gates {
+    f2 a, x, ea, ex;
+    f2 ga, gx;
+    __device__ __forceinline__ Gates(f2 ga, f2 gx) : ga(ga), gx(gx) {
+        const f2 one = both(1.f);
+        ea = Fn<E>::exp_minus(ga);
+        ex = Fn<E>::exp_minus(gx);
+        const f2 da = add2(ea, one), dx = add2(ex, one);
+        if (EXTREME) {
+            a = each(da, [](float v) { return Fn<E>::inverse_any(v); });
+            x = each(dx, [](float v) { return Fn<E>::inverse_any(v); });
+        } else {
+            const f2 r = each(mul2(da, dx), [](float v) { return Fn<E>::inverse(v); });
+            a = mul2(r, dx);
+            x = mul2(r, da);
+        }
+    }
+    static __device__ __forceinline__ f2 other(f2 g) {
+        return each(g, [](float v) { return Fn<E>::inverse_any(1.f + Fn<E>::exp_minus(-v)); });
+    }
+    __device__ __forceinline__ f2 rest_a() const { return EXTREME ? other(ga) : mul2(ea, a); }
+    __device__ __forceinline__ f2 rest_x() const { return EXTREME ? other(gx) : mul2(ex, x); }
+};
 
-// two neighbouring channels in shared memory, and back
-__device__ __forceinline__ f2 get2(const bf16* p) {
-    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
-    return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-__device__ __forceinline__ f2 get2(const float* p) {
-    const float2 w = *reinterpret_cast<const float2*>(p);
-    return pack2(w.x, w.y);
-}
+// two neighbouring channels as they lie in memory
+template <typename E> struct Pair;
+template <> struct Pair<bf16> {
+    __nv_bfloat162 v;
+    __device__ __forceinline__ explicit Pair(const bf16* p) : v(*reinterpret_cast<const __nv_bfloat162*>(p)) {}
+    __device__ __forceinline__ explicit Pair(float x) : v(__floats2bfloat162_rn(x, x)) {}
+    __device__ __forceinline__ f2 get() const {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(&v);
+        return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+    __device__ __forceinline__ void least(const Pair& o) { v = __hmin2(v, o.v); }
+    __device__ __forceinline__ bool below(float x) const { return fminf(__low2float(v), __high2float(v)) < x; }
+};
+template <> struct Pair<float> {
+    float2 v;
+    __device__ __forceinline__ explicit Pair(const float* p) : v(*reinterpret_cast<const float2*>(p)) {}
+    __device__ __forceinline__ explicit Pair(float x) : v(make_float2(x, x)) {}
+    __device__ __forceinline__ f2 get() const { return pack2(v.x, v.y); }
+    __device__ __forceinline__ void least(const Pair& o) { v.x = fminf(v.x, o.v.x), v.y = fminf(v.y, o.v.y); }
+    __device__ __forceinline__ bool below(float x) const { return fminf(v.x, v.y) < x; }
+};
+template <typename E> __device__ __forceinline__ f2 get2(const E* p) { return Pair<E>(p).get(); }
 // ... to global memory: as one word, or one after the other where C is odd or a tensor starts between two words
-template <bool PAIRS>
+template <bool WORD>
 __device__ __forceinline__ void put2(bf16* p, f2 v, bool second) {
     const __nv_bfloat162 t = __floats2bfloat162_rn(lo(v), hi(v));
-    if (PAIRS) {
+    if (WORD) {
         *reinterpret_cast<__nv_bfloat162*>(p) = t;
     } else {
         p[0] = t.x;
         if (second) p[1] = t.y;
     }
 }
-template <bool PAIRS>
+template <bool WORD>
 __device__ __forceinline__ void put2(float* p, f2 v, bool second) {
-    if (PAIRS) {
+    if (WORD) {
         *reinterpret_cast<float2*>(p) = make_float2(lo(v), hi(v));
     } else {
         p[0] = lo(v);
@@ -230,42 +263,33 @@ __device__ __forceinline__ f2 behind(f2 P, f2 before) {   // the product of two 
 struct Share {
     f2 P, H;
 };
-// All shares of the block in the order of time (backward: `reversed`): those before warp `warp` in `mine`, all of them in `all`.
+// What leaves the shares before warp `warp` (backward: those behind it, from the last one on) with the state `h`.
 template <bool REVERSED>
-__device__ __forceinline__ void fold(const ulonglong2 (*shares)[32], int warp, int lane, bool cuts, Share& mine, Share& all) {
-    Share a{both(1.f), both(0.f)};
-    if (!cuts) {
+__device__ __forceinline__ f2 through_block(const ulonglong2 (*shares)[32], int warp, int lane, bool cuts, f2 h) {
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i) {
-            const int q = REVERSED ? kWarps - 1 - i : i;
-            if (q == warp) mine = a;
-            const ulonglong2 v = shares[q][lane];
-            a.H = fma2(v.x, a.H, v.y);
-            a.P = mul2(a.P, v.x);
-        }
-        mine.P = clamp(mine.P);
-        a.P = clamp(a.P);
-    } else {
-#pragma unroll
-        for (int i = 0; i < kWarps; ++i) {
-            const int q = REVERSED ? kWarps - 1 - i : i;
-            if (q == warp) mine = a;
-            const ulonglong2 v = shares[q][lane];
-            a.H = step(v.x, v.y, a.H);
-            a.P = behind(v.x, a.P);
-        }
+    for (int i = 0; i < kWarps - 1; ++i) {
+        const int q = REVERSED ? kWarps - 1 - i : i;
+        if (REVERSED ? q <= warp : q >= warp) break;
+        const ulonglong2 v = shares[q][lane];
+        h = cuts ? step(v.x, v.y, h) : fma2(v.x, h, v.y);
     }
-    all = a;
+    return h;
 }
-// The state before this block's round and the one behind the rounds of all blocks of the cluster, from the state before them.
+// The state before this block's round, from the state before the rounds of all blocks of the cluster, which becomes the one behind them.
+// The shares of the blocks go through distributed shared memory: warp q brings this block's to block q.
 template <bool REVERSED>
-__device__ __forceinline__ f2 through_cluster(cg::cluster_group& cluster, int K, int rank, ulonglong2 (*peers)[32], const Share& all, int warp, int lane, f2& carry) {
-    if (K == 1) {
-        const f2 start = carry;
-        carry = step(all.P, all.H, carry);
-        return start;
+__device__ __forceinline__ f2 through_cluster(cg::cluster_group& cluster, int K, int rank, const ulonglong2 (*shares)[32], ulonglong2 (*peers)[32], int warp,
+                                              int lane, f2& carry) {
+    if (warp < K) {
+        Share all{both(1.f), both(0.f)};
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) {
+            const ulonglong2 v = shares[REVERSED ? kWarps - 1 - i : i][lane];
+            all.H = step(v.x, v.y, all.H);
+            all.P = behind(v.x, all.P);
+        }
+        *cluster.map_shared_rank(&peers[rank][lane], warp) = make_ulonglong2(all.P, all.H);
     }
-    if (warp < K) *cluster.map_shared_rank(&peers[rank][lane], warp) = make_ulonglong2(all.P, all.H);
     cluster.sync();
     f2 start = carry;
     for (int i = 0; i < K; ++i) {
@@ -282,14 +306,15 @@ constexpr int kBwdStages = 2;
 template <typename E> constexpr int fwd_smem() { return kFwdStages<E> * kWarps * 3 * kTokens * kTile * (int)sizeof(E); }
 template <typename E> constexpr int bwd_smem() { return kBwdStages * kWarps * 4 * kTokens * kTile * (int)sizeof(E); }
 
-template <typename E, bool WIDE, bool PAIRS>
+template <typename E, bool WIDE, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args p) {
     extern __shared__ __align__(16) unsigned char raw[];
-    __shared__ ulonglong2 shares[2][kWarps][32], peers[2][kMaxCluster][32];
+    __shared__ ulonglong2 shares[2][kWarps][32], peers[2][CLUSTER ? kMaxCluster : 1][32];
+    __shared__ f2 ends[2][32];   // the state behind a round (a lone block's)
     constexpr int S = kFwdStages<E>, kPart = kTokens * kTile;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     cg::cluster_group cluster = cg::this_cluster();
-    const int K = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), unit = blockIdx.x / K;
+    const int K = CLUSTER ? (int)cluster.num_blocks() : 1, rank = CLUSTER ? (int)cluster.block_rank() : 0, unit = blockIdx.x / K;
     const int b = unit / p.tiles, c_tile = unit % p.tiles * kTile, c0 = c_tile + lane * 2;
     const bool live = c0 < p.C, second = c0 + 1 < p.C;
     const i64 base = (i64)b * p.T * p.C + c_tile;
@@ -314,7 +339,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
     };
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) ask(rank + i * K, i);
-    if (K > 1) cluster.sync();   // (a block's shared memory is written by others once it has begun)
+    if (CLUSTER) cluster.sync();   // (a block's shared memory is written by others once it has begun)
+    else if (warp == kWarps - 1) ends[1][lane] = carry;
     int stage = 0, buf = 0;
     for (int r0 = 0; r0 < p.rounds; r0 += K, buf ^= 1) {   // (all blocks of a cluster go through the same barriers)
         const int round = r0 + rank, t = round * kRound + warp * kTokens;
@@ -324,54 +350,68 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
         const E* in = mine + stage * kWarps * 3 * kPart + lane * 2;
         const uint32_t docs = firsts(first, t, p.T, lane);
         f2 a[kTokens], w[kTokens];
-        Share mine_share{both(1.f), both(0.f)};
-        auto make = [&](auto plain) {   // plain: all tokens are there, and none begins a document
-            constexpr bool kPlain = decltype(plain)::value;
+        Share share;
+        Pair<E> least(0.f);
+        // simple: all tokens are there, none begins a document, and no gate is extreme
+        auto make = [&](auto is_simple, auto is_small) {
+            constexpr bool kSimple = decltype(is_simple)::value;
+            share.P = both(1.f);
+            share.H = both(0.f);
 #pragma unroll
             for (int j = 0; j < kTokens; ++j) {
-                const f2 vx = get2(in + j * kTile), vgx = get2(in + kPart + j * kTile), vga = get2(in + 2 * kPart + j * kTile);
-                f2 ea, ex, ra, rx;
-                gates<E>(vga, vgx, ea, ex, ra, rx);
-                const f2 q = fall<E>(mul2(s, sigmoid(vga, ea, ra)), small), v = square(q), u = mul2(sigmoid(vgx, ex, rx), vx);
-                f2 aj = decay(q), wj = mul2(mul2(v, inverse_root<E>(v)), u);
-                if (!kPlain) {
-                    if (docs >> j & 1) aj = both(0.f), wj = u;
-                    if (t + j >= p.T) aj = both(1.f), wj = both(0.f);
+                const Pair<E> vgx(in + kPart + j * kTile), vga(in + 2 * kPart + j * kTile);
+                const Gates<E, !kSimple> g(vga.get(), vgx.get());
+                if (kSimple) least.least(vga), least.least(vgx);
+                const f2 q = fall<E, decltype(is_small)::value>(mul2(s, g.a)), v = square(q), u = mul2(g.x, get2(in + j * kTile));
+                a[j] = decay(q);
+                // (v of 0 or below the normal numbers: beta is 0)
+                w[j] = kSimple ? mul2(mul2(v, each(v, [](float z) { return Fn<E>::inverse_root(fmaxf(z, 1.2e-38f)); })), u)
+                               : mul2(mul2(v, inverse_root<E>(v)), u);
+                if (!kSimple) {
+                    if (docs >> j & 1) a[j] = both(0.f), w[j] = u;
+                    if (t + j >= p.T) a[j] = both(1.f), w[j] = both(0.f);
                 }
-                a[j] = aj;
-                w[j] = wj;
-                if (kPlain) {
-                    mine_share.H = fma2(aj, mine_share.H, wj);
-                    mine_share.P = mul2(mine_share.P, aj);
-                } else {
-                    mine_share.H = docs >> j & 1 ? wj : fma2(aj, mine_share.H, wj);
-                    mine_share.P = mul2(mine_share.P, aj);
-                }
+                share.H = !kSimple && docs >> j & 1 ? w[j] : fma2(a[j], share.H, w[j]);
+                share.P = mul2(share.P, a[j]);
             }
-            mine_share.P = !kPlain && docs ? both(0.f) : clamp(mine_share.P);
+            share.P = !kSimple && docs ? both(0.f) : clamp(share.P);
         };
-        if (docs == 0 && t + kTokens <= p.T) make(std::true_type{}); else make(std::false_type{});
-        shares[buf][warp][lane] = make_ulonglong2(mine_share.P, mine_share.H);
+        bool simple = docs == 0 && t + kTokens <= p.T;
+        if (simple) {
+            if (small) make(std::true_type{}, std::true_type{}); else make(std::true_type{}, std::false_type{});
+            simple = !__any_sync(0xffffffffu, live && least.below(kFast));
+        }
+        if (!simple) make(std::false_type{}, std::false_type{});
+        shares[buf][warp][lane] = make_ulonglong2(share.P, share.H);
         const bool cuts = __syncthreads_or(docs != 0);   // (a buffer is written again two rounds on, behind the next barrier)
-        Share before, all;
-        fold<false>(shares[buf], warp, lane, cuts, before, all);
-        f2 h = through_cluster<false>(cluster, K, rank, peers[buf], all, warp, lane, carry);
-        h = step(before.P, before.H, h);
-        if (live && t < p.T) {
-            if (p.saved != nullptr && warp == 0) {
-                float* to = p.saved + ((i64)b * p.rounds + round) * p.C + c0;
-                to[0] = lo(h);
-                if (second) to[1] = hi(h);
-            }
+        f2 h = CLUSTER ? through_cluster<false>(cluster, K, rank, shares[buf], peers[buf], warp, lane, carry) : ends[buf ^ 1][lane];
+        if (p.saved != nullptr && warp == 0 && live && t < p.T) {
+            float* to = p.saved + ((i64)b * p.rounds + round) * p.C + c0;
+            to[0] = lo(h);
+            if (second) to[1] = hi(h);
+        }
+        h = through_block<false>(shares[buf], warp, lane, cuts, h);
+        E* to = y + (i64)t * p.C;
+        if (simple) {
 #pragma unroll
-            for (int j = 0; j < kTokens; ++j) {
-                if (t + j >= p.T) break;
+            for (int j = 0; j < kTokens; ++j, to += p.C) {
+                h = fma2(a[j], h, w[j]);
+                if (live) put2<WIDE>(to, h, second);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kTokens; ++j, to += p.C) {
                 h = docs >> j & 1 ? w[j] : fma2(a[j], h, w[j]);
-                put2<PAIRS>(y + (i64)(t + j) * p.C, h, second);
+                if (live && t + j < p.T) put2<WIDE>(to, h, second);
             }
         }
+        if (!CLUSTER && warp == kWarps - 1) ends[buf][lane] = h;
         stage = stage == S - 1 ? 0 : stage + 1;
         __syncwarp();
+    }
+    if (!CLUSTER) {
+        __syncthreads();
+        carry = ends[buf ^ 1][lane];
     }
     if (p.hT != nullptr && rank == 0 && warp == 0 && live) {
         p.hT[row] = lo(carry);
@@ -380,15 +420,17 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
 }
 
 // Rounds from the last to the first; e (the gradient that comes into a token from the later ones) goes the same way as h does in
-// the forward, with the same products of decays.  h before each token is made again from the saved states.
-template <typename E, bool WIDE, bool PAIRS>
+// the forward, with the same products of decays.  h before each token is made again from the saved states, and so are the gates
+// in the last walk: keeping them would take more registers than two blocks per SM have, and about as many instructions.
+template <typename E, bool WIDE, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_backward_kernel(const Args p) {
     extern __shared__ __align__(16) unsigned char raw[];
-    __shared__ ulonglong2 shares[2][kWarps][32], forward[2][kWarps][32], peers[2][kMaxCluster][32];
+    __shared__ ulonglong2 shares[2][kWarps][32], peers[2][CLUSTER ? kMaxCluster : 1][32];
+    __shared__ f2 forward[2][kWarps][32], ends[2][32];
     constexpr int S = kBwdStages, kPart = kTokens * kTile;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     cg::cluster_group cluster = cg::this_cluster();
-    const int K = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), unit = blockIdx.x / K;
+    const int K = CLUSTER ? (int)cluster.num_blocks() : 1, rank = CLUSTER ? (int)cluster.block_rank() : 0, unit = blockIdx.x / K;
     const int b = unit / p.tiles, c_tile = unit % p.tiles * kTile, c0 = c_tile + lane * 2;
     const bool live = c0 < p.C, second = c0 + 1 < p.C;
     const i64 base = (i64)b * p.T * p.C + c_tile;
@@ -416,7 +458,8 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
     const int turns = (p.rounds + K - 1) / K;
 #pragma unroll
     for (int i = 0; i < S - 1; ++i) ask((turns - 1 - i) * K + rank, i);
-    if (K > 1) cluster.sync();
+    if (CLUSTER) cluster.sync();
+    else if (warp == 0) ends[1][lane] = carry;
     int stage = 0, buf = 0;
     for (int turn = turns - 1; turn >= 0; --turn, buf ^= 1) {
         const int round = turn * K + rank, t = round * kRound + warp * kTokens;
@@ -430,91 +473,105 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
         __syncwarp();
         const E* in = mine + stage * kWarps * 4 * kPart + lane * 2;
         const uint32_t docs = firsts(first, t, p.T, lane);
-        // per token: 1 - a, the gates as pairs, 1 / beta, and w = beta u, which makes room for h before the token
-        f2 q[kTokens], r[kTokens], g[kTokens], inv[kTokens], w[kTokens], P = both(1.f), H = both(0.f), Q = both(0.f);
-        auto make = [&](auto plain) {
-            constexpr bool kPlain = decltype(plain)::value;
+        // per token: 1 - a, 1 / beta, and w = beta u, which makes room for h before the token
+        f2 q[kTokens], inv[kTokens], w[kTokens], P, H, Q;
+        Pair<E> least(0.f);
+        auto make = [&](auto is_simple, auto is_small) {
+            constexpr bool kSimple = decltype(is_simple)::value;
+            P = both(1.f);
+            H = Q = both(0.f);
 #pragma unroll
             for (int j = 0; j < kTokens; ++j) {
-                const f2 vx = get2(in + j * kTile), vgx = get2(in + kPart + j * kTile), vga = get2(in + 2 * kPart + j * kTile);
-                f2 ea, ex, ra, rx;
-                gates<E>(vga, vgx, ea, ex, ra, rx);
-                r[j] = sigmoid_pair(vga, ea, ra);
-                g[j] = sigmoid_pair(vgx, ex, rx);
-                q[j] = fall<E>(mul2(s, sigmoid(vga, ea, ra)), small);
-                const f2 v = square(q[j]), u = mul2(sigmoid(vgx, ex, rx), vx);
+                const Pair<E> vgx(in + kPart + j * kTile), vga(in + 2 * kPart + j * kTile);
+                const Gates<E, !kSimple> g(vga.get(), vgx.get());
+                if (kSimple) least.least(vga), least.least(vgx);
+                q[j] = fall<E, decltype(is_small)::value>(mul2(s, g.a));
+                const f2 v = square(q[j]), u = mul2(g.x, get2(in + j * kTile));
                 inv[j] = inverse_root<E>(v);
                 w[j] = mul2(mul2(v, inv[j]), u);
-                if (!kPlain) {
+                if (!kSimple) {
                     if (docs >> j & 1) q[j] = both(1.f), inv[j] = both(0.f), w[j] = u;
                     if (t + j >= p.T) q[j] = both(0.f), w[j] = both(0.f);
                 }
                 const f2 a = decay(q[j]);
-                H = !kPlain && docs >> j & 1 ? w[j] : fma2(a, H, w[j]);
+                H = !kSimple && docs >> j & 1 ? w[j] : fma2(a, H, w[j]);
                 P = mul2(P, a);
             }
 #pragma unroll
             for (int j = kTokens - 1; j >= 0; --j) {
-                if (kPlain) {
+                if (kSimple) {
                     Q = mul2(decay(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
                 } else if (t + j < p.T) {
                     Q = docs >> j & 1 ? both(0.f) : mul2(decay(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
                 }
             }
-            P = !kPlain && docs ? both(0.f) : clamp(P);
+            P = !kSimple && docs ? both(0.f) : clamp(P);
         };
-        if (docs == 0 && t + kTokens <= p.T) make(std::true_type{}); else make(std::false_type{});
-        shares[buf][warp][lane] = make_ulonglong2(P, Q);
-        forward[buf][warp][lane] = make_ulonglong2(P, H);
-        const bool cuts = __syncthreads_or(docs != 0);
-        Share after, all;
-        fold<true>(shares[buf], warp, lane, cuts, after, all);
-        f2 e = through_cluster<true>(cluster, K, rank, peers[buf], all, warp, lane, carry);
-        e = step(after.P, after.H, e);
-        for (int i = 0; i < warp; ++i) {
-            const ulonglong2 v = forward[buf][i][lane];
-            h = step(v.x, v.y, h);
+        bool simple = docs == 0 && t + kTokens <= p.T;
+        if (simple) {
+            if (small) make(std::true_type{}, std::true_type{}); else make(std::true_type{}, std::false_type{});
+            simple = !__any_sync(0xffffffffu, live && least.below(kFast));
         }
-        if (live && t < p.T) {
+        if (!simple) make(std::false_type{}, std::false_type{});
+        shares[buf][warp][lane] = make_ulonglong2(P, Q);
+        forward[buf][warp][lane] = H;
+        const bool cuts = __syncthreads_or(docs != 0);
+        f2 e = CLUSTER ? through_cluster<true>(cluster, K, rank, shares[buf], peers[buf], warp, lane, carry) : ends[buf ^ 1][lane];
+        e = through_block<true>(shares[buf], warp, lane, cuts, e);
+#pragma unroll
+        for (int i = 0; i < kWarps - 1; ++i) {
+            if (i >= warp) break;
+            h = step(shares[buf][i][lane].x, forward[buf][i][lane], h);
+        }
+        auto walk = [&](auto is_simple) {
+            constexpr bool kSimple = decltype(is_simple)::value;
 #pragma unroll
             for (int j = 0; j < kTokens; ++j) {
                 const f2 before = h;
-                h = docs >> j & 1 ? w[j] : fma2(decay(q[j]), h, w[j]);
+                h = !kSimple && docs >> j & 1 ? w[j] : fma2(decay(q[j]), h, w[j]);
                 w[j] = before;
             }
+            i64 at = (i64)(t + kTokens) * p.C;
 #pragma unroll
             for (int j = kTokens - 1; j >= 0; --j) {
-                if (t + j >= p.T) continue;
-                const bool doc = docs >> j & 1;
+                at -= p.C;
+                if (!kSimple && t + j >= p.T) continue;
+                const bool doc = !kSimple && docs >> j & 1;
+                const Gates<E, !kSimple> g(get2(in + 2 * kPart + j * kTile), get2(in + kPart + j * kTile));
                 const f2 vx = get2(in + j * kTile), a = decay(q[j]), G = add2(get2(in + 3 * kPart + j * kTile), e);
-                const f2 sr = each(r[j], of_pair), sg = each(g[j], of_pair), beta = doc ? both(1.f) : mul2(square(q[j]), inv[j]);
-                const f2 ox = mul2(mul2(G, beta), sg), og = mul2(mul2(ox, vx), each(g[j], rest_of_pair));
-                const f2 slope = fma2(w[j], both(-1.f), mul2(mul2(mul2(sg, vx), a), inv[j]));
-                const f2 dL = doc ? both(0.f) : mul2(mul2(G, a), slope);
-                const f2 oa = mul2(mul2(dL, mul2(s, sr)), each(r[j], rest_of_pair));
-                ds = fma2(dL, sr, ds);
-                e = doc ? both(0.f) : mul2(a, G);
-                const i64 at = (i64)(t + j) * p.C;
-                put2<PAIRS>(dx + at, ox, second);
-                put2<PAIRS>(dgx + at, og, second);
-                put2<PAIRS>(dga + at, oa, second);
+                const f2 beta = doc ? both(1.f) : mul2(square(q[j]), inv[j]);
+                const f2 ox = mul2(mul2(G, beta), g.x), og = mul2(mul2(ox, vx), g.rest_x());
+                e = mul2(a, G);
+                const f2 slope = fma2(w[j], both(-1.f), mul2(mul2(mul2(g.x, vx), a), inv[j]));
+                f2 dL = mul2(e, slope);
+                if (doc) e = dL = both(0.f);
+                const f2 oa = mul2(mul2(dL, mul2(s, g.a)), g.rest_a());
+                ds = fma2(dL, g.a, ds);
+                if (live) {
+                    put2<WIDE>(dx + at, ox, second);
+                    put2<WIDE>(dgx + at, og, second);
+                    put2<WIDE>(dga + at, oa, second);
+                }
             }
-        }
+        };
+        if (simple) walk(std::true_type{}); else walk(std::false_type{});
+        if (!CLUSTER && warp == 0) ends[buf][lane] = e;
         stage = stage == S - 1 ? 0 : stage + 1;
         __syncwarp();
     }
+    // the warps' shares of ds, in their order
+    __syncthreads();
+    if (!CLUSTER) carry = ends[buf ^ 1][lane];
     if (p.dh0 != nullptr && rank == 0 && warp == 0 && live) {
         p.dh0[row] = lo(carry);
         if (second) p.dh0[row + 1] = hi(carry);
     }
-    // the warps' shares of ds, in their order
-    __syncthreads();
-    shares[0][warp][lane] = make_ulonglong2(ds, 0);
+    forward[0][warp][lane] = ds;
     __syncthreads();
     if (warp == 0 && live) {
         f2 sum = both(0.f);
 #pragma unroll
-        for (int q = 0; q < kWarps; ++q) sum = add2(sum, shares[0][q][lane].x);
+        for (int q = 0; q < kWarps; ++q) sum = add2(sum, forward[0][q][lane]);
         float* to = p.ds + ((i64)b * K + rank) * p.C + c0;
         to[0] = lo(sum);
         if (second) to[1] = hi(sum);
@@ -558,11 +615,9 @@ __global__ void __launch_bounds__(128) scan_update_kernel(int B, int C, int pool
     for (int q = b; q < B; ++q) {
         if (q == b || slots[q] == slot) {
             const i64 i = (i64)q * C + c;
-            const f2 vga = both(to_f(ga[i])), vgx = both(to_f(gx[i]));
-            f2 ea, ex, ra, rx;
-            gates<E>(vga, vgx, ea, ex, ra, rx);
-            const f2 fallen = fall<E>(mul2(both(sc), sigmoid(vga, ea, ra)), false), v = square(fallen);
-            h = fmaf(lo(decay(fallen)), h, lo(mul2(v, inverse_root<E>(v))) * (lo(sigmoid(vgx, ex, rx)) * to_f(x[i])));
+            const Gates<E, true> g(both(to_f(ga[i])), both(to_f(gx[i])));
+            const f2 fallen = fall<E, false>(mul2(both(sc), g.a)), v = square(fallen);
+            h = fmaf(lo(decay(fallen)), h, lo(mul2(v, inverse_root<E>(v))) * (lo(g.x) * to_f(x[i])));
             y[i] = from_f<E>(h);
         }
         if (!later) break;
@@ -570,7 +625,11 @@ __global__ void __launch_bounds__(128) scan_update_kernel(int B, int C, int pool
     *at = h;
 }
 
-bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+bool aligned(std::initializer_list<const void*> ps) {
+    uintptr_t all = 0;
+    for (const void* p : ps) all |= reinterpret_cast<uintptr_t>(p);
+    return all % 16 == 0;
+}
 
 int check(const char* what, int dtype, int B, int T, int C) {
     RWKV_REQUIRE(dtype == RWKVB200_F32 || dtype == RWKVB200_BF16, RWKVB200_EINVAL, "%s: unknown dtype %d", what, dtype);
@@ -613,20 +672,19 @@ int launch(const char* what, const Args& p, int B, int K, int smem, cudaStream_t
 template <typename E>
 int run_forward(const Args& p, int B, int K, cudaStream_t st) {
     const char* what = "gated_scan_forward";
-    const bool wide = p.C % (16 / sizeof(E)) == 0 && aligned(p.x, 16) && aligned(p.gx, 16) && aligned(p.ga, 16);
-    const bool pairs = p.C % 2 == 0 && aligned(p.y, 2 * sizeof(E));
+    // 16 bytes a copy where every row starts on such a boundary; else element by element
+    const bool wide = p.C % (16 / sizeof(E)) == 0 && aligned({p.x, p.gx, p.ga, p.y});
     constexpr int smem = fwd_smem<E>();
-    if (wide && pairs) return launch<scan_forward_kernel<E, true, true>>(what, p, B, K, smem, st);
-    return launch<scan_forward_kernel<E, false, false>>(what, p, B, K, smem, st);
+    if (wide) return K > 1 ? launch<scan_forward_kernel<E, true, true>>(what, p, B, K, smem, st) : launch<scan_forward_kernel<E, true, false>>(what, p, B, 1, smem, st);
+    return K > 1 ? launch<scan_forward_kernel<E, false, true>>(what, p, B, K, smem, st) : launch<scan_forward_kernel<E, false, false>>(what, p, B, 1, smem, st);
 }
 template <typename E>
 int run_backward(const Args& p, int B, int K, cudaStream_t st) {
     const char* what = "gated_scan_backward";
-    const bool wide = p.C % (16 / sizeof(E)) == 0 && aligned(p.x, 16) && aligned(p.gx, 16) && aligned(p.ga, 16) && aligned(p.dy, 16);
-    const bool pairs = p.C % 2 == 0 && aligned(p.dx, 2 * sizeof(E)) && aligned(p.dgx, 2 * sizeof(E)) && aligned(p.dga, 2 * sizeof(E));
+    const bool wide = p.C % (16 / sizeof(E)) == 0 && aligned({p.x, p.gx, p.ga, p.dy, p.dx, p.dgx, p.dga});
     constexpr int smem = bwd_smem<E>();
-    if (wide && pairs) return launch<scan_backward_kernel<E, true, true>>(what, p, B, K, smem, st);
-    return launch<scan_backward_kernel<E, false, false>>(what, p, B, K, smem, st);
+    if (wide) return K > 1 ? launch<scan_backward_kernel<E, true, true>>(what, p, B, K, smem, st) : launch<scan_backward_kernel<E, true, false>>(what, p, B, 1, smem, st);
+    return K > 1 ? launch<scan_backward_kernel<E, false, true>>(what, p, B, K, smem, st) : launch<scan_backward_kernel<E, false, false>>(what, p, B, 1, smem, st);
 }
 
 }  // namespace
