@@ -10,8 +10,8 @@
 //
 // (dL = 0 at a document's first token; where L = 0 the term through beta is taken as 0.)
 //
-// A block owns 32 lanes x 2 channels of one sequence and goes through it in rounds of kWarps x kTokens tokens, a warp owns
-// kTokens of them: it makes the gates of its tokens in registers, reduces them to (P, H) (the product of the decays and the end
+// A block owns 32 lanes x 2 channels of one sequence and goes through it in rounds of kWarps x 16 (backward: 8) tokens, a warp
+// owns 16 of them: it makes the gates of its tokens in registers, reduces them to (P, H) (the product of the decays and the end
 // state from a zero start), all warps fold those of the warps before theirs onto the block's state, and each walks its tokens
 // once more from its own start state.  Every input is read once, y is written once.  Where there are few (sequence, channel)
 // blocks, a cluster of blocks shares the rounds: block k of K takes rounds k, k + K, ..., and the (P, H) of their rounds go
@@ -30,8 +30,9 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kWarps = 8;
-constexpr int kTokens = 8;                   // per warp and round
-constexpr int kRound = kWarps * kTokens;     // the forward saves the state before every round for the backward
+template <typename E> constexpr int kFwdTokens = sizeof(E) == 2 ? 16 : 8;   // per warp and round: what fits two blocks per SM
+constexpr int kBwdTokens = 8;                // (three values per token and channel to keep instead of two)
+constexpr int kSaved = kWarps * kBwdTokens;  // the forward saves the state before every round of the backward
 constexpr int kTile = 64;                    // channels of a block
 constexpr int kMaxCluster = 8;
 
@@ -194,7 +195,7 @@ __device__ __forceinline__ void put2(float* p, f2 v, bool second) {
 }
 
 struct Args {
-    int T, C, tiles, rounds;   // channel tiles, rounds of kRound tokens
+    int T, C, tiles, rounds, saves;   // channel tiles, rounds of the kernel, of the backward
     const float* h0;
     const void *x, *gx, *ga;
     const float* s;
@@ -211,37 +212,59 @@ struct Args {
 };
 
 // which of a warp's tokens from t on begin a document, a bit each
+template <int L>
 __device__ __forceinline__ uint32_t firsts(const uint8_t* first, int t, int T, int lane) {
     if (first == nullptr) return 0;
-    const bool f = lane < kTokens && t + lane < T && first[t + lane] != 0;
+    const bool f = lane < L && t + lane < T && first[t + lane] != 0;
     return __ballot_sync(0xffffffffu, f);
 }
 
-// The [kTokens][kTile] tile of a tensor from token t on: to shared memory, without waiting.  WIDE: every row of C starts on a 16-byte
+// Tiles of N tensors, [L][kTile] each, from token t on: to shared memory, without waiting.  WIDE: every row of C starts on a 16-byte
 // boundary, and a piece of 16 bytes is asked for at a time; else element by element, at once.  What lies outside is left alone.
-template <typename E, bool WIDE>
-__device__ __forceinline__ void fetch(E* tile, const E* from, int t, int T, int C, int c_tile, int lane) {
-    if (WIDE) {
-        constexpr int n = 16 / sizeof(E), row = kTile / n;   // pieces of a row
+template <typename E, bool WIDE, int L, int N>
+struct Fetch {
+    static constexpr int n = 16 / sizeof(E), kRow = kTile / n, kRows = 32 / kRow;   // elements of a piece, pieces of a row, rows at a time
+    const E* from[N];
+    int T, C, row, lane;
+    i64 at;        // of this lane's first piece
+    bool inside;   // its channels
+    __device__ __forceinline__ Fetch(int T, int C, int c_tile, int lane) : T(T), C(C), row(lane / kRow), lane(lane) {
+        const int c = lane % kRow * n;
+        at = (i64)row * C + c;
+        inside = c_tile + c < C;
+    }
+    __device__ __forceinline__ void operator()(E* to, int t, int c_tile) const {
+        if (WIDE) {
+            const uint32_t shared = (uint32_t)__cvta_generic_to_shared(to) + lane * 16;
+            const i64 first = (i64)t * C + at, step = (i64)kRows * C;
+            if (t + L <= T) {
+                if (inside) {
 #pragma unroll
-        for (int i = 0; i < kTokens * row / 32; ++i) {
-            const int piece = i * 32 + lane, j = piece / row, c = piece % row * n;
-            if (t + j < T && c_tile + c < C) {
-                const uint32_t to = (uint32_t)__cvta_generic_to_shared(tile + j * kTile + c);
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from + (i64)(t + j) * C + c) : "memory");
+                    for (int k = 0; k < N; ++k) {
+                        const E* p = from[k] + first;
+#pragma unroll
+                        for (int i = 0; i < L / kRows; ++i, p += step) copy(shared + (k * L + i * kRows) * kTile * (int)sizeof(E), p);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+#pragma unroll
+                    for (int i = 0; i < L / kRows; ++i)
+                        if (inside && t + i * kRows + row < T) copy(shared + (k * L + i * kRows) * kTile * (int)sizeof(E), from[k] + first + i * step);
             }
-        }
-    } else {
+        } else {
 #pragma unroll
-        for (int j = 0; j < kTokens; ++j) {
+            for (int k = 0; k < N; ++k)
+#pragma unroll 4
+                for (int j = 0; j < L; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int c = i * 32 + lane;
-                if (t + j < T && c_tile + c < C) tile[j * kTile + c] = from[(i64)(t + j) * C + c];
-            }
+                    for (int c = lane; c < kTile; c += 32)
+                        if (t + j < T) to[(k * L + j) * kTile + c] = c_tile + c < C ? from[k][(i64)(t + j) * C + c] : from_f<E>(0.f);
         }
     }
-}
+    static __device__ __forceinline__ void copy(uint32_t to, const E* p) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p) : "memory"); }
+};
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void wait_group() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
@@ -266,13 +289,16 @@ struct Share {
 // What leaves the shares before warp `warp` (backward: those behind it, from the last one on) with the state `h`.
 template <bool REVERSED>
 __device__ __forceinline__ f2 through_block(const ulonglong2 (*shares)[32], int warp, int lane, bool cuts, f2 h) {
+    auto walk = [&](auto plain) {
 #pragma unroll
-    for (int i = 0; i < kWarps - 1; ++i) {
-        const int q = REVERSED ? kWarps - 1 - i : i;
-        if (REVERSED ? q <= warp : q >= warp) break;
-        const ulonglong2 v = shares[q][lane];
-        h = cuts ? step(v.x, v.y, h) : fma2(v.x, h, v.y);
-    }
+        for (int i = 0; i < kWarps - 1; ++i) {
+            const int q = REVERSED ? kWarps - 1 - i : i;
+            if (REVERSED ? q <= warp : q >= warp) break;
+            const ulonglong2 v = shares[q][lane];
+            h = decltype(plain)::value ? fma2(v.x, h, v.y) : step(v.x, v.y, h);
+        }
+    };
+    if (cuts) walk(std::false_type{}); else walk(std::true_type{});
     return h;
 }
 // The state before this block's round, from the state before the rounds of all blocks of the cluster, which becomes the one behind them.
@@ -301,24 +327,31 @@ __device__ __forceinline__ f2 through_cluster(cg::cluster_group& cluster, int K,
     return start;
 }
 
-template <typename E> constexpr int kFwdStages = sizeof(E) == 2 ? 3 : 2;
+constexpr int kFwdStages = 2;
 constexpr int kBwdStages = 2;
-template <typename E> constexpr int fwd_smem() { return kFwdStages<E> * kWarps * 3 * kTokens * kTile * (int)sizeof(E); }
-template <typename E> constexpr int bwd_smem() { return kBwdStages * kWarps * 4 * kTokens * kTile * (int)sizeof(E); }
+template <typename E> constexpr int fwd_smem() { return kFwdStages * kWarps * 3 * kFwdTokens<E> * kTile * (int)sizeof(E); }
+template <typename E> constexpr int bwd_smem() { return kBwdStages * kWarps * 4 * kBwdTokens * kTile * (int)sizeof(E); }
+
+// A warp's tile: all tokens are there and none begins a document; or not; or some gate is below kFast (found on the way)
+enum { kSimpleTile, kDocumentTile, kExtremeTile };
+template <int M> using Mode = std::integral_constant<int, M>;
 
 template <typename E, bool WIDE, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args p) {
     extern __shared__ __align__(16) unsigned char raw[];
     __shared__ ulonglong2 shares[2][kWarps][32], peers[2][CLUSTER ? kMaxCluster : 1][32];
     __shared__ f2 ends[2][32];   // the state behind a round (a lone block's)
-    constexpr int S = kFwdStages<E>, kPart = kTokens * kTile;
+    constexpr int S = kFwdStages, kTokens = kFwdTokens<E>, kRound = kWarps * kTokens, kPart = kTokens * kTile;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     cg::cluster_group cluster = cg::this_cluster();
     const int K = CLUSTER ? (int)cluster.num_blocks() : 1, rank = CLUSTER ? (int)cluster.block_rank() : 0, unit = blockIdx.x / K;
     const int b = unit / p.tiles, c_tile = unit % p.tiles * kTile, c0 = c_tile + lane * 2;
     const bool live = c0 < p.C, second = c0 + 1 < p.C;
     const i64 base = (i64)b * p.T * p.C + c_tile;
-    const E *x = static_cast<const E*>(p.x) + base, *gx = static_cast<const E*>(p.gx) + base, *ga = static_cast<const E*>(p.ga) + base;
+    Fetch<E, WIDE, kTokens, 3> fetch(p.T, p.C, c_tile, lane);
+    fetch.from[0] = static_cast<const E*>(p.x) + base;
+    fetch.from[1] = static_cast<const E*>(p.gx) + base;
+    fetch.from[2] = static_cast<const E*>(p.ga) + base;
     E* y = static_cast<E*>(p.y) + base + lane * 2;
     E* mine = reinterpret_cast<E*>(raw) + warp * 3 * kPart;
     const uint8_t* first = p.first ? p.first + (i64)b * p.T : nullptr;
@@ -329,12 +362,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
 
     auto ask = [&](int round, int stage) {
         const int t = round * kRound + warp * kTokens;
-        E* to = mine + stage * kWarps * 3 * kPart;
-        if (t < p.T) {
-            fetch<E, WIDE>(to, x, t, p.T, p.C, c_tile, lane);
-            fetch<E, WIDE>(to + kPart, gx, t, p.T, p.C, c_tile, lane);
-            fetch<E, WIDE>(to + 2 * kPart, ga, t, p.T, p.C, c_tile, lane);
-        }
+        if (t < p.T) fetch(mine + stage * kWarps * 3 * kPart, t, c_tile);
         commit();
     };
 #pragma unroll
@@ -348,20 +376,19 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
         wait_group<S - 1>();
         __syncwarp();
         const E* in = mine + stage * kWarps * 3 * kPart + lane * 2;
-        const uint32_t docs = firsts(first, t, p.T, lane);
+        const uint32_t docs = firsts<kTokens>(first, t, p.T, lane);
         f2 a[kTokens], w[kTokens];
         Share share;
         Pair<E> least(0.f);
-        // simple: all tokens are there, none begins a document, and no gate is extreme
-        auto make = [&](auto is_simple, auto is_small) {
-            constexpr bool kSimple = decltype(is_simple)::value;
+        auto make = [&](auto mode, auto is_small) {
+            constexpr bool kSimple = decltype(mode)::value == kSimpleTile, kExtreme = decltype(mode)::value == kExtremeTile;
             share.P = both(1.f);
             share.H = both(0.f);
 #pragma unroll
             for (int j = 0; j < kTokens; ++j) {
                 const Pair<E> vgx(in + kPart + j * kTile), vga(in + 2 * kPart + j * kTile);
-                const Gates<E, !kSimple> g(vga.get(), vgx.get());
-                if (kSimple) least.least(vga), least.least(vgx);
+                const Gates<E, kExtreme> g(vga.get(), vgx.get());
+                if (!kExtreme && (kSimple || t + j < p.T)) least.least(vga), least.least(vgx);   // (other rows hold anything)
                 const f2 q = fall<E, decltype(is_small)::value>(mul2(s, g.a)), v = square(q), u = mul2(g.x, get2(in + j * kTile));
                 a[j] = decay(q);
                 // (v of 0 or below the normal numbers: beta is 0)
@@ -376,23 +403,25 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
             }
             share.P = !kSimple && docs ? both(0.f) : clamp(share.P);
         };
-        bool simple = docs == 0 && t + kTokens <= p.T;
-        if (simple) {
-            if (small) make(std::true_type{}, std::true_type{}); else make(std::true_type{}, std::false_type{});
-            simple = !__any_sync(0xffffffffu, live && least.below(kFast));
+        int mode = docs == 0 && t + kTokens <= p.T ? kSimpleTile : kDocumentTile;
+        if (mode == kDocumentTile) make(Mode<kDocumentTile>{}, std::false_type{});
+        else if (small) make(Mode<kSimpleTile>{}, std::true_type{});
+        else make(Mode<kSimpleTile>{}, std::false_type{});
+        if (__any_sync(0xffffffffu, live && least.below(kFast))) {
+            mode = kExtremeTile;
+            make(Mode<kExtremeTile>{}, std::false_type{});
         }
-        if (!simple) make(std::false_type{}, std::false_type{});
         shares[buf][warp][lane] = make_ulonglong2(share.P, share.H);
         const bool cuts = __syncthreads_or(docs != 0);   // (a buffer is written again two rounds on, behind the next barrier)
         f2 h = CLUSTER ? through_cluster<false>(cluster, K, rank, shares[buf], peers[buf], warp, lane, carry) : ends[buf ^ 1][lane];
-        if (p.saved != nullptr && warp == 0 && live && t < p.T) {
-            float* to = p.saved + ((i64)b * p.rounds + round) * p.C + c0;
+        h = through_block<false>(shares[buf], warp, lane, cuts, h);
+        if (p.saved != nullptr && t % kSaved == 0 && live && t < p.T) {
+            float* to = p.saved + ((i64)b * p.saves + t / kSaved) * p.C + c0;
             to[0] = lo(h);
             if (second) to[1] = hi(h);
         }
-        h = through_block<false>(shares[buf], warp, lane, cuts, h);
         E* to = y + (i64)t * p.C;
-        if (simple) {
+        if (mode == kSimpleTile) {
 #pragma unroll
             for (int j = 0; j < kTokens; ++j, to += p.C) {
                 h = fma2(a[j], h, w[j]);
@@ -427,15 +456,18 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
     extern __shared__ __align__(16) unsigned char raw[];
     __shared__ ulonglong2 shares[2][kWarps][32], peers[2][CLUSTER ? kMaxCluster : 1][32];
     __shared__ f2 forward[2][kWarps][32], ends[2][32];
-    constexpr int S = kBwdStages, kPart = kTokens * kTile;
+    constexpr int S = kBwdStages, kTokens = kBwdTokens, kRound = kWarps * kTokens, kPart = kTokens * kTile;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     cg::cluster_group cluster = cg::this_cluster();
     const int K = CLUSTER ? (int)cluster.num_blocks() : 1, rank = CLUSTER ? (int)cluster.block_rank() : 0, unit = blockIdx.x / K;
     const int b = unit / p.tiles, c_tile = unit % p.tiles * kTile, c0 = c_tile + lane * 2;
     const bool live = c0 < p.C, second = c0 + 1 < p.C;
     const i64 base = (i64)b * p.T * p.C + c_tile;
-    const E *x = static_cast<const E*>(p.x) + base, *gx = static_cast<const E*>(p.gx) + base, *ga = static_cast<const E*>(p.ga) + base,
-            *dy = static_cast<const E*>(p.dy) + base;
+    Fetch<E, WIDE, kTokens, 4> fetch(p.T, p.C, c_tile, lane);
+    fetch.from[0] = static_cast<const E*>(p.x) + base;
+    fetch.from[1] = static_cast<const E*>(p.gx) + base;
+    fetch.from[2] = static_cast<const E*>(p.ga) + base;
+    fetch.from[3] = static_cast<const E*>(p.dy) + base;
     E *dx = static_cast<E*>(p.dx) + base + lane * 2, *dgx = static_cast<E*>(p.dgx) + base + lane * 2, *dga = static_cast<E*>(p.dga) + base + lane * 2;
     E* mine = reinterpret_cast<E*>(raw) + warp * 4 * kPart;
     const uint8_t* first = p.first ? p.first + (i64)b * p.T : nullptr;
@@ -446,13 +478,7 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
 
     auto ask = [&](int round, int stage) {
         const int t = round * kRound + warp * kTokens;
-        E* to = mine + stage * kWarps * 4 * kPart;
-        if (round >= 0 && t < p.T) {
-            fetch<E, WIDE>(to, x, t, p.T, p.C, c_tile, lane);
-            fetch<E, WIDE>(to + kPart, gx, t, p.T, p.C, c_tile, lane);
-            fetch<E, WIDE>(to + 2 * kPart, ga, t, p.T, p.C, c_tile, lane);
-            fetch<E, WIDE>(to + 3 * kPart, dy, t, p.T, p.C, c_tile, lane);
-        }
+        if (round >= 0 && t < p.T) fetch(mine + stage * kWarps * 4 * kPart, t, c_tile);
         commit();
     };
     const int turns = (p.rounds + K - 1) / K;
@@ -472,19 +498,19 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
         wait_group<S - 1>();
         __syncwarp();
         const E* in = mine + stage * kWarps * 4 * kPart + lane * 2;
-        const uint32_t docs = firsts(first, t, p.T, lane);
+        const uint32_t docs = firsts<kTokens>(first, t, p.T, lane);
         // per token: 1 - a, 1 / beta, and w = beta u, which makes room for h before the token
         f2 q[kTokens], inv[kTokens], w[kTokens], P, H, Q;
         Pair<E> least(0.f);
-        auto make = [&](auto is_simple, auto is_small) {
-            constexpr bool kSimple = decltype(is_simple)::value;
+        auto make = [&](auto mode, auto is_small) {
+            constexpr bool kSimple = decltype(mode)::value == kSimpleTile, kExtreme = decltype(mode)::value == kExtremeTile;
             P = both(1.f);
             H = Q = both(0.f);
 #pragma unroll
             for (int j = 0; j < kTokens; ++j) {
                 const Pair<E> vgx(in + kPart + j * kTile), vga(in + 2 * kPart + j * kTile);
-                const Gates<E, !kSimple> g(vga.get(), vgx.get());
-                if (kSimple) least.least(vga), least.least(vgx);
+                const Gates<E, kExtreme> g(vga.get(), vgx.get());
+                if (!kExtreme && (kSimple || t + j < p.T)) least.least(vga), least.least(vgx);   // (other rows hold anything)
                 q[j] = fall<E, decltype(is_small)::value>(mul2(s, g.a));
                 const f2 v = square(q[j]), u = mul2(g.x, get2(in + j * kTile));
                 inv[j] = inverse_root<E>(v);
@@ -507,24 +533,30 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
             }
             P = !kSimple && docs ? both(0.f) : clamp(P);
         };
-        bool simple = docs == 0 && t + kTokens <= p.T;
-        if (simple) {
-            if (small) make(std::true_type{}, std::true_type{}); else make(std::true_type{}, std::false_type{});
-            simple = !__any_sync(0xffffffffu, live && least.below(kFast));
+        int mode = docs == 0 && t + kTokens <= p.T ? kSimpleTile : kDocumentTile;
+        if (mode == kDocumentTile) make(Mode<kDocumentTile>{}, std::false_type{});
+        else if (small) make(Mode<kSimpleTile>{}, std::true_type{});
+        else make(Mode<kSimpleTile>{}, std::false_type{});
+        if (__any_sync(0xffffffffu, live && least.below(kFast))) {
+            mode = kExtremeTile;
+            make(Mode<kExtremeTile>{}, std::false_type{});
         }
-        if (!simple) make(std::false_type{}, std::false_type{});
         shares[buf][warp][lane] = make_ulonglong2(P, Q);
         forward[buf][warp][lane] = H;
         const bool cuts = __syncthreads_or(docs != 0);
         f2 e = CLUSTER ? through_cluster<true>(cluster, K, rank, shares[buf], peers[buf], warp, lane, carry) : ends[buf ^ 1][lane];
         e = through_block<true>(shares[buf], warp, lane, cuts, e);
+        if (cuts) {
+            for (int i = 0; i < warp; ++i) h = step(shares[buf][i][lane].x, forward[buf][i][lane], h);
+        } else {
 #pragma unroll
-        for (int i = 0; i < kWarps - 1; ++i) {
-            if (i >= warp) break;
-            h = step(shares[buf][i][lane].x, forward[buf][i][lane], h);
+            for (int i = 0; i < kWarps - 1; ++i) {
+                if (i >= warp) break;
+                h = fma2(shares[buf][i][lane].x, h, forward[buf][i][lane]);
+            }
         }
-        auto walk = [&](auto is_simple) {
-            constexpr bool kSimple = decltype(is_simple)::value;
+        auto walk = [&](auto mode) {
+            constexpr bool kSimple = decltype(mode)::value == kSimpleTile, kExtreme = decltype(mode)::value == kExtremeTile;
 #pragma unroll
             for (int j = 0; j < kTokens; ++j) {
                 const f2 before = h;
@@ -537,7 +569,7 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
                 at -= p.C;
                 if (!kSimple && t + j >= p.T) continue;
                 const bool doc = !kSimple && docs >> j & 1;
-                const Gates<E, !kSimple> g(get2(in + 2 * kPart + j * kTile), get2(in + kPart + j * kTile));
+                const Gates<E, kExtreme> g(get2(in + 2 * kPart + j * kTile), get2(in + kPart + j * kTile));
                 const f2 vx = get2(in + j * kTile), a = decay(q[j]), G = add2(get2(in + 3 * kPart + j * kTile), e);
                 const f2 beta = doc ? both(1.f) : mul2(square(q[j]), inv[j]);
                 const f2 ox = mul2(mul2(G, beta), g.x), og = mul2(mul2(ox, vx), g.rest_x());
@@ -554,7 +586,9 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
                 }
             }
         };
-        if (simple) walk(std::true_type{}); else walk(std::false_type{});
+        if (mode == kSimpleTile) walk(Mode<kSimpleTile>{});
+        else if (mode == kDocumentTile) walk(Mode<kDocumentTile>{});
+        else walk(Mode<kExtremeTile>{});
         if (!CLUSTER && warp == 0) ends[buf][lane] = e;
         stage = stage == S - 1 ? 0 : stage + 1;
         __syncwarp();
@@ -701,7 +735,7 @@ using namespace rwkvb200;
 
 extern "C" size_t rwkvb200_gated_scan_saved_bytes(int B, int T, int C) {
     if (B <= 0 || T <= 0 || C <= 0) return 0;
-    return (size_t)B * ((T + kRound - 1) / kRound) * C * sizeof(float);
+    return (size_t)B * ((T + kSaved - 1) / kSaved) * C * sizeof(float);
 }
 extern "C" size_t rwkvb200_gated_scan_work_bytes(int B, int T, int C) {
     if (B <= 0 || T <= 0 || C <= 0) return 0;
@@ -713,7 +747,8 @@ extern "C" int rwkvb200_gated_scan_forward(int dtype, int B, int T, int C, const
     if (int e = check("gated_scan_forward", dtype, B, T, C)) return e;
     RWKV_NOTNULL(x); RWKV_NOTNULL(gx); RWKV_NOTNULL(ga); RWKV_NOTNULL(s); RWKV_NOTNULL(y);
     Args p{};
-    p.T = T; p.C = C; p.tiles = (C + kTile - 1) / kTile; p.rounds = (T + kRound - 1) / kRound;
+    p.T = T; p.C = C; p.tiles = (C + kTile - 1) / kTile; p.saves = (T + kSaved - 1) / kSaved; const int round = kWarps * (dtype == RWKVB200_BF16 ? kFwdTokens<bf16> : kFwdTokens<float>);
+    p.rounds = (T + round - 1) / round;
     p.h0 = h0; p.x = x; p.gx = gx; p.ga = ga; p.s = s; p.first = first; p.y = y; p.hT = hT; p.saved = static_cast<float*>(saved);
     const cudaStream_t st = as_stream(stream);
     const int K = cluster_size(B * p.tiles, p.rounds, 2 * sm_count());
@@ -727,7 +762,7 @@ extern "C" int rwkvb200_gated_scan_backward(int dtype, int B, int T, int C, cons
     RWKV_NOTNULL(x); RWKV_NOTNULL(gx); RWKV_NOTNULL(ga); RWKV_NOTNULL(s); RWKV_NOTNULL(saved); RWKV_NOTNULL(dy);
     RWKV_NOTNULL(dx); RWKV_NOTNULL(dgx); RWKV_NOTNULL(dga); RWKV_NOTNULL(ds); RWKV_NOTNULL(work);
     Args p{};
-    p.T = T; p.C = C; p.tiles = (C + kTile - 1) / kTile; p.rounds = (T + kRound - 1) / kRound;
+    p.T = T; p.C = C; p.tiles = (C + kTile - 1) / kTile; p.rounds = p.saves = (T + kSaved - 1) / kSaved;
     p.x = x; p.gx = gx; p.ga = ga; p.s = s; p.first = first; p.saved = static_cast<float*>(const_cast<void*>(saved));
     p.dy = dy; p.dhT = dhT; p.dh0 = dh0; p.dx = dx; p.dgx = dgx; p.dga = dga; p.ds = static_cast<float*>(work);
     const cudaStream_t st = as_stream(stream);
