@@ -123,9 +123,9 @@ __device__ __forceinline__ f2 inverse_root(f2 v) {
     return each(v, [](float x) { return fabsf(x) < 1.2e-38f ? 0.f : Fn<E>::inverse_root(x); });
 }
 
-// sigmoid(ga), sigmoid(gx) and what they lack of 1, without loss of either.  Two forms: as long as no gate is below kFast, so that
+// sigmoid(ga), sigmoid(gx) and what they lack of 1, without loss of either.  Two forms: as long as no gate is below kLeast, so that
 // exp(-ga) exp(-gx) does not overflow, both come from one division; tiles with a gate that is (EXTREME) take one each.
-constexpr float kFast = -41.f;
+constexpr float kLeast = -41.f;
 template <typename E, bool EXTREME>
 struct Gates {
     f2 a, x, ea, ex;
@@ -193,6 +193,10 @@ __device__ __forceinline__ void put2(float* p, f2 v, bool second) {
         if (second) p[1] = hi(v);
     }
 }
+
+// j rows of C elements behind p (one wide multiply-add)
+template <typename E>
+__device__ __forceinline__ E* rows_on(E* p, uint32_t row_bytes, int j) { return reinterpret_cast<E*>(reinterpret_cast<char*>(p) + (uint64_t)row_bytes * (uint32_t)j); }
 
 struct Args {
     int T, C, tiles, rounds, saves;   // channel tiles, rounds of the kernel, of the backward
@@ -332,7 +336,7 @@ constexpr int kBwdStages = 2;
 template <typename E> constexpr int fwd_smem() { return kFwdStages * kWarps * 3 * kFwdTokens<E> * kTile * (int)sizeof(E); }
 template <typename E> constexpr int bwd_smem() { return kBwdStages * kWarps * 4 * kBwdTokens * kTile * (int)sizeof(E); }
 
-// A warp's tile: all tokens are there and none begins a document; or not; or some gate is below kFast (found on the way)
+// A warp's tile: all tokens and channels are there and no document begins; or not; or some gate is out of range (found on the way)
 enum { kSimpleTile, kDocumentTile, kExtremeTile };
 template <int M> using Mode = std::integral_constant<int, M>;
 
@@ -354,6 +358,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
     fetch.from[2] = static_cast<const E*>(p.ga) + base;
     E* y = static_cast<E*>(p.y) + base + lane * 2;
     E* mine = reinterpret_cast<E*>(raw) + warp * 3 * kPart;
+    const uint32_t row_bytes = p.C * (uint32_t)sizeof(E);
     const uint8_t* first = p.first ? p.first + (i64)b * p.T : nullptr;
     const f2 s = pack2(live ? p.s[c0] : 0.f, second ? p.s[c0 + 1] : 0.f);
     const i64 row = (i64)b * p.C + c0;
@@ -403,11 +408,11 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
             }
             share.P = !kSimple && docs ? both(0.f) : clamp(share.P);
         };
-        int mode = docs == 0 && t + kTokens <= p.T ? kSimpleTile : kDocumentTile;
+        int mode = docs == 0 && t + kTokens <= p.T && c_tile + kTile <= p.C ? kSimpleTile : kDocumentTile;
         if (mode == kDocumentTile) make(Mode<kDocumentTile>{}, std::false_type{});
         else if (small) make(Mode<kSimpleTile>{}, std::true_type{});
         else make(Mode<kSimpleTile>{}, std::false_type{});
-        if (__any_sync(0xffffffffu, live && least.below(kFast))) {
+        if (__any_sync(0xffffffffu, live && least.below(kLeast))) {
             mode = kExtremeTile;
             make(Mode<kExtremeTile>{}, std::false_type{});
         }
@@ -423,15 +428,15 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
         E* to = y + (i64)t * p.C;
         if (mode == kSimpleTile) {
 #pragma unroll
-            for (int j = 0; j < kTokens; ++j, to += p.C) {
+            for (int j = 0; j < kTokens; ++j) {
                 h = fma2(a[j], h, w[j]);
-                if (live) put2<WIDE>(to, h, second);
+                put2<WIDE>(rows_on(to, row_bytes, j), h, second);
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < kTokens; ++j, to += p.C) {
+            for (int j = 0; j < kTokens; ++j) {
                 h = docs >> j & 1 ? w[j] : fma2(a[j], h, w[j]);
-                if (live && t + j < p.T) put2<WIDE>(to, h, second);
+                if (live && t + j < p.T) put2<WIDE>(rows_on(to, row_bytes, j), h, second);
             }
         }
         if (!CLUSTER && warp == kWarps - 1) ends[buf][lane] = h;
@@ -450,7 +455,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
 
 // Rounds from the last to the first; e (the gradient that comes into a token from the later ones) goes the same way as h does in
 // the forward, with the same products of decays.  h before each token is made again from the saved states, and so are the gates
-// in the last walk: keeping them would take more registers than two blocks per SM have, and about as many instructions.
+// in the last walk: keeping them would take more registers than two blocks per SM have.
 template <typename E, bool WIDE, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_backward_kernel(const Args p) {
     extern __shared__ __align__(16) unsigned char raw[];
@@ -470,6 +475,7 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
     fetch.from[3] = static_cast<const E*>(p.dy) + base;
     E *dx = static_cast<E*>(p.dx) + base + lane * 2, *dgx = static_cast<E*>(p.dgx) + base + lane * 2, *dga = static_cast<E*>(p.dga) + base + lane * 2;
     E* mine = reinterpret_cast<E*>(raw) + warp * 4 * kPart;
+    const uint32_t row_bytes = p.C * (uint32_t)sizeof(E);
     const uint8_t* first = p.first ? p.first + (i64)b * p.T : nullptr;
     const f2 s = pack2(live ? p.s[c0] : 0.f, second ? p.s[c0 + 1] : 0.f);
     const i64 row = (i64)b * p.C + c0;
@@ -533,11 +539,11 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
             }
             P = !kSimple && docs ? both(0.f) : clamp(P);
         };
-        int mode = docs == 0 && t + kTokens <= p.T ? kSimpleTile : kDocumentTile;
+        int mode = docs == 0 && t + kTokens <= p.T && c_tile + kTile <= p.C ? kSimpleTile : kDocumentTile;
         if (mode == kDocumentTile) make(Mode<kDocumentTile>{}, std::false_type{});
         else if (small) make(Mode<kSimpleTile>{}, std::true_type{});
         else make(Mode<kSimpleTile>{}, std::false_type{});
-        if (__any_sync(0xffffffffu, live && least.below(kFast))) {
+        if (__any_sync(0xffffffffu, live && least.below(kLeast))) {
             mode = kExtremeTile;
             make(Mode<kExtremeTile>{}, std::false_type{});
         }
@@ -563,10 +569,10 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
                 h = !kSimple && docs >> j & 1 ? w[j] : fma2(decay(q[j]), h, w[j]);
                 w[j] = before;
             }
-            i64 at = (i64)(t + kTokens) * p.C;
+            const i64 at = (i64)t * p.C;
+            E *px = dx + at, *pgx = dgx + at, *pga = dga + at;
 #pragma unroll
             for (int j = kTokens - 1; j >= 0; --j) {
-                at -= p.C;
                 if (!kSimple && t + j >= p.T) continue;
                 const bool doc = !kSimple && docs >> j & 1;
                 const Gates<E, kExtreme> g(get2(in + 2 * kPart + j * kTile), get2(in + kPart + j * kTile));
@@ -579,10 +585,10 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
                 if (doc) e = dL = both(0.f);
                 const f2 oa = mul2(mul2(dL, mul2(s, g.a)), g.rest_a());
                 ds = fma2(dL, g.a, ds);
-                if (live) {
-                    put2<WIDE>(dx + at, ox, second);
-                    put2<WIDE>(dgx + at, og, second);
-                    put2<WIDE>(dga + at, oa, second);
+                if (kSimple || live) {
+                    put2<WIDE>(rows_on(px, row_bytes, j), ox, second);
+                    put2<WIDE>(rows_on(pgx, row_bytes, j), og, second);
+                    put2<WIDE>(rows_on(pga, row_bytes, j), oa, second);
                 }
             }
         };
@@ -673,17 +679,11 @@ int check(const char* what, int dtype, int B, int T, int C) {
     return RWKVB200_OK;
 }
 
-// How many blocks share a (sequence, channel tile): the K for which the rounds that an SM's places go through one after the other are
-// fewest, a barrier of a cluster counting as a quarter of a round.
-int cluster_size(int units, int rounds, int places) {
-    int best = 1;
-    double least = 0;
-    for (int K = 1; K <= kMaxCluster; K *= 2) {
-        if (K > 1 && K > rounds) break;
-        const double cost = (double)(((i64)units * K + places - 1) / places) * ((rounds + K - 1) / K) * (K > 1 ? 1.25 : 1.0);
-        if (K == 1 || cost < least) best = K, least = cost;
-    }
-    return best;
+// How many blocks share a (sequence, channel tile): as many as leave two blocks for every SM, up to what a cluster may have.
+int cluster_size(int units, int rounds) {
+    int K = 1;
+    while (K < kMaxCluster && 2 * K <= rounds && (i64)units * K * 2 <= 2 * sm_count()) K *= 2;
+    return K;
 }
 
 template <auto Kernel>
@@ -751,7 +751,7 @@ extern "C" int rwkvb200_gated_scan_forward(int dtype, int B, int T, int C, const
     p.rounds = (T + round - 1) / round;
     p.h0 = h0; p.x = x; p.gx = gx; p.ga = ga; p.s = s; p.first = first; p.y = y; p.hT = hT; p.saved = static_cast<float*>(saved);
     const cudaStream_t st = as_stream(stream);
-    const int K = cluster_size(B * p.tiles, p.rounds, 2 * sm_count());
+    const int K = cluster_size(B * p.tiles, p.rounds);
     return dtype == RWKVB200_BF16 ? run_forward<bf16>(p, B, K, st) : run_forward<float>(p, B, K, st);
 }
 
@@ -766,7 +766,7 @@ extern "C" int rwkvb200_gated_scan_backward(int dtype, int B, int T, int C, cons
     p.x = x; p.gx = gx; p.ga = ga; p.s = s; p.first = first; p.saved = static_cast<float*>(const_cast<void*>(saved));
     p.dy = dy; p.dhT = dhT; p.dh0 = dh0; p.dx = dx; p.dgx = dgx; p.dga = dga; p.ds = static_cast<float*>(work);
     const cudaStream_t st = as_stream(stream);
-    const int K = cluster_size(B * p.tiles, p.rounds, (dtype == RWKVB200_BF16 ? 2 : 1) * sm_count());
+    const int K = cluster_size(B * p.tiles, p.rounds);
     const int rc = dtype == RWKVB200_BF16 ? run_backward<bf16>(p, B, K, st) : run_backward<float>(p, B, K, st);
     return rc != RWKVB200_OK ? rc : sum_rows(RWKVB200_F32, (i64)B * K, C, p.ds, ds, st);
 }
