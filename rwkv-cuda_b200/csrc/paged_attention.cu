@@ -9,6 +9,8 @@
 // the others each block leaves (m, sum, sum of exp v) and a second kernel joins them.  A block's run has at most one unit that
 // began before it and one that ends behind it: two places a block.
 #include "paged.cuh"
+#include "wkv7_umma.cuh"
+#include <cuda.h>
 
 namespace rwkvb200 {
 namespace {
@@ -30,15 +32,18 @@ struct AttentionArgs {
 };
 
 struct Range {
-    int lo, hi, tiles;   // tokens of a sequence that count, and their tiles: one at least, so that empty sequences get their zeros
+    int lo, hi, start, tiles;   // tokens of a sequence that count; its tiles, from a multiple of 16 on: one at least, so that empty
+                                // sequences get their zeros, and none for a row that only pads the batch
     __device__ __forceinline__ Range(const AttentionArgs& p, int b) {
         hi = min(p.lengths[b], p.width * (int)p.page.d);
         lo = p.window > 0 ? max(0, hi - p.window) : 0;
-        tiles = hi < 0 ? 0 : max(1, (hi - lo + kTile - 1) / kTile);   // a negative length is a row that only pads the batch
+        start = lo & ~15;
+        tiles = hi < 0 ? 0 : max(1, (hi - start + kTile - 1) / kTile);
     }
 };
 
-// All threads: the number of tiles of all units, and of those of the sequences before b_of.
+// All threads: the number of tiles of the units of the sequences before `end`.
+template <int THREADS>
 __device__ __forceinline__ i64 sum_block(i64 v, i64* shared) {
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -47,21 +52,23 @@ __device__ __forceinline__ i64 sum_block(i64 v, i64* shared) {
     __syncthreads();
     v = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) v += shared[w];
+    for (int w = 0; w < THREADS / 32; ++w) v += shared[w];
     return v;
 }
+template <int THREADS = kThreads>
 __device__ __forceinline__ i64 tiles_before(const AttentionArgs& p, int end, i64* shared) {
     i64 n = 0;
-    for (int b = threadIdx.x; b < end; b += kThreads) n += Range(p, b).tiles;
-    return sum_block(n, shared) * (p.Hkv * p.blocks);
+    for (int b = threadIdx.x; b < end; b += THREADS) n += Range(p, b).tiles;
+    return sum_block<THREADS>(n, shared) * (p.Hkv * p.blocks);
 }
 __device__ __forceinline__ i64 run_length(i64 all, i64 blocks) { return max((i64)kMinTiles, (all + blocks - 1) / blocks); }
 
 // The sequence that tile `begin` of all lies in, and the tiles of those before it.
+template <int THREADS = kThreads>
 __device__ __forceinline__ void find_start(const AttentionArgs& p, i64 begin, int units, i64* shared, i64* start) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     i64 base = 0;
-    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+    for (int b0 = 0; b0 < p.B; b0 += THREADS) {
         const int b = b0 + threadIdx.x;
         i64 n = b < p.B ? (i64)Range(p, b).tiles * units : 0, x = n;
 #pragma unroll
@@ -73,7 +80,7 @@ __device__ __forceinline__ void find_start(const AttentionArgs& p, i64 begin, in
         if (lane == 31) shared[warp] = x;
         __syncthreads();
         i64 before = base;
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < THREADS / 32; ++w) {
             if (w < warp) before += shared[w];
             base += shared[w];
         }
@@ -152,8 +159,9 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const AttentionArgs
         struct alignas(sizeof(E) * W) Piece {
             E e[W];
         };
-        const int last = min(r.lo + t1 * kTile, r.hi);
-        for (int j = r.lo + t0 * kTile + token; j < last; j += kWarps * 4) {
+        const int last = min(r.start + t1 * kTile, r.hi);
+        for (int j = r.start + t0 * kTile + token; j < last; j += kWarps * 4) {
+            if (j < r.lo) continue;
             const i64 place = cache.at(j);
             const bool found = place >= 0;
             const E *k = static_cast<const E*>(p.k_pages) + (found ? place : 0), *v = static_cast<const E*>(p.v_pages) + (found ? place : 0);
@@ -244,13 +252,15 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const AttentionArgs
 
 // bf16, heads of whole 16-byte pieces: products on mma.sync m16n8k16 with the tokens in the rows, S^T = K q^T and O^T = V^T P^T, for up
 // to 8 HT query heads that share the keys: HT = 1 wastes nothing on groups of 8, and memory bounds both anyway.  Each warp takes
-// 16 of a tile's tokens and keeps its own maxima and sums.  The order of the elements of a head (and of the tokens in the second product) is
-// free as long as both operands agree, so a lane reads its fragments as 16-byte pieces of rows:
-//   keys    lane (g, q): rows g and g + 8, pieces 4 i + q            values  rows 2q, 2q+1, 2q+8, 2q+9, pieces 8 i + g
-// They come through shared memory by cp.async (kStages - 1 steps ahead), every lane to a place of its own: no barrier, no bank
-// conflict, and rows that do not count are filled with zeros.  Weights are taken into the second product as the sum of two
-// bf16 numbers (2^-16 relative; one would double the output's rounding), both above 0, so that an infinite value stays one.
-constexpr int kStages = 2;
+// 16 of a tile's tokens and keeps its own maxima and sums.  Both operands come out of shared memory by ldmatrix (the values transposed), from
+// tiles of [16 tokens][64 elements] in the 128-byte swizzle.  They get there
+//   TMA:  by one bulk copy of 16 rows each for keys and values (pages of a multiple of 16 tokens, heads of 64 or 128): a warp's
+//         lane 0 asks, keys two steps ahead and values one, and counts the bytes on a barrier of the slot;
+//   else: by cp.async in pieces of 16 bytes, rows that do not count filled with zeros.  (Taken for every page size, with a lane's
+//         pieces in places of its own, this read 4.0 TB/s at 128 sequences of up to 4096 tokens; without any product 4.1.)
+// Weights are taken into the second product as the sum of two bf16 numbers (2^-16 relative; one would double the output's
+// rounding), both above 0, so that an infinite value stays one.
+constexpr int kTimeout = 3;       // a wait for a copy ran out
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -286,28 +296,53 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&t);
 }
-__device__ __forceinline__ void copy_or_zero(void* to, const bf16* from, bool there) {
-    const uint32_t shared = (uint32_t)__cvta_generic_to_shared(to);
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copy_or_zero(uint32_t shared, const bf16* from, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 
-template <int NP, int HT>
-__global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const AttentionArgs p) {
-    constexpr int kK = NP / 32, kV = NP / 64;            // pieces of a key's, of a value's row per lane
-    constexpr int kPieces = 2 * kK + 4 * kV, kHeads = 8 * HT;
-    extern __shared__ __align__(16) uint4 staged[];      // [warp][stage][piece][lane]
+__device__ __forceinline__ void ldmatrix(uint32_t (&d)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_transposed(uint32_t (&d)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(at) : "memory");
+}
+// 16 rows of a pool, from number `row` on, counted on `bar`
+__device__ __forceinline__ void copy_rows(uint32_t to, const CUtensorMap* map, int row, uint64_t* bar, int bytes) {
+    const uint32_t b = (uint32_t)__cvta_generic_to_shared(bar);
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(to),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(row), "r"(0), "r"(b)
+                 : "memory");
+}
+struct Maps {
+    CUtensorMap keys, values;
+};
+
+template <int NP, int HT, bool TMA>
+__global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const AttentionArgs p, const __grid_constant__ Maps maps) {
+    constexpr int kHalves = NP / 64, kRows = 2048 * kHalves;   // bytes of 16 rows
+    constexpr int kHeads = 8 * HT, kWarpBytes = 4 * kRows;     // a warp's slots: keys of two steps, values of two
+    extern __shared__ __align__(1024) unsigned char staged[];
     __shared__ i64 shared[kWarps], sStart[2];
     __shared__ float sM[kWarps][kHeads], sL[kWarps][kHeads];
+    __shared__ uint64_t bars[kWarps][4];                       // TMA: one per slot
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
-    const int units = p.Hkv * p.blocks;
+    const int units = p.Hkv * p.blocks, N = TMA ? NP : p.N;
+    if (TMA && lane < 4) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(&bars[warp][lane])));
+    if (TMA) v7u::proxy_fence();
     const i64 all = tiles_before(p, p.B, shared), run = run_length(all, gridDim.x);
     const i64 begin = run * blockIdx.x, end = min(begin + run, all);
     if (begin >= end) return;
     find_start(p, begin, units, shared, sStart);
-    uint4* mine = staged + warp * kStages * kPieces * 32 + lane;
-    float* sO = reinterpret_cast<float*>(staged + warp * kStages * kPieces * 32);   // [head][NP], between the tokens of two units
-    const bf16 *keys = static_cast<const bf16*>(p.k_pages), *values = static_cast<const bf16*>(p.v_pages);
+    unsigned char* mine = staged + warp * kWarpBytes;
+    const uint32_t base_keys = (uint32_t)__cvta_generic_to_shared(mine), base_values = base_keys + 2 * kRows;
+    float* sO = reinterpret_cast<float*>(mine);                // [head][NP], between the tokens of two units
+    // where a lane's rows for ldmatrix lie: keys: rows lane & 15, piece lane / 16; values: rows by 8 from lane / 16, piece by lane / 8
+    const uint32_t key_row = (lane & 15) * 128, key_piece = lane >> 4, value_row = ((lane & 7) + (lane >> 4) * 8) * 128, value_piece = lane >> 3 & 1, swizzle = lane & 7;
     const float scale = p.cap > 0.f ? p.scale / p.cap : p.scale * kLog2e, cap = p.cap * kLog2e;
+    uint32_t phases = 0;     // of the four barriers
+    bool lost = false;       // a wait ran out: nothing more is asked for, and the results are NaN
     int b = (int)sStart[0];
     i64 base = sStart[1];
     for (i64 at = begin; at < end;) {
@@ -322,49 +357,65 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
         const int head = unit / p.blocks, h0 = head * p.group + unit % p.blocks * kHeads, heads = min(kHeads, (head + 1) * p.group - h0);
         if (threadIdx.x == 0 && p.lengths[b] > r.hi) atomicMax(&g_error, kBadLength);
         const int* row = p.table + (i64)b * p.width;
-        const int from = r.lo + t0 * kTile + warp * 16, last = min(r.lo + t1 * kTile, r.hi), steps = t1 - t0;
-        // the row of the pools that token (lane & 15) of a step lies in; -1: the token does not count
-        auto rows_of = [&](int step) {
-            const int j = from + step * kTile + (lane & 15);
-            int n = -1;
-            if (step < steps && j < last) {
-                const uint32_t col = p.page.quotient((uint32_t)j);
-                const int id = row[col];
-                if ((unsigned)id < (unsigned)p.pages) n = (id * p.Hkv + head) * (int)p.page.d + (j - (int)(col * p.page.d));
-                else atomicMax(&g_error, kBadPage);
-            }
-            return n;
+        const int from = r.start + t0 * kTile + warp * 16, last = min(r.start + t1 * kTile, r.hi), steps = lost ? 0 : t1 - t0;
+        // Of a step's tokens the lane answers for number lane & 15 (TMA: all for the first: they share a page).  Its page is asked for a
+        // step before it is looked at.
+        auto counts = [&](int j) { return j >= r.lo && j < last; };
+        auto token_of = [&](int step) { return from + step * kTile + (TMA ? 0 : lane & 15); };
+        auto in_use = [&](int step, int j) { return step < steps && (TMA ? j < last : counts(j)); };
+        auto page_of = [&](int step) {
+            const int j = token_of(step);
+            return in_use(step, j) ? row[p.page.quotient((uint32_t)j)] : 0;
         };
-        auto ask = [&](int n, int stage) {   // copies the step whose rows are n
-            uint4* to = mine + stage * kPieces * 32;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int k = __shfl_sync(0xffffffffu, n, g + 8 * i);
-                const bf16* at = keys + (i64)max(k, 0) * p.N + q * 8;
-#pragma unroll
-                for (int j = 0; j < kK; ++j) copy_or_zero(to + (i * kK + j) * 32, at + j * 32, k >= 0 && j * 32 + q * 8 < p.N);
+        // the row of the pools that the token lies in; -1: it does not count
+        auto row_of = [&](int step, int id) {
+            const int j = token_of(step);
+            if (!in_use(step, j)) return -1;
+            if ((unsigned)id >= (unsigned)p.pages) {
+                atomicMax(&g_error, kBadPage);
+                return -1;
             }
+            return (id * p.Hkv + head) * (int)p.page.d + (j - (int)(p.page.quotient((uint32_t)j) * p.page.d));
+        };
+        auto ask = [&](bool values, int step, int n) {
+            const int slot = step & 1;
+            const uint32_t to = (values ? base_values : base_keys) + slot * kRows;
+            if (TMA) {
+                if (lane == 0 && n >= 0) copy_rows(to, values ? &maps.values : &maps.keys, n, &bars[warp][values * 2 + slot], kRows);
+            } else {
+                const bf16* pool = static_cast<const bf16*>(values ? p.v_pages : p.k_pages);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int v = __shfl_sync(0xffffffffu, n, 2 * q + (i & 1) + 8 * (i >> 1));
-                const bf16* at = values + (i64)max(v, 0) * p.N + g * 8;
-#pragma unroll
-                for (int j = 0; j < kV; ++j) copy_or_zero(to + (2 * kK + i * kV + j) * 32, at + j * 64, v >= 0 && j * 64 + g * 8 < p.N);
+                for (int i = 0; i < kRows / 512; ++i) {
+                    const int piece = i * 32 + lane, token = piece / (8 * kHalves), c = piece % (8 * kHalves);
+                    const int k = __shfl_sync(0xffffffffu, n, token);
+                    copy_or_zero(to + (c >> 3) * 2048 + token * 128 + (((c ^ token) & 7) << 4), pool + (i64)max(k, 0) * N + min(c * 8, N - 8), k >= 0 && c * 8 < N);
+                }
             }
         };
-        // q as the second operand of the scores: head g (and g + 8), the elements that the lane has of the keys
-        uint32_t qf[HT][kK][4];
+        auto arrived = [&](bool values, int step, int n) {   // TMA: waits for what has been asked for
+            const int which = values * 2 + (step & 1);
+            if (!TMA || n < 0) return;
+            if (__any_sync(0xffffffffu, !v7u::mbar_wait(&bars[warp][which], phases >> which & 1))) lost = true;
+            phases ^= 1u << which;
+        };
+        const int id0 = page_of(0), id1 = page_of(1);
+        int id2 = page_of(2);
+        int n0 = row_of(0, id0), n1 = row_of(1, id1);
+        ask(false, 0, n0);
+        commit();
+        ask(false, 1, n1);
+        ask(true, 0, n0);
+        commit();
+        // q as the second operand of the scores: head g (and g + 8)
+        uint32_t qf[HT][NP / 16][2];
 #pragma unroll
         for (int h = 0; h < HT; ++h)
 #pragma unroll
-            for (int j = 0; j < kK; ++j) {
-                const bf16* from = static_cast<const bf16*>(p.q) + ((i64)b * p.Hq + h0 + h * 8 + g) * p.N + j * 32 + q * 8;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    __nv_bfloat162 v = __floats2bfloat162_rn(0.f, 0.f);
-                    if (h * 8 + g < heads && j * 32 + q * 8 < p.N) v.x = from[2 * e], v.y = from[2 * e + 1];
-                    qf[h][j][e] = *reinterpret_cast<const uint32_t*>(&v);
-                }
+            for (int j = 0; j < NP / 8; ++j) {
+                const bf16* from = static_cast<const bf16*>(p.q) + ((i64)b * p.Hq + h0 + h * 8 + g) * N + j * 8 + q * 2;
+                __nv_bfloat162 v = __floats2bfloat162_rn(0.f, 0.f);
+                if (h * 8 + g < heads && j * 8 < N) v.x = from[0], v.y = from[1];
+                qf[h][j / 2][j % 2] = *reinterpret_cast<const uint32_t*>(&v);
             }
         float slope[HT][2], m[HT][2], l[HT][2], o[HT][NP / 16][4];   // heads 8 h + 2q, + 1
 #pragma unroll
@@ -380,34 +431,51 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[h][i][e] = 0.f;
         }
-        int next = rows_of(0), ahead = rows_of(1);   // rows of the next step, and of the one behind it
-        ask(next, 0);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        for (int step = 0; step < steps; ++step) {
-            const int n = next;
-            uint4* in = mine + (step & 1) * kPieces * 32;
-            ask(ahead, (step + 1) & 1);
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            next = ahead;
-            ahead = rows_of(step + 2);
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        // The scores of a step are made while the step before it is summed.
+        float next[HT][4];
+        auto scores = [&](int step) {
+            const uint32_t in = base_keys + (step & 1) * kRows + key_row;
+#pragma unroll
+            for (int h = 0; h < HT; ++h)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) next[h][e] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NP / 16; ++j) {
+                uint32_t a[4];
+                ldmatrix(a, in + j / 4 * 2048 + (((j % 4 * 2 + key_piece) ^ swizzle) << 4));
+#pragma unroll
+                for (int h = 0; h < HT; ++h) mma(next[h], a[0], a[1], a[2], a[3], qf[h][j][0], qf[h][j][1]);
+            }
+        };
+        if (!TMA) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        arrived(false, 0, n0);
+        __syncwarp();
+        scores(0);
+        for (int step = 0; step < steps && !lost; ++step) {
             float z[HT][4];
 #pragma unroll
             for (int h = 0; h < HT; ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) z[h][e] = 0.f;
-#pragma unroll
-            for (int j = 0; j < kK; ++j) {
-                const uint4 x = in[j * 32], y = in[(kK + j) * 32];
-#pragma unroll
-                for (int h = 0; h < HT; ++h) {
-                    mma(z[h], x.x, y.x, x.y, y.y, qf[h][j][0], qf[h][j][1]);
-                    mma(z[h], x.z, y.z, x.w, y.w, qf[h][j][2], qf[h][j][3]);
-                }
-            }
+                for (int e = 0; e < 4; ++e) z[h][e] = next[h][e];
+            const int n2 = row_of(step + 2, id2);
+            id2 = page_of(step + 3);
+            __syncwarp();                 // (all lanes have read the slots that are asked for)
+            ask(false, step + 2, n2);
+            ask(true, step + 1, n1);
+            commit();
+            if (!TMA) asm volatile("cp.async.wait_group 1;" ::: "memory");
+            arrived(false, step + 1, n1);
+            arrived(true, step, n0);
+            __syncwarp();
+            scores(step + 1);
+            const int n = n0;
+            n0 = n1;
+            n1 = n2;
+            if (!__any_sync(0xffffffffu, n >= 0)) continue;   // no token counts
             // scores as exponents of 2: tokens g (elements 0, 1) and g + 8 (2, 3)
-            const bool there[2] = {__shfl_sync(0xffffffffu, n, g) >= 0, __shfl_sync(0xffffffffu, n, g + 8) >= 0};
-            const float distance = (float)(from + step * kTile + g - (r.hi - 1));
+            const int j = from + step * kTile + g;
+            const bool there[2] = {TMA ? counts(j) : __shfl_sync(0xffffffffu, n, g) >= 0, TMA ? counts(j + 8) : __shfl_sync(0xffffffffu, n, g + 8) >= 0};
+            const float distance = (float)(j - (r.hi - 1));
             bool more = false, none = false;   // a new maximum; a score of -infinity
 #pragma unroll
             for (int h = 0; h < HT; ++h)
@@ -440,25 +508,29 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
                         for (int e = 0; e < 4; ++e) o[h][i][e] *= keep[e & 1];
                 }
             }
+            const uint32_t in = base_values + (step & 1) * kRows;
             if (__any_sync(0xffffffffu, none)) {
-                // a token without weight in any head counts for nothing, whatever its value holds
+                // a token without weight in any head counts for nothing, whatever its value (or the memory behind the last token) holds
                 bool dead[2] = {true, true};
 #pragma unroll
                 for (int h = 0; h < HT; ++h)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) dead[e >> 1] &= h * 8 + 2 * q + (e & 1) >= heads || z[h][e] == -INFINITY;
-                uint32_t gone[2];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    uint32_t x = __ballot_sync(0xffffffffu, dead[i]);
-                    x &= x >> 1;
-                    gone[i] = x & x >> 2;   // bit 4 g: token g (+ 8)
+                    uint32_t gone = __ballot_sync(0xffffffffu, dead[i]);
+                    gone &= gone >> 1;
+                    gone = gone & gone >> 2 & 0x11111111u;   // bit 4 t: token t (+ 8)
+                    for (; gone != 0; gone &= gone - 1) {
+                        const int token = i * 8 + (__ffs(gone) - 1) / 4;
+                        if (lane < 8 * kHalves) {
+                            unsigned char* to = mine + 2 * kRows + (step & 1) * kRows + lane / 8 * 2048 + token * 128 + lane % 8 * 16;
+                            *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
+                        }
+                    }
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (gone[i >> 1] >> (4 * (2 * q + (i & 1))) & 1)
-#pragma unroll
-                        for (int j = 0; j < kV; ++j) in[(2 * kK + i * kV + j) * 32] = make_uint4(0, 0, 0, 0);
+                if (TMA) v7u::proxy_fence();
+                __syncwarp();
             }
             // weights, and as the second operand of the second product
             uint32_t high[HT][2], low[HT][2];
@@ -478,36 +550,24 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
                     low[h][i] = transposed(pack_bf16(y[2 * i], y[2 * i + 1]));
                 }
             }
-            // rows of O^T: g is element i of the lane's first piece, g + 8 of its second (NP = 64: element i + 4 of the only one)
 #pragma unroll
-            for (int half = 0; half < (NP == 64 ? 1 : 2); ++half) {
-                uint32_t v[4][4];   // [token][word]: NP = 128: words 2 half, + 1 of both pieces; 64: all words
+            for (int i = 0; i < NP / 16; ++i) {
+                uint32_t a[4];
+                ldmatrix_transposed(a, in + value_row + i / 4 * 2048 + (((i % 4 * 2 + value_piece) ^ swizzle) << 4));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (NP == 64) {
-                        const uint4 x = in[(2 * kK + i) * 32];
-                        v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
-                    } else {
-                        const uint2 x = reinterpret_cast<const uint2*>(&in[(2 * kK + i * kV) * 32])[half], y = reinterpret_cast<const uint2*>(&in[(2 * kK + i * kV + kV - 1) * 32])[half];
-                        v[i][0] = x.x, v[i][1] = x.y, v[i][2] = y.x, v[i][3] = y.y;
-                    }
+                for (int h = 0; h < HT; ++h) {
+                    mma(o[h][i], a[0], a[1], a[2], a[3], high[h][0], high[h][1]);
+                    mma(o[h][i], a[0], a[1], a[2], a[3], low[h][0], low[h][1]);
                 }
-#pragma unroll
-                for (int w = 0; w < 2; ++w)
-#pragma unroll
-                    for (int odd = 0; odd < 2; ++odd) {
-                        const uint32_t pick = odd ? 0x7632 : 0x5410;
-                        const uint32_t a0 = __byte_perm(v[0][w], v[1][w], pick), a1 = __byte_perm(v[0][w + 2], v[1][w + 2], pick);
-                        const uint32_t a2 = __byte_perm(v[2][w], v[3][w], pick), a3 = __byte_perm(v[2][w + 2], v[3][w + 2], pick);
-#pragma unroll
-                        for (int h = 0; h < HT; ++h) {
-                            mma(o[h][half * 4 + w * 2 + odd], a0, a1, a2, a3, high[h][0], high[h][1]);
-                            mma(o[h][half * 4 + w * 2 + odd], a0, a1, a2, a3, low[h][0], low[h][1]);
-                        }
-                    }
             }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (!TMA) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (lost) {   // what may still be in flight, and results that cannot pass as such
+            for (int i = 0; i < 4; ++i) v7u::mbar_wait(&bars[warp][i], phases >> i & 1, 1 << 10);
+            if (lane == 0) atomicMax(&g_error, kTimeout);
+#pragma unroll
+            for (int h = 0; h < HT; ++h) m[h][0] = m[h][1] = 0.f, l[h][0] = l[h][1] = __int_as_float(0x7fffffff);
+        }
         __syncwarp();
         // the warp's shares: O^T back to heads in rows
 #pragma unroll
@@ -521,17 +581,14 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
 #pragma unroll
             for (int i = 0; i < NP / 16; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int n = g * 8 + (NP == 64 ? i + (e >> 1) * 4 : i + (e >> 1) * 64);
-                    sO[(h * 8 + 2 * q + (e & 1)) * NP + n] = o[h][i][e];
-                }
+                for (int e = 0; e < 4; ++e) sO[(h * 8 + 2 * q + (e & 1)) * NP + i * 16 + g + (e >> 1) * 8] = o[h][i][e];
         }
         __syncthreads();
         const bool whole = t0 == 0 && t1 == r.tiles;
-        float* part = p.work + ((i64)blockIdx.x * 2 + (t0 == 0)) * kHeads * (p.N + 2);
-        const float* all_o = reinterpret_cast<const float*>(staged);
-        for (int i = threadIdx.x; i < heads * p.N; i += kThreads) {
-            const int h = i / p.N, n = i % p.N;
+        float* part = p.work + ((i64)blockIdx.x * 2 + (t0 == 0)) * kHeads * (N + 2);
+        for (int i = threadIdx.x; i < heads * NP; i += kThreads) {
+            const int h = i / NP, n = i % NP;
+            if (n >= N) continue;
             float top = -INFINITY, x = 0.f, sum = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sM[w][h]);
@@ -540,50 +597,93 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
                 const float keep = sM[w][h] == -INFINITY ? 0.f : ex2(sM[w][h] - top);
                 sum += sL[w][h] * keep;
                 // (a warp whose maximum is -infinity has sums of zeros, or NaN from a NaN score)
-                if (sM[w][h] != -INFINITY) x += all_o[w * kStages * kPieces * 128 + h * NP + n] * keep;
+                if (sM[w][h] != -INFINITY) x += reinterpret_cast<const float*>(staged + w * kWarpBytes)[h * NP + n] * keep;
             }
             if (whole) {
-                static_cast<bf16*>(p.out)[((i64)b * p.Hq + h0 + h) * p.N + n] = __float2bfloat16_rn(sum == 0.f ? 0.f : x / sum);
+                static_cast<bf16*>(p.out)[((i64)b * p.Hq + h0 + h) * N + n] = __float2bfloat16_rn(sum == 0.f ? 0.f : x / sum);
                 if (n == 0 && p.lse != nullptr) p.lse[(i64)b * p.Hq + h0 + h] = sum == 0.f ? -INFINITY : top * kLn2 + logf(sum);
             } else {
-                part[h * (p.N + 2) + n] = x;
-                if (n == 0) part[h * (p.N + 2) + p.N] = top, part[h * (p.N + 2) + p.N + 1] = sum;
+                part[h * (N + 2) + n] = x;
+                if (n == 0) part[h * (N + 2) + N] = top, part[h * (N + 2) + N + 1] = sum;
             }
         }
+        if (TMA) v7u::proxy_fence();
         __syncthreads();
     }
 }
 
-// A block per unit: joins what the blocks `parts` of the kernel above have left of it.
+// Joins what the `parts` blocks of a kernel above have left: block i does the unit that goes over the border of runs i and i + 1, if it
+// began in run i.  Weights of the shares first, then a thread per element of a head and kSplit-th share.
+constexpr int kJoinThreads = 512;
 template <typename E>
-__global__ void __launch_bounds__(kThreads) join_kernel(const AttentionArgs p, int parts, int HB) {
-    __shared__ i64 shared[kWarps];
-    const int units = p.Hkv * p.blocks, b = blockIdx.x / units, unit = blockIdx.x % units;
-    const i64 all = tiles_before(p, p.B, shared), run = run_length(all, parts);
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttentionArgs p, int parts, int HB) {
+    extern __shared__ float weights[];   // [head][share], then [head]: the sums
+    __shared__ i64 shared[kJoinThreads / 32], sStart[2];
+    __shared__ float sums[kJoinThreads];
+    const int units = p.Hkv * p.blocks;
+    const i64 all = tiles_before<kJoinThreads>(p, p.B, shared), run = run_length(all, parts);
+    const i64 border = run * (blockIdx.x + 1);
+    if (border >= all) return;
+    find_start<kJoinThreads>(p, border, units, shared, sStart);
+    const int b = (int)sStart[0];
     const Range r(p, b);
-    if (r.tiles == 0) return;
-    const i64 begin = tiles_before(p, b, shared) + (i64)unit * r.tiles;
-    const i64 c0 = begin / run, c1 = (begin + r.tiles - 1) / run;
-    if (c0 == c1) return;
+    const int unit = (int)((border - sStart[1]) / r.tiles);
+    const i64 begin = sStart[1] + (i64)unit * r.tiles;
+    if (begin == border || begin < border - run) return;   // nothing goes over the border, or it began earlier
+    const int c0 = blockIdx.x, count = (int)((begin + r.tiles - 1) / run) - c0 + 1;
     const int head = unit / p.blocks, h0 = head * p.group + unit % p.blocks * HB, heads = min(HB, (head + 1) * p.group - h0);
     const int stride = p.N + 2;
-    for (int i = threadIdx.x; i < heads * p.N; i += kThreads) {
-        const int h = i / p.N, n = i % p.N;
-        float top = -INFINITY, x = 0.f, sum = 0.f;
-        for (i64 c = c0; c <= c1; ++c) top = fmaxf(top, p.work[((c * 2 + (c == c0)) * HB + h) * stride + p.N]);
-        for (i64 c = c0; c <= c1; ++c) {
-            const float* part = p.work + ((c * 2 + (c == c0)) * HB + h) * stride;
-            const float m = part[p.N], keep = m == -INFINITY ? 0.f : exp2f((m - top) * p.to_log2);
-            sum += part[p.N + 1] * keep;
-            if (m != -INFINITY) x += part[n] * keep;
+    // share c of the unit: in the second place of the block where it begins, in the first of the others
+    auto share = [&](int c, int h) { return p.work + (((i64)(c0 + c) * 2 + (c == 0)) * HB + h) * stride; };
+    const int lane = threadIdx.x & 31;
+    for (int h = threadIdx.x >> 5; h < heads; h += kJoinThreads / 32) {
+        float top = -INFINITY, sum = 0.f;
+        for (int c = lane; c < count; c += 32) top = fmaxf(top, weights[h * count + c] = share(c, h)[p.N]);
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        for (int c = lane; c < count; c += 32) {
+            const float m = weights[h * count + c], w = m == -INFINITY ? 0.f : exp2f((m - top) * p.to_log2);
+            weights[h * count + c] = w;
+            sum = fmaf(share(c, h)[p.N + 1], w, sum);
         }
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) {
+            weights[HB * count + h] = sum;
+            if (p.lse != nullptr) p.lse[(i64)b * p.Hq + h0 + h] = sum == 0.f ? -INFINITY : (top * p.to_log2 + log2f(sum)) * kLn2;
+        }
+    }
+    __syncthreads();
+    const int elements = heads * p.N, split = max(1, kJoinThreads / elements), slice = threadIdx.x / elements;
+    for (int i = split > 1 ? threadIdx.x % elements : threadIdx.x; i < elements; i += split > 1 ? elements : kJoinThreads) {
+        const int h = i / p.N, n = i % p.N;
+        float x = 0.f;
+        if (split == 1 || slice < split) {
+#pragma unroll 8
+            for (int c = split > 1 ? slice : 0; c < count; c += split) {
+                const float w = weights[h * count + c], v = share(c, h)[n];
+                if (w != 0.f) x = fmaf(v, w, x);   // (a share without weight may hold NaN)
+            }
+        }
+        if (split > 1) {
+            sums[threadIdx.x] = x;
+            __syncthreads();
+            if (slice != 0) break;
+            for (int q = 1; q < split; ++q) x += sums[q * elements + i];
+        }
+        const float sum = weights[HB * count + h];
         static_cast<E*>(p.out)[((i64)b * p.Hq + h0 + h) * p.N + n] = from_f<E>(sum == 0.f ? 0.f : x / sum);
-        if (n == 0 && p.lse != nullptr) p.lse[(i64)b * p.Hq + h0 + h] = sum == 0.f ? -INFINITY : (top * p.to_log2 + log2f(sum)) * kLn2;
     }
 }
 
 constexpr int kBlocksPerSm = 3;
 int run_blocks() { return max(1, sm_count()) * kBlocksPerSm; }
+template <typename E>
+int launch_join(const AttentionArgs& p, int parts, int HB, cudaStream_t st) {
+    const int smem = HB * (parts + 1) * (int)sizeof(float);   // (at most 16 heads and three shares per SM: under 48 KB up to 250 SMs)
+    join_kernel<E><<<parts - 1, kJoinThreads, smem, st>>>(p, parts, HB);
+    return check_launch("paged_attention");
+}
 int heads_of(int group) { return group >= 4 ? 4 : group >= 2 ? 2 : 1; }
 int mma_heads_of(int group) { return group > 8 ? 16 : 8; }
 
@@ -593,21 +693,39 @@ int launch(AttentionArgs& p, cudaStream_t st) {
     const int parts = run_blocks();
     attention_kernel<E, W, HB><<<parts, kThreads, 0, st>>>(p);
     if (int e = check_launch("paged_attention")) return e;
-    join_kernel<E><<<(unsigned)((i64)p.B * p.Hkv * p.blocks), kThreads, 0, st>>>(p, parts, HB);
-    return check_launch("paged_attention");
+    return launch_join<E>(p, parts, HB, st);
 }
-template <int NP, int HT>
-int launch_mma(AttentionArgs& p, cudaStream_t st) {
-    constexpr int smem = kWarps * kStages * (2 * (NP / 32) + 4 * (NP / 64)) * 32 * 16;
-    static_assert(kStages * (2 * (NP / 32) + 4 * (NP / 64)) * 32 * 16 >= 8 * HT * NP * 4, "a warp's sums fit its stages");
-    if (allow_smem<attention_mma_kernel<NP, HT>>(smem) != cudaSuccess) return check_launch("paged_attention");
+// A pool as rows of 64 or 128 elements, in boxes of [16 rows][64 elements], one behind the other for rows of 128.
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+bool make_row_map(CUtensorMap* map, const void* pool, i64 rows, int N) {
+    static const EncodeTiled encode = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) fn = nullptr;
+        return reinterpret_cast<EncodeTiled>(fn);
+    }();
+    if (encode == nullptr || tensor_maps_disabled()) return false;
+    const cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)N / 64}, strides[2] = {(cuuint64_t)N * 2, 128};
+    const cuuint32_t box[3] = {64, 16, (cuuint32_t)N / 64}, step[3] = {1, 1, 1};
+    auto make = [&] {
+        return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    return make() || (cudaFree(nullptr) == cudaSuccess && make());   // (a thread without a context yet)
+}
+
+template <int NP, int HT, bool TMA>
+int launch_mma(AttentionArgs& p, const Maps& maps, cudaStream_t st) {
+    constexpr int smem = kWarps * 4 * 2048 * (NP / 64);
+    static_assert(4 * 2048 * (NP / 64) >= 8 * HT * NP * 4, "a warp's sums fit its slots");
+    if (allow_smem<attention_mma_kernel<NP, HT, TMA>>(smem) != cudaSuccess) return check_launch("paged_attention");
     p.blocks = (p.group + 8 * HT - 1) / (8 * HT);
     p.to_log2 = 1.f;
     const int parts = run_blocks();
-    attention_mma_kernel<NP, HT><<<parts, kThreads, smem, st>>>(p);
+    attention_mma_kernel<NP, HT, TMA><<<parts, kThreads, smem, st>>>(p, maps);
     if (int e = check_launch("paged_attention")) return e;
-    join_kernel<bf16><<<(unsigned)((i64)p.B * p.Hkv * p.blocks), kThreads, 0, st>>>(p, parts, 8 * HT);
-    return check_launch("paged_attention");
+    return launch_join<bf16>(p, parts, 8 * HT, st);
 }
 // Heads of whole 16-byte pieces that start on such boundaries, and rows of the pools that an int can number.
 bool takes_mma(const AttentionArgs& p) {
@@ -617,8 +735,20 @@ bool takes_mma(const AttentionArgs& p) {
 template <typename E>
 int dispatch(AttentionArgs& p, cudaStream_t st) {
     if (sizeof(E) == 2 && takes_mma(p)) {
-        if (p.group > 8) return p.N <= 64 ? launch_mma<64, 2>(p, st) : launch_mma<128, 2>(p, st);
-        return p.N <= 64 ? launch_mma<64, 1>(p, st) : launch_mma<128, 1>(p, st);
+        Maps maps;
+        const i64 rows = (i64)p.pages * p.Hkv * p.page.d;
+        const bool tma = p.page.d % 16 == 0 && (p.N == 64 || p.N == 128) && make_row_map(&maps.keys, p.k_pages, rows, p.N) &&
+                         make_row_map(&maps.values, p.v_pages, rows, p.N);
+        switch ((p.N > 64) * 4 + (p.group > 8) * 2 + tma) {
+            case 0: return launch_mma<64, 1, false>(p, maps, st);
+            case 1: return launch_mma<64, 1, true>(p, maps, st);
+            case 2: return launch_mma<64, 2, false>(p, maps, st);
+            case 3: return launch_mma<64, 2, true>(p, maps, st);
+            case 4: return launch_mma<128, 1, false>(p, maps, st);
+            case 5: return launch_mma<128, 1, true>(p, maps, st);
+            case 6: return launch_mma<128, 2, false>(p, maps, st);
+            default: return launch_mma<128, 2, true>(p, maps, st);
+        }
     }
     p.to_log2 = kLog2e;
     const uintptr_t all = reinterpret_cast<uintptr_t>(p.k_pages) | reinterpret_cast<uintptr_t>(p.v_pages);
