@@ -42,53 +42,68 @@ struct Range {
     }
 };
 
-// All threads: the number of tiles of the units of the sequences before `end`.
-template <int THREADS>
-__device__ __forceinline__ i64 sum_block(i64 v, i64* shared) {
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) shared[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) v += shared[w];
-    return v;
-}
-template <int THREADS = kThreads>
-__device__ __forceinline__ i64 tiles_before(const AttentionArgs& p, int end, i64* shared) {
-    i64 n = 0;
-    for (int b = threadIdx.x; b < end; b += THREADS) n += Range(p, b).tiles;
-    return sum_block<THREADS>(n, shared) * (p.Hkv * p.blocks);
-}
 __device__ __forceinline__ i64 run_length(i64 all, i64 blocks) { return max((i64)kMinTiles, (all + blocks - 1) / blocks); }
 
-// The sequence that tile `begin` of all lies in, and the tiles of those before it.
-template <int THREADS = kThreads>
-__device__ __forceinline__ void find_start(const AttentionArgs& p, i64 begin, int units, i64* shared, i64* start) {
+// Where a run begins among the tiles of all units.
+struct Start {
+    i64 all, run, tile;   // tiles of all units; of a run; the run's first
+    i64 base;             // tiles of the sequences before `b`, which `tile` lies in
+    int b;
+};
+// All threads of a block: run number `index` of `runs`; tile >= all: there is none.
+template <int THREADS>
+__device__ __forceinline__ Start find_start(const AttentionArgs& p, int index, int runs, int units) {
+    __shared__ i64 sums[THREADS / 32], found[2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // up to a sequence per thread in one pass; more are gone through twice, as their sum has to be known first
+    const bool once = p.B <= THREADS;
+    Start s;
+    s.all = 0;
+    if (!once) {
+        i64 n = 0;
+        for (int b = threadIdx.x; b < p.B; b += THREADS) n += Range(p, b).tiles;
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+        if (lane == 0) sums[warp] = n;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) s.all += sums[w];
+        s.all *= units;
+        s.run = run_length(s.all, runs);
+        s.tile = s.run * index;
+        __syncthreads();
+    }
     i64 base = 0;
     for (int b0 = 0; b0 < p.B; b0 += THREADS) {
         const int b = b0 + threadIdx.x;
-        i64 n = b < p.B ? (i64)Range(p, b).tiles * units : 0, x = n;
+        const i64 n = b < p.B ? (i64)Range(p, b).tiles * units : 0;
+        i64 x = n;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const i64 o = __shfl_up_sync(0xffffffffu, x, d);
             if (lane >= d) x += o;
         }
-        __syncthreads();
-        if (lane == 31) shared[warp] = x;
+        if (lane == 31) sums[warp] = x;
         __syncthreads();
         i64 before = base;
+#pragma unroll
         for (int w = 0; w < THREADS / 32; ++w) {
-            if (w < warp) before += shared[w];
-            base += shared[w];
+            if (w < warp) before += sums[w];
+            base += sums[w];
         }
         x += before;
-        if (begin >= x - n && begin < x) start[0] = b, start[1] = x - n;
-        if (base > begin) break;   // (the same for all threads)
+        if (once) {
+            s.all = base;
+            s.run = run_length(s.all, runs);
+            s.tile = s.run * index;
+        }
+        if (s.tile >= x - n && s.tile < x) found[0] = b, found[1] = x - n;
+        __syncthreads();
+        if (base > s.tile) break;   // (the same for all threads)
     }
-    __syncthreads();
+    s.b = (int)found[0];
+    s.base = found[1];
+    return s;
 }
 
 // One sequence's cache as a lane sees it
@@ -117,19 +132,17 @@ __device__ __forceinline__ float capped(float z, float cap) { return cap > 0.f ?
 template <typename E, int W, int HB>
 __global__ void __launch_bounds__(kThreads) attention_kernel(const AttentionArgs p) {
     constexpr int kPieces = RWKVB200_MAX_HEAD_SIZE / (8 * W);
-    __shared__ i64 shared[kWarps];
     __shared__ float sO[kWarps][HB][RWKVB200_MAX_HEAD_SIZE], sM[kWarps][HB], sL[kWarps][HB];
-    __shared__ i64 sStart[2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, token = warp * 4 + (lane >> 3);
     const unsigned mask = 0xffu << (lane & 24);   // the lanes that share a token
     const int units = p.Hkv * p.blocks;
-    const i64 all = tiles_before(p, p.B, shared), run = run_length(all, gridDim.x);
-    const i64 begin = run * blockIdx.x, end = min(begin + run, all);
-    if (begin >= end) return;
-    find_start(p, begin, units, shared, sStart);
-    int b = (int)sStart[0];
-    i64 base = sStart[1];
-    for (i64 at = begin; at < end;) {
+    const Start start = find_start<kThreads>(p, blockIdx.x, gridDim.x, units);
+    const i64 end = min(start.tile + start.run, start.all);
+    if (start.tile >= end) return;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    int b = start.b;
+    i64 base = start.base;
+    for (i64 at = start.tile; at < end;) {
         const Range r(p, b);
         if (at >= base + (i64)r.tiles * units) {   // (a row without tiles is passed over as well)
             base += (i64)r.tiles * units;
@@ -324,17 +337,15 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
     constexpr int kHalves = NP / 64, kRows = 2048 * kHalves;   // bytes of 16 rows
     constexpr int kHeads = 8 * HT, kWarpBytes = 4 * kRows;     // a warp's slots: keys of two steps, values of two
     extern __shared__ __align__(1024) unsigned char staged[];
-    __shared__ i64 shared[kWarps], sStart[2];
     __shared__ float sM[kWarps][kHeads], sL[kWarps][kHeads];
     __shared__ uint64_t bars[kWarps][4];                       // TMA: one per slot
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const int units = p.Hkv * p.blocks, N = TMA ? NP : p.N;
     if (TMA && lane < 4) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(&bars[warp][lane])));
     if (TMA) v7u::proxy_fence();
-    const i64 all = tiles_before(p, p.B, shared), run = run_length(all, gridDim.x);
-    const i64 begin = run * blockIdx.x, end = min(begin + run, all);
-    if (begin >= end) return;
-    find_start(p, begin, units, shared, sStart);
+    const Start start = find_start<kThreads>(p, blockIdx.x, gridDim.x, units);
+    const i64 end = min(start.tile + start.run, start.all);
+    if (start.tile >= end) return;
     unsigned char* mine = staged + warp * kWarpBytes;
     const uint32_t base_keys = (uint32_t)__cvta_generic_to_shared(mine), base_values = base_keys + 2 * kRows;
     float* sO = reinterpret_cast<float*>(mine);                // [head][NP], between the tokens of two units
@@ -343,9 +354,10 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
     const float scale = p.cap > 0.f ? p.scale / p.cap : p.scale * kLog2e, cap = p.cap * kLog2e;
     uint32_t phases = 0;     // of the four barriers
     bool lost = false;       // a wait ran out: nothing more is asked for, and the results are NaN
-    int b = (int)sStart[0];
-    i64 base = sStart[1];
-    for (i64 at = begin; at < end;) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    int b = start.b;
+    i64 base = start.base;
+    for (i64 at = start.tile; at < end;) {
         const Range r(p, b);
         if (at >= base + (i64)r.tiles * units) {   // (a row without tiles is passed over as well)
             base += (i64)r.tiles * units;
@@ -612,33 +624,38 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
     }
 }
 
-// Joins what the `parts` blocks of a kernel above have left: block i does the unit that goes over the border of runs i and i + 1, if it
-// began in run i.  Weights of the shares first, then a thread per element of a head and kSplit-th share.
-constexpr int kJoinThreads = 512;
+// Joins what the `parts` blocks of a kernel above have left.  Block i looks at the border between runs i and i + 1: the blocks of all
+// borders that a unit goes over have an equal share of its elements each.  Weights of the runs first, then a thread per element
+// and every kSplit-th run.  It is launched while the kernel above still runs, and waits for its end before it reads what that left.
+constexpr int kJoinThreads = 256;
 template <typename E>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttentionArgs p, int parts, int HB) {
-    extern __shared__ float weights[];   // [head][share], then [head]: the sums
-    __shared__ i64 shared[kJoinThreads / 32], sStart[2];
+    extern __shared__ float weights[];   // [head][run], then [head]: the sums
     __shared__ float sums[kJoinThreads];
     const int units = p.Hkv * p.blocks;
-    const i64 all = tiles_before<kJoinThreads>(p, p.B, shared), run = run_length(all, parts);
-    const i64 border = run * (blockIdx.x + 1);
-    if (border >= all) return;
-    find_start<kJoinThreads>(p, border, units, shared, sStart);
-    const int b = (int)sStart[0];
-    const Range r(p, b);
-    const int unit = (int)((border - sStart[1]) / r.tiles);
-    const i64 begin = sStart[1] + (i64)unit * r.tiles;
-    if (begin == border || begin < border - run) return;   // nothing goes over the border, or it began earlier
-    const int c0 = blockIdx.x, count = (int)((begin + r.tiles - 1) / run) - c0 + 1;
+    const Start start = find_start<kJoinThreads>(p, blockIdx.x + 1, parts, units);
+    const i64 border = start.tile, run = start.run;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // (all blocks: this kernel must not end before the other)
+    if (border >= start.all) return;
+    const int b = start.b, tiles = Range(p, b).tiles;
+    const int unit = (int)((border - start.base) / tiles);
+    const i64 begin = start.base + (i64)unit * tiles;
+    if (begin == border) return;   // nothing goes over it
+    const int c0 = (int)(begin / run), count = (int)((begin + tiles - 1) / run) - c0 + 1, mine = blockIdx.x - c0;
     const int head = unit / p.blocks, h0 = head * p.group + unit % p.blocks * HB, heads = min(HB, (head + 1) * p.group - h0);
+    const int elements = heads * p.N, e0 = (int)((i64)elements * mine / (count - 1)), e1 = (int)((i64)elements * (mine + 1) / (count - 1));
+    const int first = e0 / p.N, last = (e1 - 1) / p.N;   // heads
     const int stride = p.N + 2;
-    // share c of the unit: in the second place of the block where it begins, in the first of the others
+    // what run c left of the unit: in the second place of the block where the unit begins, in the first of the others
     auto share = [&](int c, int h) { return p.work + (((i64)(c0 + c) * 2 + (c == 0)) * HB + h) * stride; };
     const int lane = threadIdx.x & 31;
-    for (int h = threadIdx.x >> 5; h < heads; h += kJoinThreads / 32) {
+    for (int h = first + (threadIdx.x >> 5); h <= last; h += kJoinThreads / 32) {
         float top = -INFINITY, sum = 0.f;
-        for (int c = lane; c < count; c += 32) top = fmaxf(top, weights[h * count + c] = share(c, h)[p.N]);
+        for (int c = lane; c < count; c += 32) {
+            const float m = share(c, h)[p.N];
+            weights[h * count + c] = m;
+            top = fmaxf(top, m);
+        }
 #pragma unroll
         for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         for (int c = lane; c < count; c += 32) {
@@ -650,29 +667,32 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttentionArgs 
         for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (lane == 0) {
             weights[HB * count + h] = sum;
-            if (p.lse != nullptr) p.lse[(i64)b * p.Hq + h0 + h] = sum == 0.f ? -INFINITY : (top * p.to_log2 + log2f(sum)) * kLn2;
+            if (p.lse != nullptr && h * p.N >= e0) p.lse[(i64)b * p.Hq + h0 + h] = sum == 0.f ? -INFINITY : (top * p.to_log2 + log2f(sum)) * kLn2;
         }
     }
     __syncthreads();
-    const int elements = heads * p.N, split = max(1, kJoinThreads / elements), slice = threadIdx.x / elements;
-    for (int i = split > 1 ? threadIdx.x % elements : threadIdx.x; i < elements; i += split > 1 ? elements : kJoinThreads) {
-        const int h = i / p.N, n = i % p.N;
+    const int width = min(e1 - e0, kJoinThreads), split = kJoinThreads / width, slice = threadIdx.x / width;
+    for (int i0 = e0; i0 < e1; i0 += width) {   // (the same steps for all threads)
+        const int i = i0 + threadIdx.x % width, h = i / p.N, n = i % p.N;
         float x = 0.f;
-        if (split == 1 || slice < split) {
-#pragma unroll 8
-            for (int c = split > 1 ? slice : 0; c < count; c += split) {
+        if (i < e1 && slice < split) {
+#pragma unroll 4
+            for (int c = slice; c < count; c += split) {
                 const float w = weights[h * count + c], v = share(c, h)[n];
-                if (w != 0.f) x = fmaf(v, w, x);   // (a share without weight may hold NaN)
+                if (w != 0.f) x = fmaf(v, w, x);   // (a run without weight may hold NaN)
             }
         }
         if (split > 1) {
             sums[threadIdx.x] = x;
             __syncthreads();
-            if (slice != 0) break;
-            for (int q = 1; q < split; ++q) x += sums[q * elements + i];
+            if (slice == 0)
+                for (int q = 1; q < split; ++q) x += sums[q * width + threadIdx.x];
+            __syncthreads();
         }
-        const float sum = weights[HB * count + h];
-        static_cast<E*>(p.out)[((i64)b * p.Hq + h0 + h) * p.N + n] = from_f<E>(sum == 0.f ? 0.f : x / sum);
+        if (slice == 0 && i < e1) {
+            const float sum = weights[HB * count + h];
+            static_cast<E*>(p.out)[((i64)b * p.Hq + h0 + h) * p.N + n] = from_f<E>(sum == 0.f ? 0.f : x / sum);
+        }
     }
 }
 
@@ -681,7 +701,17 @@ int run_blocks() { return max(1, sm_count()) * kBlocksPerSm; }
 template <typename E>
 int launch_join(const AttentionArgs& p, int parts, int HB, cudaStream_t st) {
     const int smem = HB * (parts + 1) * (int)sizeof(float);   // (at most 16 heads and three shares per SM: under 48 KB up to 250 SMs)
-    join_kernel<E><<<parts - 1, kJoinThreads, smem, st>>>(p, parts, HB);
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(parts - 1);
+    config.blockDim = dim3(kJoinThreads);
+    config.dynamicSmemBytes = smem;
+    config.stream = st;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    cudaLaunchKernelEx(&config, join_kernel<E>, p, parts, HB);
     return check_launch("paged_attention");
 }
 int heads_of(int group) { return group >= 4 ? 4 : group >= 2 ? 2 : 1; }
