@@ -3,11 +3,12 @@
 //   z_j = scale q.k_j      z_j = cap tanh(z_j / cap)      z_j += slope_h (j - (len - 1))      max(0, len - window) <= j < len
 //   out = sum_j exp(z_j - m) v_j / sum_j exp(z_j - m)     lse = m + log(sum)                  m = max_j z_j
 //
-// The keys and values of the sequences are read once; memory bounds it.  The work is all tiles of kTile tokens of all units (a
+// The keys and values of the sequences are read once; memory bounds it.  The work is all tiles (of 64 or 32 tokens) of all units (a
 // sequence, a key-value head, a block of its query heads) behind one another; every block takes an equal run of them, so that
 // one long sequence and many of different lengths both fill the GPU.  A unit that lies in one block's run is finished there; of
 // the others each block leaves (m, sum, sum of exp v) and a second kernel joins them.  A block's run has at most one unit that
 // began before it and one that ends behind it: two places a block.
+#include "packed.cuh"
 #include "paged.cuh"
 #include "wkv7_umma.cuh"
 #include <cuda.h>
@@ -17,11 +18,11 @@ namespace {
 
 __device__ int g_error = 0;
 constexpr int kThreads = 128, kWarps = kThreads / 32;
-constexpr int kTile = 64;
-constexpr int kMinTiles = 4;      // a block's run: fewer would cost more to join than they save
+constexpr int kMinTokens = 256;   // of a block's run: fewer would cost more to join than they save
 
 struct AttentionArgs {
     int B, Hq, Hkv, N, pages, width, window, group, blocks;   // blocks of query heads per key-value head
+    int tile_bits;                                            // a tile has 1 << tile_bits tokens, 16 or 8 for each warp
     float scale, cap, to_log2;   // to_log2: what makes the partial maxima exponents of 2
     Divisor page;
     const void *q, *k_pages, *v_pages;
@@ -38,11 +39,11 @@ struct Range {
         hi = min(p.lengths[b], p.width * (int)p.page.d);
         lo = p.window > 0 ? max(0, hi - p.window) : 0;
         start = lo & ~15;
-        tiles = hi < 0 ? 0 : max(1, (hi - start + kTile - 1) / kTile);
+        tiles = hi < 0 ? 0 : max(1, (hi - start + (1 << p.tile_bits) - 1) >> p.tile_bits);
     }
 };
 
-__device__ __forceinline__ i64 run_length(i64 all, i64 blocks) { return max((i64)kMinTiles, (all + blocks - 1) / blocks); }
+__device__ __forceinline__ i64 run_length(const AttentionArgs& p, i64 all, int blocks) { return max((i64)(kMinTokens >> p.tile_bits), (all + blocks - 1) / blocks); }
 
 // Where a run begins among the tiles of all units.
 struct Start {
@@ -69,7 +70,7 @@ __device__ __forceinline__ Start find_start(const AttentionArgs& p, int index, i
 #pragma unroll
         for (int w = 0; w < THREADS / 32; ++w) s.all += sums[w];
         s.all *= units;
-        s.run = run_length(s.all, runs);
+        s.run = run_length(p, s.all, runs);
         s.tile = s.run * index;
         __syncthreads();
     }
@@ -94,7 +95,7 @@ __device__ __forceinline__ Start find_start(const AttentionArgs& p, int index, i
         x += before;
         if (once) {
             s.all = base;
-            s.run = run_length(s.all, runs);
+            s.run = run_length(p, s.all, runs);
             s.tile = s.run * index;
         }
         if (s.tile >= x - n && s.tile < x) found[0] = b, found[1] = x - n;
@@ -172,8 +173,8 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const AttentionArgs
         struct alignas(sizeof(E) * W) Piece {
             E e[W];
         };
-        const int last = min(r.start + t1 * kTile, r.hi);
-        for (int j = r.start + t0 * kTile + token; j < last; j += kWarps * 4) {
+        const int last = min(r.start + (t1 << p.tile_bits), r.hi);
+        for (int j = r.start + (t0 << p.tile_bits) + token; j < last; j += kWarps * 4) {
             if (j < r.lo) continue;
             const i64 place = cache.at(j);
             const bool found = place >= 0;
@@ -263,16 +264,14 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const AttentionArgs
     }
 }
 
-// bf16, heads of whole 16-byte pieces: products on mma.sync m16n8k16 with the tokens in the rows, S^T = K q^T and O^T = V^T P^T, for up
-// to 8 HT query heads that share the keys: HT = 1 wastes nothing on groups of 8, and memory bounds both anyway.  Each warp takes
-// 16 of a tile's tokens and keeps its own maxima and sums.  Both operands come out of shared memory by ldmatrix (the values transposed), from
-// tiles of [16 tokens][64 elements] in the 128-byte swizzle.  They get there
-//   TMA:  by one bulk copy of 16 rows each for keys and values (pages of a multiple of 16 tokens, heads of 64 or 128): a warp's
-//         lane 0 asks, keys two steps ahead and values one, and counts the bytes on a barrier of the slot;
-//   else: by cp.async in pieces of 16 bytes, rows that do not count filled with zeros.  (Taken for every page size, with a lane's
-//         pieces in places of its own, this read 4.0 TB/s at 128 sequences of up to 4096 tokens; without any product 4.1.)
-// Weights are taken into the second product as the sum of two bf16 numbers (2^-16 relative; one would double the output's
-// rounding), both above 0, so that an infinite value stays one.
+// ---- kernels that bring a warp's tokens through shared memory ------------------------------------------------------------
+// A step of a warp is 16 (bf16) or 8 (fp32) tokens.  Their keys and values lie in shared memory as boxes of [tokens][128 bytes] in the
+// 128-byte swizzle (piece c of 16 bytes of row t is at c ^ (t & 7)), one behind the other for longer rows; a warp has slots for
+// the keys of two steps and the values of two.  They get there
+//   TMA:  by one bulk copy each (pages of a multiple of 16 tokens, rows of 128, 256 or 512 bytes): a warp's lane 0 asks, keys two
+//         steps ahead and values one, and counts the bytes on a barrier of the slot.  A step lies in one page: one lookup;
+//   else: by cp.async in pieces of 16 bytes, rows that do not count filled with zeros.
+// (128 sequences of up to 4096 tokens: 205 us by TMA; 273 us by cp.async, 267 of them without any product.)
 constexpr int kTimeout = 3;       // a wait for a copy ran out
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -310,7 +309,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&t);
 }
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copy_or_zero(uint32_t shared, const bf16* from, bool there) {
+__device__ __forceinline__ void copy_or_zero(uint32_t shared, const void* from, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 
@@ -320,7 +319,7 @@ __device__ __forceinline__ void ldmatrix(uint32_t (&d)[4], uint32_t at) {
 __device__ __forceinline__ void ldmatrix_transposed(uint32_t (&d)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : "r"(at) : "memory");
 }
-// 16 rows of a pool, from number `row` on, counted on `bar`
+// a step's rows of a pool, from number `row` on, counted on `bar`
 __device__ __forceinline__ void copy_rows(uint32_t to, const CUtensorMap* map, int row, uint64_t* bar, int bytes) {
     const uint32_t b = (uint32_t)__cvta_generic_to_shared(bar);
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(bytes) : "memory");
@@ -332,29 +331,149 @@ struct Maps {
     CUtensorMap keys, values;
 };
 
+// A warp's part of a unit: tokens, pages and slots.
+template <typename E, int NP, bool TMA>
+struct Steps {
+    static constexpr int kTokens = sizeof(E) == 2 ? 16 : 8, kBoxes = NP * (int)sizeof(E) / 128, kBox = kTokens * 128, kRows = kBox * kBoxes;
+    static constexpr int kWarpBytes = 4 * kRows;   // the slots: keys, keys, values, values
+    const AttentionArgs& p;
+    const Maps& maps;
+    uint64_t* bars;          // TMA: one per slot
+    uint32_t slots;          // address in shared memory
+    int lane;
+    uint32_t phases = 0;     // of the four barriers
+    bool lost = false;       // a wait ran out: nothing more is asked for, and the results are NaN
+    // the unit
+    const int* row;
+    int head, lo, from, last, steps;
+
+    __device__ __forceinline__ Steps(const AttentionArgs& p, const Maps& maps, uint64_t* bars, void* slots, int lane)
+        : p(p), maps(maps), bars(bars), slots((uint32_t)__cvta_generic_to_shared(slots)), lane(lane) {
+        if (TMA && lane < 4) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(&bars[lane])));
+        if (TMA) v7u::proxy_fence();
+    }
+    __device__ __forceinline__ void unit(int b, const Range& r, int t0, int t1, int head_, int warp) {
+        row = p.table + (i64)b * p.width;
+        head = head_;
+        lo = r.lo;
+        from = r.start + (t0 << p.tile_bits) + warp * kTokens;
+        last = min(r.start + (t1 << p.tile_bits), r.hi);
+        steps = lost ? 0 : t1 - t0;
+    }
+    __device__ __forceinline__ int first(int step) const { return from + (step << p.tile_bits); }
+    __device__ __forceinline__ bool counts(int j) const { return j >= lo && j < last; }
+    // Of a step's tokens a lane answers for one (TMA: all for the first).  Its page is asked for a step before it is looked at.
+    __device__ __forceinline__ int token(int step) const { return first(step) + (TMA ? 0 : lane & (kTokens - 1)); }
+    __device__ __forceinline__ bool in_use(int step, int j) const { return step < steps && (TMA ? j < last : counts(j)); }
+    __device__ __forceinline__ int page(int step) const {
+        const int j = token(step);
+        return in_use(step, j) ? row[p.page.quotient((uint32_t)j)] : 0;
+    }
+    // the row of the pools that the token lies in; -1: it does not count
+    __device__ __forceinline__ int place(int step, int id) const {
+        const int j = token(step);
+        if (!in_use(step, j)) return -1;
+        if ((unsigned)id >= (unsigned)p.pages) {
+            atomicMax(&g_error, kBadPage);
+            return -1;
+        }
+        return (id * p.Hkv + head) * (int)p.page.d + (j - (int)(p.page.quotient((uint32_t)j) * p.page.d));
+    }
+    // whether token t of a step counts, from its place n
+    __device__ __forceinline__ bool there(int step, int n, int t) const {
+        return TMA ? n >= 0 && counts(first(step) + t) : __shfl_sync(0xffffffffu, n, t) >= 0;
+    }
+    __device__ __forceinline__ uint32_t keys(int step) const { return slots + (step & 1) * kRows; }
+    __device__ __forceinline__ uint32_t values(int step) const { return slots + (2 + (step & 1)) * kRows; }
+    template <bool VALUES>
+    __device__ __forceinline__ void ask(int step, int n) const {
+        const uint32_t to = VALUES ? values(step) : keys(step);
+        if (TMA) {
+            if (lane == 0 && n >= 0) copy_rows(to, VALUES ? &maps.values : &maps.keys, n, &bars[VALUES * 2 + (step & 1)], kRows);
+        } else {
+            constexpr int kPer = 16 / sizeof(E);
+            const E* pool = static_cast<const E*>(VALUES ? p.v_pages : p.k_pages);
+#pragma unroll
+            for (int i = 0; i < kRows / 512; ++i) {
+                const int piece = i * 32 + lane, t = piece / (8 * kBoxes), c = piece % (8 * kBoxes);
+                const int k = __shfl_sync(0xffffffffu, n, t);
+                copy_or_zero(to + (c >> 3) * kBox + t * 128 + (((c ^ t) & 7) << 4), pool + (i64)max(k, 0) * p.N + min(c * kPer, p.N - kPer), k >= 0 && c * kPer < p.N);
+            }
+        }
+    }
+    // waits for the copies of all but the last group (TMA: for those that have been asked for)
+    template <bool VALUES>
+    __device__ __forceinline__ void arrived(int step, int n) {
+        if (!TMA) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        } else if (n >= 0) {
+            const int which = VALUES * 2 + (step & 1);
+            if (__any_sync(0xffffffffu, !v7u::mbar_wait(&bars[which], phases >> which & 1))) lost = true;
+            phases ^= 1u << which;
+        }
+    }
+    __device__ __forceinline__ void finish() {   // nothing is in flight behind it
+        if (!TMA) asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (lost) {
+            for (int i = 0; i < 4; ++i) v7u::mbar_wait(&bars[i], phases >> i & 1, 1 << 10);
+            if (lane == 0) atomicMax(&g_error, kTimeout);
+        }
+        __syncwarp();
+    }
+};
+
+// The sums of a unit's warps, sO [head][NP] behind one another every `stride` floats, with their maxima (as exponents of 2) and
+// weights: joined, and written as results or as this block's share.
+template <typename E, int NP, int HEADS>
+__device__ __forceinline__ void write_unit(const AttentionArgs& p, const float* sO, int stride, const float (*sM)[HEADS], const float (*sL)[HEADS], int b, int h0,
+                                           int heads, bool whole, bool begins) {
+    float* part = p.work + ((i64)blockIdx.x * 2 + begins) * HEADS * (p.N + 2);
+    for (int i = threadIdx.x; i < heads * NP; i += kThreads) {
+        const int h = i / NP, n = i % NP;
+        if (n >= p.N) continue;
+        float top = -INFINITY, x = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sM[w][h]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float keep = sM[w][h] == -INFINITY ? 0.f : ex2(sM[w][h] - top);
+            sum += sL[w][h] * keep;
+            // (a warp whose maximum is -infinity has sums of zeros, or NaN from a NaN score)
+            if (sM[w][h] != -INFINITY) x += sO[w * stride + h * NP + n] * keep;
+        }
+        if (whole) {
+            static_cast<E*>(p.out)[((i64)b * p.Hq + h0 + h) * p.N + n] = from_f<E>(sum == 0.f ? 0.f : x / sum);
+            if (n == 0 && p.lse != nullptr) p.lse[(i64)b * p.Hq + h0 + h] = sum == 0.f ? -INFINITY : top * kLn2 + logf(sum);
+        } else {
+            part[h * (p.N + 2) + n] = x;
+            if (n == 0) part[h * (p.N + 2) + p.N] = top, part[h * (p.N + 2) + p.N + 1] = sum;
+        }
+    }
+}
+
+// bf16, heads of whole 16-byte pieces: products on mma.sync m16n8k16 with the tokens in the rows, S^T = K q^T and O^T = V^T P^T, for up
+// to 8 HT query heads that share the keys: HT = 1 wastes nothing on groups of 8, and memory bounds both anyway.  Each warp
+// keeps its own maxima and sums.  Both first operands come out of shared memory by ldmatrix (the values transposed).
+// Weights are taken into the second product as the sum of two bf16 numbers (2^-16 relative; one would double the output's
+// rounding), both above 0, so that an infinite value stays one.
 template <int NP, int HT, bool TMA>
 __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const AttentionArgs p, const __grid_constant__ Maps maps) {
-    constexpr int kHalves = NP / 64, kRows = 2048 * kHalves;   // bytes of 16 rows
-    constexpr int kHeads = 8 * HT, kWarpBytes = 4 * kRows;     // a warp's slots: keys of two steps, values of two
+    using Way = Steps<bf16, NP, TMA>;
+    constexpr int kHeads = 8 * HT;
     extern __shared__ __align__(1024) unsigned char staged[];
     __shared__ float sM[kWarps][kHeads], sL[kWarps][kHeads];
-    __shared__ uint64_t bars[kWarps][4];                       // TMA: one per slot
+    __shared__ uint64_t bars[kWarps][4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const int units = p.Hkv * p.blocks, N = TMA ? NP : p.N;
-    if (TMA && lane < 4) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"((uint32_t)__cvta_generic_to_shared(&bars[warp][lane])));
-    if (TMA) v7u::proxy_fence();
+    unsigned char* mine = staged + warp * Way::kWarpBytes;
+    Way way(p, maps, bars[warp], mine, lane);
     const Start start = find_start<kThreads>(p, blockIdx.x, gridDim.x, units);
     const i64 end = min(start.tile + start.run, start.all);
     if (start.tile >= end) return;
-    unsigned char* mine = staged + warp * kWarpBytes;
-    const uint32_t base_keys = (uint32_t)__cvta_generic_to_shared(mine), base_values = base_keys + 2 * kRows;
-    float* sO = reinterpret_cast<float*>(mine);                // [head][NP], between the tokens of two units
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // where a lane's rows for ldmatrix lie: keys: rows lane & 15, piece lane / 16; values: rows by 8 from lane / 16, piece by lane / 8
     const uint32_t key_row = (lane & 15) * 128, key_piece = lane >> 4, value_row = ((lane & 7) + (lane >> 4) * 8) * 128, value_piece = lane >> 3 & 1, swizzle = lane & 7;
     const float scale = p.cap > 0.f ? p.scale / p.cap : p.scale * kLog2e, cap = p.cap * kLog2e;
-    uint32_t phases = 0;     // of the four barriers
-    bool lost = false;       // a wait ran out: nothing more is asked for, and the results are NaN
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int b = start.b;
     i64 base = start.base;
     for (i64 at = start.tile; at < end;) {
@@ -368,55 +487,14 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
         at += t1 - t0;
         const int head = unit / p.blocks, h0 = head * p.group + unit % p.blocks * kHeads, heads = min(kHeads, (head + 1) * p.group - h0);
         if (threadIdx.x == 0 && p.lengths[b] > r.hi) atomicMax(&g_error, kBadLength);
-        const int* row = p.table + (i64)b * p.width;
-        const int from = r.start + t0 * kTile + warp * 16, last = min(r.start + t1 * kTile, r.hi), steps = lost ? 0 : t1 - t0;
-        // Of a step's tokens the lane answers for number lane & 15 (TMA: all for the first: they share a page).  Its page is asked for a
-        // step before it is looked at.
-        auto counts = [&](int j) { return j >= r.lo && j < last; };
-        auto token_of = [&](int step) { return from + step * kTile + (TMA ? 0 : lane & 15); };
-        auto in_use = [&](int step, int j) { return step < steps && (TMA ? j < last : counts(j)); };
-        auto page_of = [&](int step) {
-            const int j = token_of(step);
-            return in_use(step, j) ? row[p.page.quotient((uint32_t)j)] : 0;
-        };
-        // the row of the pools that the token lies in; -1: it does not count
-        auto row_of = [&](int step, int id) {
-            const int j = token_of(step);
-            if (!in_use(step, j)) return -1;
-            if ((unsigned)id >= (unsigned)p.pages) {
-                atomicMax(&g_error, kBadPage);
-                return -1;
-            }
-            return (id * p.Hkv + head) * (int)p.page.d + (j - (int)(p.page.quotient((uint32_t)j) * p.page.d));
-        };
-        auto ask = [&](bool values, int step, int n) {
-            const int slot = step & 1;
-            const uint32_t to = (values ? base_values : base_keys) + slot * kRows;
-            if (TMA) {
-                if (lane == 0 && n >= 0) copy_rows(to, values ? &maps.values : &maps.keys, n, &bars[warp][values * 2 + slot], kRows);
-            } else {
-                const bf16* pool = static_cast<const bf16*>(values ? p.v_pages : p.k_pages);
-#pragma unroll
-                for (int i = 0; i < kRows / 512; ++i) {
-                    const int piece = i * 32 + lane, token = piece / (8 * kHalves), c = piece % (8 * kHalves);
-                    const int k = __shfl_sync(0xffffffffu, n, token);
-                    copy_or_zero(to + (c >> 3) * 2048 + token * 128 + (((c ^ token) & 7) << 4), pool + (i64)max(k, 0) * N + min(c * 8, N - 8), k >= 0 && c * 8 < N);
-                }
-            }
-        };
-        auto arrived = [&](bool values, int step, int n) {   // TMA: waits for what has been asked for
-            const int which = values * 2 + (step & 1);
-            if (!TMA || n < 0) return;
-            if (__any_sync(0xffffffffu, !v7u::mbar_wait(&bars[warp][which], phases >> which & 1))) lost = true;
-            phases ^= 1u << which;
-        };
-        const int id0 = page_of(0), id1 = page_of(1);
-        int id2 = page_of(2);
-        int n0 = row_of(0, id0), n1 = row_of(1, id1);
-        ask(false, 0, n0);
+        way.unit(b, r, t0, t1, head, warp);
+        const int id0 = way.page(0), id1 = way.page(1);
+        int id2 = way.page(2);
+        int n0 = way.place(0, id0), n1 = way.place(1, id1);
+        way.template ask<false>(0, n0);
         commit();
-        ask(false, 1, n1);
-        ask(true, 0, n0);
+        way.template ask<false>(1, n1);
+        way.template ask<true>(0, n0);
         commit();
         // q as the second operand of the scores: head g (and g + 8)
         uint32_t qf[HT][NP / 16][2];
@@ -446,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
         // The scores of a step are made while the step before it is summed.
         float next[HT][4];
         auto scores = [&](int step) {
-            const uint32_t in = base_keys + (step & 1) * kRows + key_row;
+            const uint32_t in = way.keys(step) + key_row;
 #pragma unroll
             for (int h = 0; h < HT; ++h)
 #pragma unroll
@@ -454,30 +532,28 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
 #pragma unroll
             for (int j = 0; j < NP / 16; ++j) {
                 uint32_t a[4];
-                ldmatrix(a, in + j / 4 * 2048 + (((j % 4 * 2 + key_piece) ^ swizzle) << 4));
+                ldmatrix(a, in + j / 4 * Way::kBox + (((j % 4 * 2 + key_piece) ^ swizzle) << 4));
 #pragma unroll
                 for (int h = 0; h < HT; ++h) mma(next[h], a[0], a[1], a[2], a[3], qf[h][j][0], qf[h][j][1]);
             }
         };
-        if (!TMA) asm volatile("cp.async.wait_group 1;" ::: "memory");
-        arrived(false, 0, n0);
+        way.template arrived<false>(0, n0);
         __syncwarp();
         scores(0);
-        for (int step = 0; step < steps && !lost; ++step) {
+        for (int step = 0; step < way.steps && !way.lost; ++step) {
             float z[HT][4];
 #pragma unroll
             for (int h = 0; h < HT; ++h)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) z[h][e] = next[h][e];
-            const int n2 = row_of(step + 2, id2);
-            id2 = page_of(step + 3);
+            const int n2 = way.place(step + 2, id2);
+            id2 = way.page(step + 3);
             __syncwarp();                 // (all lanes have read the slots that are asked for)
-            ask(false, step + 2, n2);
-            ask(true, step + 1, n1);
+            way.template ask<false>(step + 2, n2);
+            way.template ask<true>(step + 1, n1);
             commit();
-            if (!TMA) asm volatile("cp.async.wait_group 1;" ::: "memory");
-            arrived(false, step + 1, n1);
-            arrived(true, step, n0);
+            way.template arrived<false>(step + 1, n1);
+            way.template arrived<true>(step, n0);
             __syncwarp();
             scores(step + 1);
             const int n = n0;
@@ -485,9 +561,8 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
             n1 = n2;
             if (!__any_sync(0xffffffffu, n >= 0)) continue;   // no token counts
             // scores as exponents of 2: tokens g (elements 0, 1) and g + 8 (2, 3)
-            const int j = from + step * kTile + g;
-            const bool there[2] = {TMA ? counts(j) : __shfl_sync(0xffffffffu, n, g) >= 0, TMA ? counts(j + 8) : __shfl_sync(0xffffffffu, n, g + 8) >= 0};
-            const float distance = (float)(j - (r.hi - 1));
+            const bool there[2] = {way.there(step, n, g), way.there(step, n, g + 8)};
+            const float distance = (float)(way.first(step) + g - (r.hi - 1));
             bool more = false, none = false;   // a new maximum; a score of -infinity
 #pragma unroll
             for (int h = 0; h < HT; ++h)
@@ -520,7 +595,6 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
                         for (int e = 0; e < 4; ++e) o[h][i][e] *= keep[e & 1];
                 }
             }
-            const uint32_t in = base_values + (step & 1) * kRows;
             if (__any_sync(0xffffffffu, none)) {
                 // a token without weight in any head counts for nothing, whatever its value (or the memory behind the last token) holds
                 bool dead[2] = {true, true};
@@ -535,8 +609,8 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
                     gone = gone & gone >> 2 & 0x11111111u;   // bit 4 t: token t (+ 8)
                     for (; gone != 0; gone &= gone - 1) {
                         const int token = i * 8 + (__ffs(gone) - 1) / 4;
-                        if (lane < 8 * kHalves) {
-                            unsigned char* to = mine + 2 * kRows + (step & 1) * kRows + lane / 8 * 2048 + token * 128 + lane % 8 * 16;
+                        if (lane < 8 * Way::kBoxes) {
+                            unsigned char* to = mine + (2 + (step & 1)) * Way::kRows + lane / 8 * Way::kBox + token * 128 + lane % 8 * 16;
                             *reinterpret_cast<uint4*>(to) = make_uint4(0, 0, 0, 0);
                         }
                     }
@@ -562,10 +636,11 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
                     low[h][i] = transposed(pack_bf16(y[2 * i], y[2 * i + 1]));
                 }
             }
+            const uint32_t in = way.values(step) + value_row;
 #pragma unroll
             for (int i = 0; i < NP / 16; ++i) {
                 uint32_t a[4];
-                ldmatrix_transposed(a, in + value_row + i / 4 * 2048 + (((i % 4 * 2 + value_piece) ^ swizzle) << 4));
+                ldmatrix_transposed(a, in + i / 4 * Way::kBox + (((i % 4 * 2 + value_piece) ^ swizzle) << 4));
 #pragma unroll
                 for (int h = 0; h < HT; ++h) {
                     mma(o[h][i], a[0], a[1], a[2], a[3], high[h][0], high[h][1]);
@@ -573,19 +648,14 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
                 }
             }
         }
-        if (!TMA) asm volatile("cp.async.wait_group 0;" ::: "memory");
-        if (lost) {   // what may still be in flight, and results that cannot pass as such
-            for (int i = 0; i < 4; ++i) v7u::mbar_wait(&bars[warp][i], phases >> i & 1, 1 << 10);
-            if (lane == 0) atomicMax(&g_error, kTimeout);
-#pragma unroll
-            for (int h = 0; h < HT; ++h) m[h][0] = m[h][1] = 0.f, l[h][0] = l[h][1] = __int_as_float(0x7fffffff);
-        }
-        __syncwarp();
-        // the warp's shares: O^T back to heads in rows
+        way.finish();
+        // the warp's shares, in its slots: O^T back to heads in rows
+        float* sO = reinterpret_cast<float*>(mine);
 #pragma unroll
         for (int h = 0; h < HT; ++h) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
+                if (way.lost) m[h][e] = 0.f, l[h][e] = __int_as_float(0x7fffffff);   // results that cannot pass as such
 #pragma unroll
                 for (int d = 4; d <= 16; d <<= 1) l[h][e] += __shfl_xor_sync(0xffffffffu, l[h][e], d);
                 if (g == 0) sM[warp][h * 8 + 2 * q + e] = m[h][e], sL[warp][h * 8 + 2 * q + e] = l[h][e];
@@ -596,29 +666,205 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
                 for (int e = 0; e < 4; ++e) sO[(h * 8 + 2 * q + (e & 1)) * NP + i * 16 + g + (e >> 1) * 8] = o[h][i][e];
         }
         __syncthreads();
-        const bool whole = t0 == 0 && t1 == r.tiles;
-        float* part = p.work + ((i64)blockIdx.x * 2 + (t0 == 0)) * kHeads * (N + 2);
-        for (int i = threadIdx.x; i < heads * NP; i += kThreads) {
+        write_unit<bf16, NP, kHeads>(p, reinterpret_cast<const float*>(staged), Way::kWarpBytes / 4, sM, sL, b, h0, heads, t0 == 0 && t1 == r.tiles, t0 == 0);
+        if (TMA) v7u::proxy_fence();
+        __syncthreads();
+    }
+}
+
+// fp32, heads of whole 16-byte pieces, for up to HB query heads that share the keys.  Scores: lane (part, t) takes a quarter of key t
+// times all queries (which lie in shared memory, scaled), and the quarters are added so that lane (part, t) ends with the scores of
+// HB / 4 heads.  Sums: a lane has NP / 32 elements of every head, the weights of a token come out of shared memory.
+template <int NP, int HB, bool TMA>
+__global__ void __launch_bounds__(kThreads, 3) attention_fp32_kernel(const AttentionArgs p, const __grid_constant__ Maps maps) {
+    using Way = Steps<float, NP, TMA>;
+    constexpr int kMine = HB / 4, kQuarter = NP / 4, kPad = kQuarter + 4;   // (padded: the four quarters are read at once)
+    extern __shared__ __align__(1024) unsigned char staged[];
+    __shared__ float sM[kWarps][HB], sL[kWarps][HB];
+    __shared__ __align__(16) float sQ[HB][4][kPad], sW[kWarps][8][HB];
+    __shared__ uint64_t bars[kWarps][4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 7, part = lane >> 3;
+    const int units = p.Hkv * p.blocks;
+    unsigned char* mine = staged + warp * Way::kWarpBytes;
+    Way way(p, maps, bars[warp], mine, lane);
+    const Start start = find_start<kThreads>(p, blockIdx.x, gridDim.x, units);
+    const i64 end = min(start.tile + start.run, start.all);
+    if (start.tile >= end) return;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const float scale = p.cap > 0.f ? p.scale / p.cap : p.scale * kLog2e, cap = p.cap * kLog2e;
+    int b = start.b;
+    i64 base = start.base;
+    for (i64 at = start.tile; at < end;) {
+        const Range r(p, b);
+        if (at >= base + (i64)r.tiles * units) {   // (a row without tiles is passed over as well)
+            base += (i64)r.tiles * units;
+            ++b;
+            continue;
+        }
+        const int unit = (int)((at - base) / r.tiles), t0 = (int)((at - base) % r.tiles), t1 = (int)min((i64)r.tiles, t0 + (end - at));
+        at += t1 - t0;
+        const int head = unit / p.blocks, h0 = head * p.group + unit % p.blocks * HB, heads = min(HB, (head + 1) * p.group - h0);
+        if (threadIdx.x == 0 && p.lengths[b] > r.hi) atomicMax(&g_error, kBadLength);
+        way.unit(b, r, t0, t1, head, warp);
+        const int id0 = way.page(0), id1 = way.page(1);
+        int id2 = way.page(2);
+        int n0 = way.place(0, id0), n1 = way.place(1, id1);
+        way.template ask<false>(0, n0);
+        commit();
+        way.template ask<false>(1, n1);
+        way.template ask<true>(0, n0);
+        commit();
+        for (int i = threadIdx.x; i < HB * NP; i += kThreads) {
             const int h = i / NP, n = i % NP;
-            if (n >= N) continue;
-            float top = -INFINITY, x = 0.f, sum = 0.f;
+            sQ[h][n / kQuarter][n % kQuarter] = h < heads && n < p.N ? static_cast<const float*>(p.q)[((i64)b * p.Hq + h0 + h) * p.N + n] * scale : 0.f;
+        }
+        __syncthreads();
+        float slope[kMine], m[kMine], l[kMine];   // heads part * kMine + i
+        f2 o[HB][NP / 64];
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sM[w][h]);
+        for (int i = 0; i < kMine; ++i) {
+            slope[i] = p.slopes != nullptr && part * kMine + i < heads ? p.slopes[h0 + part * kMine + i] * kLog2e : 0.f;
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+        }
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float keep = sM[w][h] == -INFINITY ? 0.f : ex2(sM[w][h] - top);
-                sum += sL[w][h] * keep;
-                // (a warp whose maximum is -infinity has sums of zeros, or NaN from a NaN score)
-                if (sM[w][h] != -INFINITY) x += reinterpret_cast<const float*>(staged + w * kWarpBytes)[h * NP + n] * keep;
+        for (int h = 0; h < HB; ++h)
+#pragma unroll
+            for (int e = 0; e < NP / 64; ++e) o[h][e] = 0;
+        float next[kMine];
+        auto scores = [&](int step) {
+            const unsigned char* in = mine + (step & 1) * Way::kRows + t * 128;
+            f2 sum[HB];
+#pragma unroll
+            for (int h = 0; h < HB; ++h) sum[h] = 0;
+#pragma unroll
+            for (int c = 0; c < kQuarter / 4; ++c) {
+                const int piece = part * (kQuarter / 4) + c;
+                const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(in + piece / 8 * Way::kBox + (((piece & 7) ^ t) << 4));
+#pragma unroll
+                for (int h = 0; h < HB; ++h) {
+                    const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sQ[h][part][c * 4]);
+                    sum[h] = fma2(k.x, v.x, sum[h]);
+                    sum[h] = fma2(k.y, v.y, sum[h]);
+                }
             }
-            if (whole) {
-                static_cast<bf16*>(p.out)[((i64)b * p.Hq + h0 + h) * N + n] = __float2bfloat16_rn(sum == 0.f ? 0.f : x / sum);
-                if (n == 0 && p.lse != nullptr) p.lse[(i64)b * p.Hq + h0 + h] = sum == 0.f ? -INFINITY : top * kLn2 + logf(sum);
-            } else {
-                part[h * (N + 2) + n] = x;
-                if (n == 0) part[h * (N + 2) + N] = top, part[h * (N + 2) + N + 1] = sum;
+            // a half of the heads stays, the other goes to the lane across, twice
+            float x[HB];
+#pragma unroll
+            for (int h = 0; h < HB; ++h) x[h] = sum2(sum[h]);
+#pragma unroll
+            for (int i = 0; i < HB / 2; ++i) {
+                const float keep = part & 2 ? x[HB / 2 + i] : x[i], give = part & 2 ? x[i] : x[HB / 2 + i];
+                x[i] = keep + __shfl_xor_sync(0xffffffffu, give, 16);
+            }
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const float keep = part & 1 ? x[kMine + i] : x[i], give = part & 1 ? x[i] : x[kMine + i];
+                next[i] = keep + __shfl_xor_sync(0xffffffffu, give, 8);
+            }
+        };
+        way.template arrived<false>(0, n0);
+        __syncwarp();
+        scores(0);
+        for (int step = 0; step < way.steps && !way.lost; ++step) {
+            float z[kMine];
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) z[i] = next[i];
+            const int n2 = way.place(step + 2, id2);
+            id2 = way.page(step + 3);
+            __syncwarp();                 // (all lanes have read the slots that are asked for, and the weights)
+            way.template ask<false>(step + 2, n2);
+            way.template ask<true>(step + 1, n1);
+            commit();
+            way.template arrived<false>(step + 1, n1);
+            way.template arrived<true>(step, n0);
+            __syncwarp();
+            scores(step + 1);
+            const int n = n0;
+            n0 = n1;
+            n1 = n2;
+            if (!__any_sync(0xffffffffu, n >= 0)) continue;   // no token counts
+            const bool there = way.there(step, n, t);
+            const float distance = (float)(way.first(step) + t - (r.hi - 1));
+            bool more = false, dead = true;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                float v = z[i];
+                if (p.cap > 0.f) v = cap * hyperbolic_tangent(v);
+                v = fmaf(slope[i], distance, v);
+                v = there ? v : -INFINITY;
+                z[i] = v;
+                more |= v > m[i];
+                dead &= part * kMine + i >= heads || v == -INFINITY;
+            }
+            // a token without weight in any head counts for nothing, whatever its value (or the memory behind the last token) holds
+            uint32_t gone = __ballot_sync(0xffffffffu, dead);
+            gone &= gone >> 16;
+            gone &= gone >> 8;
+            if (__any_sync(0xffffffffu, more)) {
+                float keep[kMine];
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) {
+                    float top = fmaxf(m[i], z[i]);
+#pragma unroll
+                    for (int d = 1; d <= 4; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    keep[i] = m[i] == -INFINITY ? 1.f : ex2(m[i] - top);   // (nothing, or NaN, has been summed before)
+                    m[i] = top;
+                    l[i] *= keep[i];
+                }
+#pragma unroll
+                for (int h = 0; h < HB; ++h) {
+                    const float k = __shfl_sync(0xffffffffu, keep[h % kMine], h / kMine * 8);
+#pragma unroll
+                    for (int e = 0; e < NP / 64; ++e) o[h][e] = mul2(o[h][e], pack2(k, k));
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const float w = ex2(z[i] - (m[i] == -INFINITY ? 0.f : m[i]));
+                l[i] += w;
+                sW[warp][t][part * kMine + i] = w;
+            }
+            __syncwarp();
+            const unsigned char* in = mine + (2 + (step & 1)) * Way::kRows;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (gone >> k & 1) continue;
+                f2 v[NP / 64];
+                if (NP == 128) {
+                    const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(in + lane / 8 * Way::kBox + k * 128 + (((lane & 7) ^ k) << 4));
+                    v[0] = x.x, v[NP / 64 - 1] = x.y;
+                } else {
+                    v[0] = *reinterpret_cast<const f2*>(in + lane / 16 * Way::kBox + k * 128 + (((lane / 2 & 7) ^ k) << 4) + (lane & 1) * 8);
+                }
+#pragma unroll
+                for (int h = 0; h < HB; h += 4) {
+                    const float4 w = *reinterpret_cast<const float4*>(&sW[warp][k][h]);
+#pragma unroll
+                    for (int e = 0; e < NP / 64; ++e) {
+                        o[h][e] = fma2(pack2(w.x, w.x), v[e], o[h][e]);
+                        o[h + 1][e] = fma2(pack2(w.y, w.y), v[e], o[h + 1][e]);
+                        o[h + 2][e] = fma2(pack2(w.z, w.z), v[e], o[h + 2][e]);
+                        o[h + 3][e] = fma2(pack2(w.w, w.w), v[e], o[h + 3][e]);
+                    }
+                }
             }
         }
+        way.finish();
+        float* sO = reinterpret_cast<float*>(mine);
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            if (way.lost) m[i] = 0.f, l[i] = __int_as_float(0x7fffffff);   // results that cannot pass as such
+#pragma unroll
+            for (int d = 1; d <= 4; d <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], d);
+            if (t == 0) sM[warp][part * kMine + i] = m[i], sL[warp][part * kMine + i] = l[i];
+        }
+#pragma unroll
+        for (int h = 0; h < HB; ++h)
+#pragma unroll
+            for (int e = 0; e < NP / 64; ++e) *reinterpret_cast<f2*>(sO + h * NP + lane * (NP / 32) + e * 2) = o[h][e];
+        __syncthreads();
+        write_unit<float, NP, HB>(p, reinterpret_cast<const float*>(staged), Way::kWarpBytes / 4, sM, sL, b, h0, heads, t0 == 0 && t1 == r.tiles, t0 == 0);
         if (TMA) v7u::proxy_fence();
         __syncthreads();
     }
@@ -716,6 +962,7 @@ int launch_join(const AttentionArgs& p, int parts, int HB, cudaStream_t st) {
 }
 int heads_of(int group) { return group >= 4 ? 4 : group >= 2 ? 2 : 1; }
 int mma_heads_of(int group) { return group > 8 ? 16 : 8; }
+int fp32_heads_of(int group) { return group > 4 ? 8 : 4; }
 
 template <typename E, int W, int HB>
 int launch(AttentionArgs& p, cudaStream_t st) {
@@ -725,10 +972,10 @@ int launch(AttentionArgs& p, cudaStream_t st) {
     if (int e = check_launch("paged_attention")) return e;
     return launch_join<E>(p, parts, HB, st);
 }
-// A pool as rows of 64 or 128 elements, in boxes of [16 rows][64 elements], one behind the other for rows of 128.
+// A pool as rows of N elements, in boxes of a step's tokens and 128 bytes, one behind the other.
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-bool make_row_map(CUtensorMap* map, const void* pool, i64 rows, int N) {
+bool make_row_map(CUtensorMap* map, const void* pool, i64 rows, int N, int element) {
     static const EncodeTiled encode = [] {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult found;
@@ -736,59 +983,64 @@ bool make_row_map(CUtensorMap* map, const void* pool, i64 rows, int N) {
         return reinterpret_cast<EncodeTiled>(fn);
     }();
     if (encode == nullptr || tensor_maps_disabled()) return false;
-    const cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)N / 64}, strides[2] = {(cuuint64_t)N * 2, 128};
-    const cuuint32_t box[3] = {64, 16, (cuuint32_t)N / 64}, step[3] = {1, 1, 1};
+    const cuuint32_t size = element == 2 ? 2 : 4, columns = 128 / size, boxes = (cuuint32_t)N / columns;
+    const cuuint64_t dims[3] = {columns, (cuuint64_t)rows, boxes}, strides[2] = {(cuuint64_t)N * size, 128};
+    const cuuint32_t box[3] = {columns, 32 / size, boxes}, step[3] = {1, 1, 1};
     auto make = [&] {
-        return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+        return encode(map, size == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(pool), dims, strides, box, step,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
     };
     return make() || (cudaFree(nullptr) == cudaSuccess && make());   // (a thread without a context yet)
 }
 
-template <int NP, int HT, bool TMA>
-int launch_mma(AttentionArgs& p, const Maps& maps, cudaStream_t st) {
-    constexpr int smem = kWarps * 4 * 2048 * (NP / 64);
-    static_assert(4 * 2048 * (NP / 64) >= 8 * HT * NP * 4, "a warp's sums fit its slots");
-    if (allow_smem<attention_mma_kernel<NP, HT, TMA>>(smem) != cudaSuccess) return check_launch("paged_attention");
-    p.blocks = (p.group + 8 * HT - 1) / (8 * HT);
+template <typename E, int NP, int HEADS, bool TMA>
+int launch_steps(AttentionArgs& p, const Maps& maps, cudaStream_t st) {
+    constexpr auto kernel = [] {
+        if constexpr (sizeof(E) == 2) return attention_mma_kernel<NP, HEADS / 8, TMA>;
+        else return attention_fp32_kernel<NP, HEADS, TMA>;
+    }();
+    using Way = Steps<E, NP, TMA>;
+    constexpr int smem = kWarps * Way::kWarpBytes;
+    static_assert(Way::kWarpBytes >= HEADS * NP * 4, "a warp's sums fit its slots");
+    if (allow_smem<kernel>(smem) != cudaSuccess) return check_launch("paged_attention");
+    p.blocks = (p.group + HEADS - 1) / HEADS;
     p.to_log2 = 1.f;
+    p.tile_bits = sizeof(E) == 2 ? 6 : 5;
     const int parts = run_blocks();
-    attention_mma_kernel<NP, HT, TMA><<<parts, kThreads, smem, st>>>(p, maps);
+    kernel<<<parts, kThreads, smem, st>>>(p, maps);
     if (int e = check_launch("paged_attention")) return e;
-    return launch_join<bf16>(p, parts, 8 * HT, st);
+    return launch_join<E>(p, parts, HEADS, st);
 }
-// Heads of whole 16-byte pieces that start on such boundaries, and rows of the pools that an int can number.
-bool takes_mma(const AttentionArgs& p) {
-    const uintptr_t all = reinterpret_cast<uintptr_t>(p.k_pages) | reinterpret_cast<uintptr_t>(p.v_pages);
-    return p.N % 8 == 0 && all % 16 == 0 && (i64)p.pages * p.Hkv * p.page.d <= 0x7fffffff;
+template <typename E, int FEW, int MANY>
+int dispatch_steps(AttentionArgs& p, bool many, cudaStream_t st) {
+    Maps maps;
+    const i64 rows = (i64)p.pages * p.Hkv * p.page.d;
+    const bool tma = p.page.d % 16 == 0 && (p.N == 64 || p.N == 128) && make_row_map(&maps.keys, p.k_pages, rows, p.N, sizeof(E)) &&
+                     make_row_map(&maps.values, p.v_pages, rows, p.N, sizeof(E));
+    switch ((p.N > 64) * 4 + many * 2 + tma) {
+        case 0: return launch_steps<E, 64, FEW, false>(p, maps, st);
+        case 1: return launch_steps<E, 64, FEW, true>(p, maps, st);
+        case 2: return launch_steps<E, 64, MANY, false>(p, maps, st);
+        case 3: return launch_steps<E, 64, MANY, true>(p, maps, st);
+        case 4: return launch_steps<E, 128, FEW, false>(p, maps, st);
+        case 5: return launch_steps<E, 128, FEW, true>(p, maps, st);
+        case 6: return launch_steps<E, 128, MANY, false>(p, maps, st);
+        default: return launch_steps<E, 128, MANY, true>(p, maps, st);
+    }
 }
 template <typename E>
 int dispatch(AttentionArgs& p, cudaStream_t st) {
-    if (sizeof(E) == 2 && takes_mma(p)) {
-        Maps maps;
-        const i64 rows = (i64)p.pages * p.Hkv * p.page.d;
-        const bool tma = p.page.d % 16 == 0 && (p.N == 64 || p.N == 128) && make_row_map(&maps.keys, p.k_pages, rows, p.N) &&
-                         make_row_map(&maps.values, p.v_pages, rows, p.N);
-        switch ((p.N > 64) * 4 + (p.group > 8) * 2 + tma) {
-            case 0: return launch_mma<64, 1, false>(p, maps, st);
-            case 1: return launch_mma<64, 1, true>(p, maps, st);
-            case 2: return launch_mma<64, 2, false>(p, maps, st);
-            case 3: return launch_mma<64, 2, true>(p, maps, st);
-            case 4: return launch_mma<128, 1, false>(p, maps, st);
-            case 5: return launch_mma<128, 1, true>(p, maps, st);
-            case 6: return launch_mma<128, 2, false>(p, maps, st);
-            default: return launch_mma<128, 2, true>(p, maps, st);
-        }
+    // heads of whole 16-byte pieces that start on such boundaries, and rows of the pools that an int can number
+    const uintptr_t all = reinterpret_cast<uintptr_t>(p.k_pages) | reinterpret_cast<uintptr_t>(p.v_pages);
+    if (p.N * sizeof(E) % 16 == 0 && all % 16 == 0 && (i64)p.pages * p.Hkv * p.page.d <= 0x7fffffff) {
+        if constexpr (sizeof(E) == 2) return dispatch_steps<E, 8, 16>(p, mma_heads_of(p.group) > 8, st);
+        else return dispatch_steps<E, 4, 8>(p, fp32_heads_of(p.group) > 4, st);
     }
     p.to_log2 = kLog2e;
-    const uintptr_t all = reinterpret_cast<uintptr_t>(p.k_pages) | reinterpret_cast<uintptr_t>(p.v_pages);
-    const bool wide = p.N % 4 == 0 && all % (4 * sizeof(E)) == 0;   // a piece of four elements is one load
-    switch (heads_of(p.group) * 2 + wide) {
-        case 9: return launch<E, 4, 4>(p, st);
-        case 8: return launch<E, 1, 4>(p, st);
-        case 5: return launch<E, 4, 2>(p, st);
-        case 4: return launch<E, 1, 2>(p, st);
-        case 3: return launch<E, 4, 1>(p, st);
+    p.tile_bits = 6;
+    switch (heads_of(p.group)) {
+        case 4: return launch<E, 1, 4>(p, st);
+        case 2: return launch<E, 1, 2>(p, st);
         default: return launch<E, 1, 1>(p, st);
     }
 }
@@ -807,7 +1059,7 @@ using namespace rwkvb200;
 
 extern "C" size_t rwkvb200_paged_attention_work_bytes(int dtype, int Hq, int Hkv, int N) {
     if (Hq <= 0 || Hkv <= 0 || N <= 0) return 0;
-    const int heads = dtype == RWKVB200_BF16 ? mma_heads_of(Hq / Hkv) : heads_of(Hq / Hkv);
+    const int heads = dtype == RWKVB200_BF16 ? mma_heads_of(Hq / Hkv) : fp32_heads_of(Hq / Hkv);   // (no fewer than heads_of)
     return (size_t)run_blocks() * 2 * heads * (N + 2) * sizeof(float);
 }
 
@@ -825,6 +1077,6 @@ extern "C" int rwkvb200_paged_attention(int dtype, int B, int Hq, int Hkv, int N
     RWKV_REQUIRE(window >= 0, RWKVB200_EINVAL, "%s: window=%d is negative", what, window);
     RWKV_REQUIRE(cap >= 0.f, RWKVB200_EINVAL, "%s: cap=%g is negative", what, cap);
     RWKV_NOTNULL(q); RWKV_NOTNULL(k_pages); RWKV_NOTNULL(v_pages); RWKV_NOTNULL(table); RWKV_NOTNULL(lengths); RWKV_NOTNULL(out); RWKV_NOTNULL(work);
-    AttentionArgs p{B, Hq, Hkv, N, pages, width, window, Hq / Hkv, 1, scale, cap, 1.f, Divisor((uint32_t)page), q, k_pages, v_pages, table, lengths, slopes, out, lse, static_cast<float*>(work)};
+    AttentionArgs p{B, Hq, Hkv, N, pages, width, window, Hq / Hkv, 1, 0, scale, cap, 1.f, Divisor((uint32_t)page), q, k_pages, v_pages, table, lengths, slopes, out, lse, static_cast<float*>(work)};
     return dtype == RWKVB200_BF16 ? dispatch<bf16>(p, as_stream(stream)) : dispatch<float>(p, as_stream(stream));
 }
