@@ -11,6 +11,7 @@
 #include "packed.cuh"
 #include "paged.cuh"
 #include "wkv7_umma.cuh"
+#include <cooperative_groups.h>
 #include <cuda.h>
 
 namespace rwkvb200 {
@@ -18,7 +19,7 @@ namespace {
 
 __device__ int g_error = 0;
 constexpr int kThreads = 128, kWarps = kThreads / 32;
-constexpr int kMinTokens = 256;   // of a block's run: fewer would cost more to join than they save
+constexpr int kMinTokens = 64;    // of a block's run (1000 tokens of 12 heads, fp32: 18.9 us with 256, 14.6 with 128, 12.9, 13.5 with 32)
 
 struct AttentionArgs {
     int B, Hq, Hkv, N, pages, width, window, group, blocks;   // blocks of query heads per key-value head
@@ -272,6 +273,8 @@ __global__ void __launch_bounds__(kThreads) attention_kernel(const AttentionArgs
 //         steps ahead and values one, and counts the bytes on a barrier of the slot.  A step lies in one page: one lookup;
 //   else: by cp.async in pieces of 16 bytes, rows that do not count filled with zeros.
 // (128 sequences of up to 4096 tokens: 205 us by TMA; 273 us by cp.async, 267 of them without any product.)
+// LONE: a cluster of blocks has a unit of its own and nothing is left for a second kernel (launch_steps has the rule).
+constexpr int kMaxCluster = 8;
 constexpr int kTimeout = 3;       // a wait for a copy ran out
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -451,40 +454,108 @@ __device__ __forceinline__ void write_unit(const AttentionArgs& p, const float* 
     }
 }
 
+// The same where a cluster of K blocks has a unit to itself: the warps' sums are joined in the block's shared memory (in place of the first
+// warp's), then every block joins a K-th of the elements of all blocks and writes the results.
+template <typename E, int NP, int HEADS>
+__device__ __forceinline__ void write_from_cluster(const AttentionArgs& p, float* sO, int stride, const float (*sM)[HEADS], const float (*sL)[HEADS], float* sTop,
+                                                   float* sSum, int b, int h0, int heads) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int K = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    for (int i = threadIdx.x; i < heads * NP; i += kThreads) {
+        const int h = i / NP;
+        float top = -INFINITY, x = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sM[w][h]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float keep = sM[w][h] == -INFINITY ? 0.f : ex2(sM[w][h] - top);
+            sum += sL[w][h] * keep;
+            if (sM[w][h] != -INFINITY) x += sO[w * stride + i] * keep;
+        }
+        sO[i] = x;
+        if (i % NP == 0) sTop[h] = top, sSum[h] = sum;
+    }
+    cluster.sync();
+    const int each = (heads * NP + K - 1) / K, end = min((rank + 1) * each, heads * NP);
+    for (int i = rank * each + threadIdx.x; i < end; i += kThreads) {
+        const int h = i / NP, n = i % NP;
+        if (n >= p.N) continue;
+        float m[kMaxCluster], l[kMaxCluster], x[kMaxCluster], top = -INFINITY, all = 0.f, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) {
+            const bool there = k < K;
+            m[k] = there ? *cluster.map_shared_rank(sTop + h, k) : -INFINITY;
+            l[k] = there ? *cluster.map_shared_rank(sSum + h, k) : 0.f;
+            x[k] = there ? *cluster.map_shared_rank(sO + i, k) : 0.f;
+            top = fmaxf(top, m[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kMaxCluster; ++k) {
+            const float keep = m[k] == -INFINITY ? 0.f : ex2(m[k] - top);
+            sum += l[k] * keep;
+            if (m[k] != -INFINITY) all += x[k] * keep;
+        }
+        static_cast<E*>(p.out)[((i64)b * p.Hq + h0 + h) * p.N + n] = from_f<E>(sum == 0.f ? 0.f : all / sum);
+        if (n == 0 && p.lse != nullptr) p.lse[(i64)b * p.Hq + h0 + h] = sum == 0.f ? -INFINITY : top * kLn2 + logf(sum);
+    }
+    cluster.sync();   // (a block's shared memory is read until all are done)
+}
+
 // bf16, heads of whole 16-byte pieces: products on mma.sync m16n8k16 with the tokens in the rows, S^T = K q^T and O^T = V^T P^T, for up
 // to 8 HT query heads that share the keys: HT = 1 wastes nothing on groups of 8, and memory bounds both anyway.  Each warp
 // keeps its own maxima and sums.  Both first operands come out of shared memory by ldmatrix (the values transposed).
 // Weights are taken into the second product as the sum of two bf16 numbers (2^-16 relative; one would double the output's
 // rounding), both above 0, so that an infinite value stays one.
-template <int NP, int HT, bool TMA>
+template <int NP, int HT, bool TMA, bool LONE>
 __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const AttentionArgs p, const __grid_constant__ Maps maps) {
     using Way = Steps<bf16, NP, TMA>;
     constexpr int kHeads = 8 * HT;
     extern __shared__ __align__(1024) unsigned char staged[];
-    __shared__ float sM[kWarps][kHeads], sL[kWarps][kHeads];
+    __shared__ float sM[kWarps][kHeads], sL[kWarps][kHeads], sTop[kHeads], sSum[kHeads];
     __shared__ uint64_t bars[kWarps][4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const int units = p.Hkv * p.blocks, N = TMA ? NP : p.N;
     unsigned char* mine = staged + warp * Way::kWarpBytes;
     Way way(p, maps, bars[warp], mine, lane);
-    const Start start = find_start<kThreads>(p, blockIdx.x, gridDim.x, units);
-    const i64 end = min(start.tile + start.run, start.all);
-    if (start.tile >= end) return;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    Start start{0, 1, 0, 0, 0};
+    if (!LONE) {
+        start = find_start<kThreads>(p, blockIdx.x, gridDim.x, units);
+        if (start.tile >= start.all) return;
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    }
+    const i64 end = LONE ? 1 : min(start.tile + start.run, start.all);
     // where a lane's rows for ldmatrix lie: keys: rows lane & 15, piece lane / 16; values: rows by 8 from lane / 16, piece by lane / 8
     const uint32_t key_row = (lane & 15) * 128, key_piece = lane >> 4, value_row = ((lane & 7) + (lane >> 4) * 8) * 128, value_piece = lane >> 3 & 1, swizzle = lane & 7;
     const float scale = p.cap > 0.f ? p.scale / p.cap : p.scale * kLog2e, cap = p.cap * kLog2e;
     int b = start.b;
     i64 base = start.base;
     for (i64 at = start.tile; at < end;) {
-        const Range r(p, b);
-        if (at >= base + (i64)r.tiles * units) {   // (a row without tiles is passed over as well)
-            base += (i64)r.tiles * units;
-            ++b;
-            continue;
+        int unit, t0, t1;
+        if (LONE) {
+            const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+            const int K = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+            unit = blockIdx.x / K;
+            b = unit / units;
+            unit -= b * units;
+            const int tiles = Range(p, b).tiles;
+            if (tiles == 0) return;   // (the same for the whole cluster)
+            t0 = tiles * rank / K;
+            t1 = tiles * (rank + 1) / K;
+            at = 1;
+        } else {
+            const int tiles = Range(p, b).tiles;
+            if (at >= base + (i64)tiles * units) {   // (a row without tiles is passed over as well)
+                base += (i64)tiles * units;
+                ++b;
+                continue;
+            }
+            unit = (int)((at - base) / tiles);
+            t0 = (int)((at - base) % tiles);
+            t1 = (int)min((i64)tiles, t0 + (end - at));
+            at += t1 - t0;
         }
-        const int unit = (int)((at - base) / r.tiles), t0 = (int)((at - base) % r.tiles), t1 = (int)min((i64)r.tiles, t0 + (end - at));
-        at += t1 - t0;
+        const Range r(p, b);
         const int head = unit / p.blocks, h0 = head * p.group + unit % p.blocks * kHeads, heads = min(kHeads, (head + 1) * p.group - h0);
         if (threadIdx.x == 0 && p.lengths[b] > r.hi) atomicMax(&g_error, kBadLength);
         way.unit(b, r, t0, t1, head, warp);
@@ -666,6 +737,10 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
                 for (int e = 0; e < 4; ++e) sO[(h * 8 + 2 * q + (e & 1)) * NP + i * 16 + g + (e >> 1) * 8] = o[h][i][e];
         }
         __syncthreads();
+        if (LONE) {
+            write_from_cluster<bf16, NP, kHeads>(p, reinterpret_cast<float*>(staged), Way::kWarpBytes / 4, sM, sL, sTop, sSum, b, h0, heads);
+            return;
+        }
         write_unit<bf16, NP, kHeads>(p, reinterpret_cast<const float*>(staged), Way::kWarpBytes / 4, sM, sL, b, h0, heads, t0 == 0 && t1 == r.tiles, t0 == 0);
         if (TMA) v7u::proxy_fence();
         __syncthreads();
@@ -675,34 +750,54 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
 // fp32, heads of whole 16-byte pieces, for up to HB query heads that share the keys.  Scores: lane (part, t) takes a quarter of key t
 // times all queries (which lie in shared memory, scaled), and the quarters are added so that lane (part, t) ends with the scores of
 // HB / 4 heads.  Sums: a lane has NP / 32 elements of every head, the weights of a token come out of shared memory.
-template <int NP, int HB, bool TMA>
+template <int NP, int HB, bool TMA, bool LONE>
 __global__ void __launch_bounds__(kThreads, 3) attention_fp32_kernel(const AttentionArgs p, const __grid_constant__ Maps maps) {
     using Way = Steps<float, NP, TMA>;
     constexpr int kMine = HB / 4, kQuarter = NP / 4, kPad = kQuarter + 4;   // (padded: the four quarters are read at once)
     extern __shared__ __align__(1024) unsigned char staged[];
-    __shared__ float sM[kWarps][HB], sL[kWarps][HB];
+    __shared__ float sM[kWarps][HB], sL[kWarps][HB], sTop[HB], sSum[HB];
     __shared__ __align__(16) float sQ[HB][4][kPad], sW[kWarps][8][HB];
     __shared__ uint64_t bars[kWarps][4];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 7, part = lane >> 3;
     const int units = p.Hkv * p.blocks;
     unsigned char* mine = staged + warp * Way::kWarpBytes;
     Way way(p, maps, bars[warp], mine, lane);
-    const Start start = find_start<kThreads>(p, blockIdx.x, gridDim.x, units);
-    const i64 end = min(start.tile + start.run, start.all);
-    if (start.tile >= end) return;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    Start start{0, 1, 0, 0, 0};
+    if (!LONE) {
+        start = find_start<kThreads>(p, blockIdx.x, gridDim.x, units);
+        if (start.tile >= start.all) return;
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    }
+    const i64 end = LONE ? 1 : min(start.tile + start.run, start.all);
     const float scale = p.cap > 0.f ? p.scale / p.cap : p.scale * kLog2e, cap = p.cap * kLog2e;
     int b = start.b;
     i64 base = start.base;
     for (i64 at = start.tile; at < end;) {
-        const Range r(p, b);
-        if (at >= base + (i64)r.tiles * units) {   // (a row without tiles is passed over as well)
-            base += (i64)r.tiles * units;
-            ++b;
-            continue;
+        int unit, t0, t1;
+        if (LONE) {
+            const cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+            const int K = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+            unit = blockIdx.x / K;
+            b = unit / units;
+            unit -= b * units;
+            const int tiles = Range(p, b).tiles;
+            if (tiles == 0) return;   // (the same for the whole cluster)
+            t0 = tiles * rank / K;
+            t1 = tiles * (rank + 1) / K;
+            at = 1;
+        } else {
+            const int tiles = Range(p, b).tiles;
+            if (at >= base + (i64)tiles * units) {   // (a row without tiles is passed over as well)
+                base += (i64)tiles * units;
+                ++b;
+                continue;
+            }
+            unit = (int)((at - base) / tiles);
+            t0 = (int)((at - base) % tiles);
+            t1 = (int)min((i64)tiles, t0 + (end - at));
+            at += t1 - t0;
         }
-        const int unit = (int)((at - base) / r.tiles), t0 = (int)((at - base) % r.tiles), t1 = (int)min((i64)r.tiles, t0 + (end - at));
-        at += t1 - t0;
+        const Range r(p, b);
         const int head = unit / p.blocks, h0 = head * p.group + unit % p.blocks * HB, heads = min(HB, (head + 1) * p.group - h0);
         if (threadIdx.x == 0 && p.lengths[b] > r.hi) atomicMax(&g_error, kBadLength);
         way.unit(b, r, t0, t1, head, warp);
@@ -864,6 +959,10 @@ __global__ void __launch_bounds__(kThreads, 3) attention_fp32_kernel(const Atten
 #pragma unroll
             for (int e = 0; e < NP / 64; ++e) *reinterpret_cast<f2*>(sO + h * NP + lane * (NP / 32) + e * 2) = o[h][e];
         __syncthreads();
+        if (LONE) {
+            write_from_cluster<float, NP, HB>(p, reinterpret_cast<float*>(staged), Way::kWarpBytes / 4, sM, sL, sTop, sSum, b, h0, heads);
+            return;
+        }
         write_unit<float, NP, HB>(p, reinterpret_cast<const float*>(staged), Way::kWarpBytes / 4, sM, sL, b, h0, heads, t0 == 0 && t1 == r.tiles, t0 == 0);
         if (TMA) v7u::proxy_fence();
         __syncthreads();
@@ -942,7 +1041,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttentionArgs 
     }
 }
 
-constexpr int kBlocksPerSm = 3;
+constexpr int kBlocksPerSm = 3, kLoneTokens = 512;
 int run_blocks() { return max(1, sm_count()) * kBlocksPerSm; }
 template <typename E>
 int launch_join(const AttentionArgs& p, int parts, int HB, cudaStream_t st) {
@@ -993,19 +1092,45 @@ bool make_row_map(CUtensorMap* map, const void* pool, i64 rows, int N, int eleme
     return make() || (cudaFree(nullptr) == cudaSuccess && make());   // (a thread without a context yet)
 }
 
+template <typename E, int NP, int HEADS, bool TMA, bool LONE>
+constexpr auto steps_kernel() {
+    if constexpr (sizeof(E) == 2) return attention_mma_kernel<NP, HEADS / 8, TMA, LONE>;
+    else return attention_fp32_kernel<NP, HEADS, TMA, LONE>;
+}
 template <typename E, int NP, int HEADS, bool TMA>
 int launch_steps(AttentionArgs& p, const Maps& maps, cudaStream_t st) {
-    constexpr auto kernel = [] {
-        if constexpr (sizeof(E) == 2) return attention_mma_kernel<NP, HEADS / 8, TMA>;
-        else return attention_fp32_kernel<NP, HEADS, TMA>;
-    }();
     using Way = Steps<E, NP, TMA>;
     constexpr int smem = kWarps * Way::kWarpBytes;
     static_assert(Way::kWarpBytes >= HEADS * NP * 4, "a warp's sums fit its slots");
-    if (allow_smem<kernel>(smem) != cudaSuccess) return check_launch("paged_attention");
     p.blocks = (p.group + HEADS - 1) / HEADS;
     p.to_log2 = 1.f;
     p.tile_bits = sizeof(E) == 2 ? 6 : 5;
+    // Units of which no block of a cluster gets more than kLoneTokens go to clusters of their own as long as all clusters are there at
+    // once: one launch instead of two, and no share of the work has to be found out (1000 tokens of 12 heads, bf16: 9.9 and
+    // 11.6 us; 8 sequences of up to 1024 tokens, 32 heads on 8: 12.9 and 16.7).  Beyond that equal shares are better (128 sequences of up
+    // to 4096 tokens: 261 and 198 us).
+    const i64 units = (i64)p.B * p.Hkv * p.blocks, capacity = (i64)p.width * p.page.d, most = p.window > 0 && p.window < capacity ? p.window : capacity;
+    int K = 1;
+    while (K < kMaxCluster && (most > (i64)K * kLoneTokens || (units * K * 2 <= 2 * sm_count() && most > K * 64))) K *= 2;
+    if (TMA && most <= (i64)K * kLoneTokens && units * K <= run_blocks()) {
+        constexpr auto kernel = steps_kernel<E, NP, HEADS, TMA, TMA>();
+        if (allow_smem<kernel>(smem) != cudaSuccess) return check_launch("paged_attention");
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3((unsigned)(units * K));
+        config.blockDim = dim3(kThreads);
+        config.dynamicSmemBytes = smem;
+        config.stream = st;
+        cudaLaunchAttribute cluster;
+        cluster.id = cudaLaunchAttributeClusterDimension;
+        cluster.val.clusterDim.x = K;
+        cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+        config.attrs = &cluster;
+        config.numAttrs = 1;
+        cudaLaunchKernelEx(&config, kernel, p, maps);
+        return check_launch("paged_attention");
+    }
+    constexpr auto kernel = steps_kernel<E, NP, HEADS, TMA, false>();
+    if (allow_smem<kernel>(smem) != cudaSuccess) return check_launch("paged_attention");
     const int parts = run_blocks();
     kernel<<<parts, kThreads, smem, st>>>(p, maps);
     if (int e = check_launch("paged_attention")) return e;
