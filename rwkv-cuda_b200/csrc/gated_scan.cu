@@ -309,14 +309,24 @@ __device__ __forceinline__ f2 through_block(const ulonglong2 (*shares)[32], int 
 // The shares of the blocks go through distributed shared memory: warp q brings this block's to block q.
 template <bool REVERSED>
 __device__ __forceinline__ f2 through_cluster(cg::cluster_group& cluster, int K, int rank, const ulonglong2 (*shares)[32], ulonglong2 (*peers)[32], int warp,
-                                              int lane, f2& carry) {
+                                              int lane, bool cuts, f2& carry) {
     if (warp < K) {
         Share all{both(1.f), both(0.f)};
+        if (cuts) {
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i) {
-            const ulonglong2 v = shares[REVERSED ? kWarps - 1 - i : i][lane];
-            all.H = step(v.x, v.y, all.H);
-            all.P = behind(v.x, all.P);
+            for (int i = 0; i < kWarps; ++i) {
+                const ulonglong2 v = shares[REVERSED ? kWarps - 1 - i : i][lane];
+                all.H = step(v.x, v.y, all.H);
+                all.P = behind(v.x, all.P);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) {
+                const ulonglong2 v = shares[REVERSED ? kWarps - 1 - i : i][lane];
+                all.H = fma2(v.x, all.H, v.y);
+                all.P = mul2(v.x, all.P);
+            }
+            all.P = clamp(all.P);
         }
         *cluster.map_shared_rank(&peers[rank][lane], warp) = make_ulonglong2(all.P, all.H);
     }
@@ -418,7 +428,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
         }
         shares[buf][warp][lane] = make_ulonglong2(share.P, share.H);
         const bool cuts = __syncthreads_or(docs != 0);   // (a buffer is written again two rounds on, behind the next barrier)
-        f2 h = CLUSTER ? through_cluster<false>(cluster, K, rank, shares[buf], peers[buf], warp, lane, carry) : ends[buf ^ 1][lane];
+        f2 h = CLUSTER ? through_cluster<false>(cluster, K, rank, shares[buf], peers[buf], warp, lane, cuts, carry) : ends[buf ^ 1][lane];
         h = through_block<false>(shares[buf], warp, lane, cuts, h);
         if (p.saved != nullptr && t % kSaved == 0 && live && t < p.T) {
             float* to = p.saved + ((i64)b * p.saves + t / kSaved) * p.C + c0;
@@ -550,7 +560,7 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
         shares[buf][warp][lane] = make_ulonglong2(P, Q);
         forward[buf][warp][lane] = H;
         const bool cuts = __syncthreads_or(docs != 0);
-        f2 e = CLUSTER ? through_cluster<true>(cluster, K, rank, shares[buf], peers[buf], warp, lane, carry) : ends[buf ^ 1][lane];
+        f2 e = CLUSTER ? through_cluster<true>(cluster, K, rank, shares[buf], peers[buf], warp, lane, cuts, carry) : ends[buf ^ 1][lane];
         e = through_block<true>(shares[buf], warp, lane, cuts, e);
         if (cuts) {
             for (int i = 0; i < warp; ++i) h = step(shares[buf][i][lane].x, forward[buf][i][lane], h);
