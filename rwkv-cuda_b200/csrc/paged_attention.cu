@@ -13,6 +13,7 @@
 #include "wkv7_umma.cuh"
 #include <cooperative_groups.h>
 #include <cuda.h>
+#include <type_traits>
 
 namespace rwkvb200 {
 namespace {
@@ -24,7 +25,7 @@ constexpr int kMinTokens = 64;    // of a block's run (1000 tokens of 12 heads, 
 struct AttentionArgs {
     int B, Hq, Hkv, N, pages, width, window, group, blocks;   // blocks of query heads per key-value head
     int tile_bits;                                            // a tile has 1 << tile_bits tokens, 16 or 8 for each warp
-    float scale, cap, to_log2;   // to_log2: what makes the partial maxima exponents of 2
+    float scale, cap;
     Divisor page;
     const void *q, *k_pages, *v_pages;
     const int *table, *lengths;
@@ -108,171 +109,15 @@ __device__ __forceinline__ Start find_start(const AttentionArgs& p, int index, i
     return s;
 }
 
-// One sequence's cache as a lane sees it
-template <typename E>
-struct Cache {
-    const AttentionArgs& p;
-    const int* row;
-    int head;
-    // where token j lies (elements from the pool's start), -1: its page is none of the pool's
-    __device__ __forceinline__ i64 at(int j) const {
-        const uint32_t col = p.page.quotient((uint32_t)j);
-        const int id = row[col];
-        if ((unsigned)id >= (unsigned)p.pages) {
-            atomicMax(&g_error, kBadPage);
-            return -1;
-        }
-        return (((i64)id * p.Hkv + head) * p.page.d + ((uint32_t)j - col * p.page.d)) * p.N;
-    }
-};
-
-__device__ __forceinline__ float capped(float z, float cap) { return cap > 0.f ? cap * tanhf(z / cap) : z; }
-
-// Any type, head size and alignment, fp32 arithmetic.  Eight lanes share a token (piece i of W elements of lane l is at
-// (i * 8 + l) * W), so a warp has four tokens in hand; every such group keeps a running maximum and sum of its own for HB
-// query heads, and they are joined at a run's end.
-template <typename E, int W, int HB>
-__global__ void __launch_bounds__(kThreads) attention_kernel(const AttentionArgs p) {
-    constexpr int kPieces = RWKVB200_MAX_HEAD_SIZE / (8 * W);
-    __shared__ float sO[kWarps][HB][RWKVB200_MAX_HEAD_SIZE], sM[kWarps][HB], sL[kWarps][HB];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, l8 = lane & 7, token = warp * 4 + (lane >> 3);
-    const unsigned mask = 0xffu << (lane & 24);   // the lanes that share a token
-    const int units = p.Hkv * p.blocks;
-    const Start start = find_start<kThreads>(p, blockIdx.x, gridDim.x, units);
-    const i64 end = min(start.tile + start.run, start.all);
-    if (start.tile >= end) return;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    int b = start.b;
-    i64 base = start.base;
-    for (i64 at = start.tile; at < end;) {
-        const Range r(p, b);
-        if (at >= base + (i64)r.tiles * units) {   // (a row without tiles is passed over as well)
-            base += (i64)r.tiles * units;
-            ++b;
-            continue;
-        }
-        const int unit = (int)((at - base) / r.tiles), t0 = (int)((at - base) % r.tiles), t1 = (int)min((i64)r.tiles, t0 + (end - at));
-        at += t1 - t0;
-        const int head = unit / p.blocks, h0 = head * p.group + unit % p.blocks * HB, heads = min(HB, (head + 1) * p.group - h0);
-        const Cache<E> cache{p, p.table + (i64)b * p.width, head};
-        if (threadIdx.x == 0 && p.lengths[b] > r.hi) atomicMax(&g_error, kBadLength);
-        float q[HB][kPieces * W], o[HB][kPieces * W], m[HB], l[HB];
-#pragma unroll
-        for (int h = 0; h < HB; ++h) {
-            m[h] = -INFINITY;
-            l[h] = 0.f;
-            const E* from = static_cast<const E*>(p.q) + ((i64)b * p.Hq + h0 + h) * p.N;
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i)
-#pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    const int n = (i * 8 + l8) * W + e;
-                    q[h][i * W + e] = h < heads && n < p.N ? to_f(from[n]) * p.scale : 0.f;
-                    o[h][i * W + e] = 0.f;
-                }
-        }
-        struct alignas(sizeof(E) * W) Piece {
-            E e[W];
-        };
-        const int last = min(r.start + (t1 << p.tile_bits), r.hi);
-        for (int j = r.start + (t0 << p.tile_bits) + token; j < last; j += kWarps * 4) {
-            if (j < r.lo) continue;
-            const i64 place = cache.at(j);
-            const bool found = place >= 0;
-            const E *k = static_cast<const E*>(p.k_pages) + (found ? place : 0), *v = static_cast<const E*>(p.v_pages) + (found ? place : 0);
-            Piece pk[kPieces], pv[kPieces];
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const int n = (i * 8 + l8) * W;
-                if (found && n < p.N) {
-                    pk[i] = *reinterpret_cast<const Piece*>(k + n);
-                    pv[i] = *reinterpret_cast<const Piece*>(v + n);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < W; ++e) pk[i].e[e] = pv[i].e[e] = from_f<E>(0.f);
-                }
-            }
-#pragma unroll
-            for (int h = 0; h < HB; ++h) {
-                float z = 0.f;
-#pragma unroll
-                for (int i = 0; i < kPieces; ++i)
-#pragma unroll
-                    for (int e = 0; e < W; ++e) z = fmaf(q[h][i * W + e], to_f(pk[i].e[e]), z);
-#pragma unroll
-                for (int d = 4; d >= 1; d >>= 1) z += __shfl_xor_sync(mask, z, d);
-                z = capped(z, p.cap);
-                if (p.slopes != nullptr && h < heads) z += p.slopes[h0 + h] * (float)(j - (r.hi - 1));
-                if (!found) z = -INFINITY;
-                // weights of scores of -infinity are 0, also while there is nothing else
-                const float top = fmaxf(m[h], z), keep = m[h] == -INFINITY ? 0.f : expf(m[h] - top);
-                const float w = z == -INFINITY ? 0.f : expf(z - top);
-                m[h] = top;
-                l[h] = fmaf(l[h], keep, w);
-                if (z != -INFINITY) {   // (else the maximum is what it was, and the value may hold anything)
-#pragma unroll
-                    for (int i = 0; i < kPieces; ++i)
-#pragma unroll
-                        for (int e = 0; e < W; ++e) o[h][i * W + e] = fmaf(o[h][i * W + e], keep, w * to_f(pv[i].e[e]));
-                }
-            }
-        }
-        __syncwarp();
-        // the four groups of a warp, then the warps
-        __syncthreads();
-#pragma unroll
-        for (int h = 0; h < HB; ++h) {
-            float top = m[h];
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float keep = m[h] == -INFINITY ? 0.f : expf(m[h] - top);
-            float sum = l[h] * keep;
-            sum += __shfl_xor_sync(0xffffffffu, sum, 8);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-            if (lane == 0) sM[warp][h] = top, sL[warp][h] = sum;
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i)
-#pragma unroll
-                for (int e = 0; e < W; ++e) {
-                    float x = m[h] == -INFINITY ? 0.f : o[h][i * W + e] * keep;
-                    x += __shfl_xor_sync(0xffffffffu, x, 8);
-                    x += __shfl_xor_sync(0xffffffffu, x, 16);
-                    if (lane < 8) sO[warp][h][(i * 8 + l8) * W + e] = x;
-                }
-        }
-        __syncthreads();
-        const bool whole = t0 == 0 && t1 == r.tiles;
-        float* part = p.work + ((i64)blockIdx.x * 2 + (t0 == 0)) * HB * (p.N + 2);
-        for (int i = threadIdx.x; i < heads * p.N; i += kThreads) {
-            const int h = i / p.N, n = i % p.N;
-            float top = -INFINITY, x = 0.f, sum = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sM[w][h]);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float keep = sM[w][h] == -INFINITY ? 0.f : expf(sM[w][h] - top);
-                sum += sL[w][h] * keep;
-                if (sM[w][h] != -INFINITY) x += sO[w][h][n] * keep;
-            }
-            if (whole) {
-                static_cast<E*>(p.out)[((i64)b * p.Hq + h0 + h) * p.N + n] = from_f<E>(sum == 0.f ? 0.f : x / sum);
-                if (n == 0 && p.lse != nullptr) p.lse[(i64)b * p.Hq + h0 + h] = sum == 0.f ? -INFINITY : top + logf(sum);
-            } else {
-                part[h * (p.N + 2) + n] = x;
-                if (n == 0) part[h * (p.N + 2) + p.N] = top, part[h * (p.N + 2) + p.N + 1] = sum;
-            }
-        }
-    }
-}
-
-// ---- kernels that bring a warp's tokens through shared memory ------------------------------------------------------------
 // A step of a warp is 16 (bf16) or 8 (fp32) tokens.  Their keys and values lie in shared memory as boxes of [tokens][128 bytes] in the
-// 128-byte swizzle (piece c of 16 bytes of row t is at c ^ (t & 7)), one behind the other for longer rows; a warp has slots for
-// the keys of two steps and the values of two.  They get there
-//   TMA:  by one bulk copy each (pages of a multiple of 16 tokens, rows of 128, 256 or 512 bytes): a warp's lane 0 asks, keys two
-//         steps ahead and values one, and counts the bytes on a barrier of the slot.  A step lies in one page: one lookup;
-//   else: by cp.async in pieces of 16 bytes, rows that do not count filled with zeros.
-// (128 sequences of up to 4096 tokens: 205 us by TMA; 273 us by cp.async, 267 of them without any product.)
+// 128-byte swizzle (piece c of 16 bytes of row t is at c ^ (t & 7)), one behind the other for longer rows; heads are filled up
+// with zeros to NP = 64 or 128 elements.  A warp has slots for the keys of two steps and the values of two.  They get there
+//   kTma:      by one bulk copy each (pages of a multiple of 16 tokens, heads of 64 or 128): a warp's lane 0 asks, keys two steps
+//              ahead and values one, and counts the bytes on a barrier of the slot.  A step lies in one page: one lookup;
+//   kPieces:   by cp.async in pieces of 16 bytes, rows that do not count filled with zeros (heads of whole pieces);
+//   kElements: element by element, by cp.async (fp32) or through registers (bf16).
+// (128 sequences of up to 4096 tokens, heads of 128: 205 us by TMA; 273 us by pieces, 267 of them without any product.)
+enum { kTma, kPieces, kElements };
 // LONE: a cluster of blocks has a unit of its own and nothing is left for a second kernel (launch_steps has the rule).
 constexpr int kMaxCluster = 8;
 constexpr int kTimeout = 3;       // a wait for a copy ran out
@@ -312,8 +157,10 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&t);
 }
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int BYTES>
 __device__ __forceinline__ void copy_or_zero(uint32_t shared, const void* from, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared), "l"(from), "r"(there ? 16 : 0) : "memory");
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared), "l"(from), "r"(there ? 16 : 0) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(shared), "l"(from), "r"(there ? 4 : 0) : "memory");
 }
 
 __device__ __forceinline__ void ldmatrix(uint32_t (&d)[4], uint32_t at) {
@@ -335,8 +182,10 @@ struct Maps {
 };
 
 // A warp's part of a unit: tokens, pages and slots.
-template <typename E, int NP, bool TMA>
+template <typename E, int NP, int MODE>
 struct Steps {
+    static constexpr bool TMA = MODE == kTma;
+    using Place = std::conditional_t<TMA, int, i64>;   // (the coordinate of a bulk copy is an int)
     static constexpr int kTokens = sizeof(E) == 2 ? 16 : 8, kBoxes = NP * (int)sizeof(E) / 128, kBox = kTokens * 128, kRows = kBox * kBoxes;
     static constexpr int kWarpBytes = 4 * kRows;   // the slots: keys, keys, values, values
     const AttentionArgs& p;
@@ -373,40 +222,60 @@ struct Steps {
         return in_use(step, j) ? row[p.page.quotient((uint32_t)j)] : 0;
     }
     // the row of the pools that the token lies in; -1: it does not count
-    __device__ __forceinline__ int place(int step, int id) const {
+    __device__ __forceinline__ Place place(int step, int id) const {
         const int j = token(step);
         if (!in_use(step, j)) return -1;
         if ((unsigned)id >= (unsigned)p.pages) {
             atomicMax(&g_error, kBadPage);
             return -1;
         }
-        return (id * p.Hkv + head) * (int)p.page.d + (j - (int)(p.page.quotient((uint32_t)j) * p.page.d));
+        return ((Place)id * p.Hkv + head) * (int)p.page.d + (j - (int)(p.page.quotient((uint32_t)j) * p.page.d));
     }
     // whether token t of a step counts, from its place n
-    __device__ __forceinline__ bool there(int step, int n, int t) const {
+    __device__ __forceinline__ bool there(int step, Place n, int t) const {
         return TMA ? n >= 0 && counts(first(step) + t) : __shfl_sync(0xffffffffu, n, t) >= 0;
     }
     __device__ __forceinline__ uint32_t keys(int step) const { return slots + (step & 1) * kRows; }
     __device__ __forceinline__ uint32_t values(int step) const { return slots + (2 + (step & 1)) * kRows; }
     template <bool VALUES>
-    __device__ __forceinline__ void ask(int step, int n) const {
+    __device__ __forceinline__ void ask(int step, Place n) const {
         const uint32_t to = VALUES ? values(step) : keys(step);
         if (TMA) {
             if (lane == 0 && n >= 0) copy_rows(to, VALUES ? &maps.values : &maps.keys, n, &bars[VALUES * 2 + (step & 1)], kRows);
-        } else {
-            constexpr int kPer = 16 / sizeof(E);
-            const E* pool = static_cast<const E*>(VALUES ? p.v_pages : p.k_pages);
+            return;
+        }
+        const E* pool = static_cast<const E*>(VALUES ? p.v_pages : p.k_pages);
+        constexpr int kPer = 16 / sizeof(E);
+        if (MODE == kPieces) {
 #pragma unroll
             for (int i = 0; i < kRows / 512; ++i) {
                 const int piece = i * 32 + lane, t = piece / (8 * kBoxes), c = piece % (8 * kBoxes);
-                const int k = __shfl_sync(0xffffffffu, n, t);
-                copy_or_zero(to + (c >> 3) * kBox + t * 128 + (((c ^ t) & 7) << 4), pool + (i64)max(k, 0) * p.N + min(c * kPer, p.N - kPer), k >= 0 && c * kPer < p.N);
+                const Place k = __shfl_sync(0xffffffffu, n, t);
+                copy_or_zero<16>(to + (c >> 3) * kBox + t * 128 + (((c ^ t) & 7) << 4), pool + max(k, (Place)0) * p.N + min(c * kPer, p.N - kPer), k >= 0 && c * kPer < p.N);
+            }
+        } else {
+#pragma unroll
+            for (int t = 0; t < kTokens; ++t) {
+                const Place k = __shfl_sync(0xffffffffu, n, t);
+#pragma unroll
+                for (int i = 0; i < NP / 32; ++i) {
+                    const int e = i * 32 + lane, c = e / kPer;
+                    const bool there = k >= 0 && e < p.N;
+                    const uint32_t at = to + (c >> 3) * kBox + t * 128 + (((c ^ t) & 7) << 4) + e % kPer * (int)sizeof(E);
+                    const E* from = pool + (there ? k * p.N + e : 0);
+                    if constexpr (sizeof(E) == 4) {
+                        copy_or_zero<4>(at, from, there);
+                    } else {
+                        const unsigned short v = there ? *reinterpret_cast<const unsigned short*>(from) : (unsigned short)0;
+                        asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
+                    }
+                }
             }
         }
     }
     // waits for the copies of all but the last group (TMA: for those that have been asked for)
     template <bool VALUES>
-    __device__ __forceinline__ void arrived(int step, int n) {
+    __device__ __forceinline__ void arrived(int step, Place n) {
         if (!TMA) {
             asm volatile("cp.async.wait_group 1;" ::: "memory");
         } else if (n >= 0) {
@@ -507,9 +376,11 @@ __device__ __forceinline__ void write_from_cluster(const AttentionArgs& p, float
 // keeps its own maxima and sums.  Both first operands come out of shared memory by ldmatrix (the values transposed).
 // Weights are taken into the second product as the sum of two bf16 numbers (2^-16 relative; one would double the output's
 // rounding), both above 0, so that an infinite value stays one.
-template <int NP, int HT, bool TMA, bool LONE>
+template <int NP, int HT, int MODE, bool LONE>
 __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const AttentionArgs p, const __grid_constant__ Maps maps) {
-    using Way = Steps<bf16, NP, TMA>;
+    using Way = Steps<bf16, NP, MODE>;
+    using Place = typename Way::Place;
+    constexpr bool TMA = MODE == kTma;
     constexpr int kHeads = 8 * HT;
     extern __shared__ __align__(1024) unsigned char staged[];
     __shared__ float sM[kWarps][kHeads], sL[kWarps][kHeads], sTop[kHeads], sSum[kHeads];
@@ -561,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
         way.unit(b, r, t0, t1, head, warp);
         const int id0 = way.page(0), id1 = way.page(1);
         int id2 = way.page(2);
-        int n0 = way.place(0, id0), n1 = way.place(1, id1);
+        Place n0 = way.place(0, id0), n1 = way.place(1, id1);
         way.template ask<false>(0, n0);
         commit();
         way.template ask<false>(1, n1);
@@ -575,7 +446,10 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
             for (int j = 0; j < NP / 8; ++j) {
                 const bf16* from = static_cast<const bf16*>(p.q) + ((i64)b * p.Hq + h0 + h * 8 + g) * N + j * 8 + q * 2;
                 __nv_bfloat162 v = __floats2bfloat162_rn(0.f, 0.f);
-                if (h * 8 + g < heads && j * 8 < N) v.x = from[0], v.y = from[1];
+                if (h * 8 + g < heads) {
+                    if (j * 8 + q * 2 < N) v.x = from[0];
+                    if (j * 8 + q * 2 + 1 < N) v.y = from[1];
+                }
                 qf[h][j / 2][j % 2] = *reinterpret_cast<const uint32_t*>(&v);
             }
         float slope[HT][2], m[HT][2], l[HT][2], o[HT][NP / 16][4];   // heads 8 h + 2q, + 1
@@ -617,7 +491,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
             for (int h = 0; h < HT; ++h)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) z[h][e] = next[h][e];
-            const int n2 = way.place(step + 2, id2);
+            const Place n2 = way.place(step + 2, id2);
             id2 = way.page(step + 3);
             __syncwarp();                 // (all lanes have read the slots that are asked for)
             way.template ask<false>(step + 2, n2);
@@ -627,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
             way.template arrived<true>(step, n0);
             __syncwarp();
             scores(step + 1);
-            const int n = n0;
+            const Place n = n0;
             n0 = n1;
             n1 = n2;
             if (!__any_sync(0xffffffffu, n >= 0)) continue;   // no token counts
@@ -750,9 +624,11 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
 // fp32, heads of whole 16-byte pieces, for up to HB query heads that share the keys.  Scores: lane (part, t) takes a quarter of key t
 // times all queries (which lie in shared memory, scaled), and the quarters are added so that lane (part, t) ends with the scores of
 // HB / 4 heads.  Sums: a lane has NP / 32 elements of every head, the weights of a token come out of shared memory.
-template <int NP, int HB, bool TMA, bool LONE>
+template <int NP, int HB, int MODE, bool LONE>
 __global__ void __launch_bounds__(kThreads, 3) attention_fp32_kernel(const AttentionArgs p, const __grid_constant__ Maps maps) {
-    using Way = Steps<float, NP, TMA>;
+    using Way = Steps<float, NP, MODE>;
+    using Place = typename Way::Place;
+    constexpr bool TMA = MODE == kTma;
     constexpr int kMine = HB / 4, kQuarter = NP / 4, kPad = kQuarter + 4;   // (padded: the four quarters are read at once)
     extern __shared__ __align__(1024) unsigned char staged[];
     __shared__ float sM[kWarps][HB], sL[kWarps][HB], sTop[HB], sSum[HB];
@@ -803,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_fp32_kernel(const Atten
         way.unit(b, r, t0, t1, head, warp);
         const int id0 = way.page(0), id1 = way.page(1);
         int id2 = way.page(2);
-        int n0 = way.place(0, id0), n1 = way.place(1, id1);
+        Place n0 = way.place(0, id0), n1 = way.place(1, id1);
         way.template ask<false>(0, n0);
         commit();
         way.template ask<false>(1, n1);
@@ -865,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_fp32_kernel(const Atten
             float z[kMine];
 #pragma unroll
             for (int i = 0; i < kMine; ++i) z[i] = next[i];
-            const int n2 = way.place(step + 2, id2);
+            const Place n2 = way.place(step + 2, id2);
             id2 = way.page(step + 3);
             __syncwarp();                 // (all lanes have read the slots that are asked for, and the weights)
             way.template ask<false>(step + 2, n2);
@@ -875,7 +751,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_fp32_kernel(const Atten
             way.template arrived<true>(step, n0);
             __syncwarp();
             scores(step + 1);
-            const int n = n0;
+            const Place n = n0;
             n0 = n1;
             n1 = n2;
             if (!__any_sync(0xffffffffu, n >= 0)) continue;   // no token counts
@@ -1004,7 +880,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttentionArgs 
 #pragma unroll
         for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
         for (int c = lane; c < count; c += 32) {
-            const float m = weights[h * count + c], w = m == -INFINITY ? 0.f : exp2f((m - top) * p.to_log2);
+            const float m = weights[h * count + c], w = m == -INFINITY ? 0.f : ex2(m - top);
             weights[h * count + c] = w;
             sum = fmaf(share(c, h)[p.N + 1], w, sum);
         }
@@ -1012,7 +888,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttentionArgs 
         for (int d = 16; d >= 1; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (lane == 0) {
             weights[HB * count + h] = sum;
-            if (p.lse != nullptr && h * p.N >= e0) p.lse[(i64)b * p.Hq + h0 + h] = sum == 0.f ? -INFINITY : (top * p.to_log2 + log2f(sum)) * kLn2;
+            if (p.lse != nullptr && h * p.N >= e0) p.lse[(i64)b * p.Hq + h0 + h] = sum == 0.f ? -INFINITY : top * kLn2 + logf(sum);
         }
     }
     __syncthreads();
@@ -1059,18 +935,9 @@ int launch_join(const AttentionArgs& p, int parts, int HB, cudaStream_t st) {
     cudaLaunchKernelEx(&config, join_kernel<E>, p, parts, HB);
     return check_launch("paged_attention");
 }
-int heads_of(int group) { return group >= 4 ? 4 : group >= 2 ? 2 : 1; }
-int mma_heads_of(int group) { return group > 8 ? 16 : 8; }
+int bf16_heads_of(int group) { return group > 8 ? 16 : 8; }
 int fp32_heads_of(int group) { return group > 4 ? 8 : 4; }
 
-template <typename E, int W, int HB>
-int launch(AttentionArgs& p, cudaStream_t st) {
-    p.blocks = (p.group + HB - 1) / HB;
-    const int parts = run_blocks();
-    attention_kernel<E, W, HB><<<parts, kThreads, 0, st>>>(p);
-    if (int e = check_launch("paged_attention")) return e;
-    return launch_join<E>(p, parts, HB, st);
-}
 // A pool as rows of N elements, in boxes of a step's tokens and 128 bytes, one behind the other.
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -1092,18 +959,18 @@ bool make_row_map(CUtensorMap* map, const void* pool, i64 rows, int N, int eleme
     return make() || (cudaFree(nullptr) == cudaSuccess && make());   // (a thread without a context yet)
 }
 
-template <typename E, int NP, int HEADS, bool TMA, bool LONE>
+template <typename E, int NP, int HEADS, int MODE, bool LONE>
 constexpr auto steps_kernel() {
-    if constexpr (sizeof(E) == 2) return attention_mma_kernel<NP, HEADS / 8, TMA, LONE>;
-    else return attention_fp32_kernel<NP, HEADS, TMA, LONE>;
+    if constexpr (sizeof(E) == 2) return attention_mma_kernel<NP, HEADS / 8, MODE, LONE>;
+    else return attention_fp32_kernel<NP, HEADS, MODE, LONE>;
 }
-template <typename E, int NP, int HEADS, bool TMA>
+template <typename E, int NP, int HEADS, int MODE>
 int launch_steps(AttentionArgs& p, const Maps& maps, cudaStream_t st) {
-    using Way = Steps<E, NP, TMA>;
+    using Way = Steps<E, NP, MODE>;
+    constexpr bool TMA = MODE == kTma;
     constexpr int smem = kWarps * Way::kWarpBytes;
     static_assert(Way::kWarpBytes >= HEADS * NP * 4, "a warp's sums fit its slots");
     p.blocks = (p.group + HEADS - 1) / HEADS;
-    p.to_log2 = 1.f;
     p.tile_bits = sizeof(E) == 2 ? 6 : 5;
     // Units of which no block of a cluster gets more than kLoneTokens go to clusters of their own as long as all clusters are there at
     // once: one launch instead of two, and no share of the work has to be found out (1000 tokens of 12 heads, bf16: 9.9 and
@@ -1113,7 +980,7 @@ int launch_steps(AttentionArgs& p, const Maps& maps, cudaStream_t st) {
     int K = 1;
     while (K < kMaxCluster && (most > (i64)K * kLoneTokens || (units * K * 2 <= 2 * sm_count() && most > K * 64))) K *= 2;
     if (TMA && most <= (i64)K * kLoneTokens && units * K <= run_blocks()) {
-        constexpr auto kernel = steps_kernel<E, NP, HEADS, TMA, TMA>();
+        constexpr auto kernel = steps_kernel<E, NP, HEADS, MODE, TMA>();
         if (allow_smem<kernel>(smem) != cudaSuccess) return check_launch("paged_attention");
         cudaLaunchConfig_t config{};
         config.gridDim = dim3((unsigned)(units * K));
@@ -1129,45 +996,28 @@ int launch_steps(AttentionArgs& p, const Maps& maps, cudaStream_t st) {
         cudaLaunchKernelEx(&config, kernel, p, maps);
         return check_launch("paged_attention");
     }
-    constexpr auto kernel = steps_kernel<E, NP, HEADS, TMA, false>();
+    constexpr auto kernel = steps_kernel<E, NP, HEADS, MODE, false>();
     if (allow_smem<kernel>(smem) != cudaSuccess) return check_launch("paged_attention");
     const int parts = run_blocks();
     kernel<<<parts, kThreads, smem, st>>>(p, maps);
     if (int e = check_launch("paged_attention")) return e;
     return launch_join<E>(p, parts, HEADS, st);
 }
-template <typename E, int FEW, int MANY>
-int dispatch_steps(AttentionArgs& p, bool many, cudaStream_t st) {
+template <typename E, int NP, int HEADS>
+int dispatch_mode(AttentionArgs& p, cudaStream_t st) {
     Maps maps;
     const i64 rows = (i64)p.pages * p.Hkv * p.page.d;
-    const bool tma = p.page.d % 16 == 0 && (p.N == 64 || p.N == 128) && make_row_map(&maps.keys, p.k_pages, rows, p.N, sizeof(E)) &&
-                     make_row_map(&maps.values, p.v_pages, rows, p.N, sizeof(E));
-    switch ((p.N > 64) * 4 + many * 2 + tma) {
-        case 0: return launch_steps<E, 64, FEW, false>(p, maps, st);
-        case 1: return launch_steps<E, 64, FEW, true>(p, maps, st);
-        case 2: return launch_steps<E, 64, MANY, false>(p, maps, st);
-        case 3: return launch_steps<E, 64, MANY, true>(p, maps, st);
-        case 4: return launch_steps<E, 128, FEW, false>(p, maps, st);
-        case 5: return launch_steps<E, 128, FEW, true>(p, maps, st);
-        case 6: return launch_steps<E, 128, MANY, false>(p, maps, st);
-        default: return launch_steps<E, 128, MANY, true>(p, maps, st);
-    }
-}
-template <typename E>
-int dispatch(AttentionArgs& p, cudaStream_t st) {
-    // heads of whole 16-byte pieces that start on such boundaries, and rows of the pools that an int can number
     const uintptr_t all = reinterpret_cast<uintptr_t>(p.k_pages) | reinterpret_cast<uintptr_t>(p.v_pages);
-    if (p.N * sizeof(E) % 16 == 0 && all % 16 == 0 && (i64)p.pages * p.Hkv * p.page.d <= 0x7fffffff) {
-        if constexpr (sizeof(E) == 2) return dispatch_steps<E, 8, 16>(p, mma_heads_of(p.group) > 8, st);
-        else return dispatch_steps<E, 4, 8>(p, fp32_heads_of(p.group) > 4, st);
-    }
-    p.to_log2 = kLog2e;
-    p.tile_bits = 6;
-    switch (heads_of(p.group)) {
-        case 4: return launch<E, 1, 4>(p, st);
-        case 2: return launch<E, 1, 2>(p, st);
-        default: return launch<E, 1, 1>(p, st);
-    }
+    if (p.N * sizeof(E) % 16 != 0 || all % 16 != 0) return launch_steps<E, NP, HEADS, kElements>(p, maps, st);
+    if (p.page.d % 16 == 0 && p.N == NP && rows <= 0x7fffffff && make_row_map(&maps.keys, p.k_pages, rows, p.N, sizeof(E)) &&
+        make_row_map(&maps.values, p.v_pages, rows, p.N, sizeof(E)))
+        return launch_steps<E, NP, HEADS, kTma>(p, maps, st);
+    return launch_steps<E, NP, HEADS, kPieces>(p, maps, st);
+}
+template <typename E, int FEW, int MANY>
+int dispatch(AttentionArgs& p, bool many, cudaStream_t st) {
+    if (p.N <= 64) return many ? dispatch_mode<E, 64, MANY>(p, st) : dispatch_mode<E, 64, FEW>(p, st);
+    return many ? dispatch_mode<E, 128, MANY>(p, st) : dispatch_mode<E, 128, FEW>(p, st);
 }
 
 }  // namespace
@@ -1184,7 +1034,7 @@ using namespace rwkvb200;
 
 extern "C" size_t rwkvb200_paged_attention_work_bytes(int dtype, int Hq, int Hkv, int N) {
     if (Hq <= 0 || Hkv <= 0 || N <= 0) return 0;
-    const int heads = dtype == RWKVB200_BF16 ? mma_heads_of(Hq / Hkv) : fp32_heads_of(Hq / Hkv);   // (no fewer than heads_of)
+    const int heads = dtype == RWKVB200_BF16 ? bf16_heads_of(Hq / Hkv) : fp32_heads_of(Hq / Hkv);
     return (size_t)run_blocks() * 2 * heads * (N + 2) * sizeof(float);
 }
 
@@ -1202,6 +1052,6 @@ extern "C" int rwkvb200_paged_attention(int dtype, int B, int Hq, int Hkv, int N
     RWKV_REQUIRE(window >= 0, RWKVB200_EINVAL, "%s: window=%d is negative", what, window);
     RWKV_REQUIRE(cap >= 0.f, RWKVB200_EINVAL, "%s: cap=%g is negative", what, cap);
     RWKV_NOTNULL(q); RWKV_NOTNULL(k_pages); RWKV_NOTNULL(v_pages); RWKV_NOTNULL(table); RWKV_NOTNULL(lengths); RWKV_NOTNULL(out); RWKV_NOTNULL(work);
-    AttentionArgs p{B, Hq, Hkv, N, pages, width, window, Hq / Hkv, 1, 0, scale, cap, 1.f, Divisor((uint32_t)page), q, k_pages, v_pages, table, lengths, slopes, out, lse, static_cast<float*>(work)};
-    return dtype == RWKVB200_BF16 ? dispatch<bf16>(p, as_stream(stream)) : dispatch<float>(p, as_stream(stream));
+    AttentionArgs p{B, Hq, Hkv, N, pages, width, window, Hq / Hkv, 1, 0, scale, cap, Divisor((uint32_t)page), q, k_pages, v_pages, table, lengths, slopes, out, lse, static_cast<float*>(work)};
+    return dtype == RWKVB200_BF16 ? dispatch<bf16, 8, 16>(p, bf16_heads_of(p.group) > 8, as_stream(stream)) : dispatch<float, 4, 8>(p, fp32_heads_of(p.group) > 4, as_stream(stream));
 }
