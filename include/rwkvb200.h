@@ -391,8 +391,9 @@ int rwkvb200_paged_append(int dtype, int M, int B, int Hq, int Hkv, int N, int R
  *   z_j = scale q.k_j    z_j = cap tanh(z_j / cap) if cap > 0    z_j += slopes[h] (j - (len - 1)) if slopes (Hq) is given
  *   out = softmax(z) v    lse (B,Hq; may be NULL) = log sum exp(z)
  * No token, or scores of -infinity only: out = 0, lse = -infinity.  A negative length is a row that only pads the batch: its out
- * and lse stay as they were.  Nothing is read beyond a sequence's tokens.  `work`: rwkvb200_paged_attention_work_bytes bytes,
- * free after the call; two calls that may run at the same time need one each. */
+ * and lse stay as they were.  What a page holds behind a sequence's last token has no effect, whatever it is.  `work`:
+ * rwkvb200_paged_attention_work_bytes bytes, free after the call; two calls that may run at the same time need one each.  The
+ * waits for the copies of the kernels are bounded: where one runs out the rows concerned become NaN, rwkvb200_device_status 143. */
 size_t rwkvb200_paged_attention_work_bytes(int dtype, int Hq, int Hkv, int N);
 int rwkvb200_paged_attention(int dtype, int B, int Hq, int Hkv, int N, int pages, int page, int width, const void* q,
                              const void* k_pages, const void* v_pages, const int* table, const int* lengths, float scale,
@@ -403,7 +404,7 @@ int rwkvb200_paged_attention(int dtype, int B, int Hq, int Hkv, int N, int pages
  * front / back warp group of the two-stage backward, 50.. / 55.. / 60..: loader / matrix / chain group of the
  * staged forward; 70.. / 75.. / 80..: the same groups of the staged RWKV-6 / RWKV-5 forward; 91..: their tcgen05 backward;
  * 101..: the RWKV-7 kernels with the chunks in parallel) (the outputs of
- * that call are then invalid), or 121, 131, 132, 141, 142 as the gated recurrence and the paged cache say; negative on a CUDA error.  Per device; stays set until cleared. */
+ * that call are then invalid), or 121, 131, 132, 141..143 as the gated recurrence and the paged cache say; negative on a CUDA error.  Per device; stays set until cleared. */
 int rwkvb200_device_status(void);
 /* Resets the current device's status word.  No counterpart in the reference. */
 int rwkvb200_device_status_clear(void);

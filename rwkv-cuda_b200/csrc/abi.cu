@@ -138,7 +138,7 @@ extern "C" int rwkvb200_device_status(void) {
     if (v7s) return v7s + 100;  // the RWKV-7 kernels with the chunks in parallel 101..
     if (gs) return gs + 120;    // indices that point nowhere: a slot of gated_scan_update 121
     if (append) return append + 130;        // paged_append 131, 132
-    return attend ? attend + 140 : 0;       // paged_attention 141, 142
+    return attend ? attend + 140 : 0;       // paged_attention 141, 142; 143: a wait ran out
 }
 
 extern "C" int rwkvb200_device_status_clear(void) {

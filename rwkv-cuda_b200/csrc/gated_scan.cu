@@ -101,7 +101,8 @@ template <typename F> __device__ __forceinline__ f2 each(f2 a, f2 b, F f) { retu
 
 // 1 - exp(-L) of two channels, with all its digits where L is small: for L <= 1 as L times a polynomial (interpolation of
 // (1 - exp(-L)) / L at the Chebyshev points of [0, 1]: off by 3e-9, and by one unit of fp32 as it is evaluated), which takes no
-// special function; beyond by the exponential.  SMALL: s <= 1 in all channels of the warp.
+// special function; beyond it -exp(-L), which has the digits of a instead (decay and fallen tell the two apart by the sign).
+// SMALL: s <= 1 in all channels of the warp.
 template <typename E, bool SMALL>
 __device__ __forceinline__ f2 fall(f2 L) {
     f2 q = fma2(L, both(0.0001290763f), both(-0.001300775f));
@@ -112,11 +113,19 @@ __device__ __forceinline__ f2 fall(f2 L) {
     q = fma2(q, L, both(1.f));
     q = mul2(q, L);
     if (SMALL) return q;
-    return each(L, q, [](float l, float p) { return l <= 1.f ? p : 1.f - Fn<E>::exp_minus(l); });
+    return each(L, q, [](float l, float p) { return l <= 1.f ? p : -Fn<E>::exp_minus(l); });
 }
-// 1 - a^2 = (1 - a) (2 - (1 - a))
-__device__ __forceinline__ f2 square(f2 q) { return mul2(q, fma2(q, both(-1.f), both(2.f))); }
-__device__ __forceinline__ f2 decay(f2 q) { return fma2(q, both(-1.f), both(1.f)); }
+// a and 1 - a^2 = (1 - a) (2 - (1 - a)) of what fall has made
+template <bool SMALL>
+__device__ __forceinline__ f2 decay(f2 q) {
+    if (SMALL) return fma2(q, both(-1.f), both(1.f));
+    return each(q, [](float v) { return __float_as_int(v) < 0 ? -v : 1.f - v; });
+}
+template <bool SMALL>
+__device__ __forceinline__ f2 square(f2 q) {
+    if (!SMALL) q = each(q, [](float v) { return __float_as_int(v) < 0 ? 1.f + v : v; });
+    return mul2(q, fma2(q, both(-1.f), both(2.f)));
+}
 // 1 / sqrt(1 - a^2); 0 below the normal numbers, where beta counts as 0 (and NaN below 0, which only a negative s makes)
 template <typename E>
 __device__ __forceinline__ f2 inverse_root(f2 v) {
@@ -346,7 +355,7 @@ constexpr int kBwdStages = 2;
 template <typename E> constexpr int fwd_smem() { return kFwdStages * kWarps * 3 * kFwdTokens<E> * kTile * (int)sizeof(E); }
 template <typename E> constexpr int bwd_smem() { return kBwdStages * kWarps * 4 * kBwdTokens * kTile * (int)sizeof(E); }
 
-// A warp's tile: all tokens and channels are there and no document begins; or not; or some gate is out of range (found on the way)
+// A warp's tile: all tokens and channels are there, no document begins and s <= 1; or not; or some gate is out of range (found on the way)
 enum { kSimpleTile, kDocumentTile, kExtremeTile };
 template <int M> using Mode = std::integral_constant<int, M>;
 
@@ -395,7 +404,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
         f2 a[kTokens], w[kTokens];
         Share share;
         Pair<E> least(0.f);
-        auto make = [&](auto mode, auto is_small) {
+        auto make = [&](auto mode) {
             constexpr bool kSimple = decltype(mode)::value == kSimpleTile, kExtreme = decltype(mode)::value == kExtremeTile;
             share.P = both(1.f);
             share.H = both(0.f);
@@ -404,8 +413,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
                 const Pair<E> vgx(in + kPart + j * kTile), vga(in + 2 * kPart + j * kTile);
                 const Gates<E, kExtreme> g(vga.get(), vgx.get());
                 if (!kExtreme && (kSimple || t + j < p.T)) least.least(vga), least.least(vgx);   // (other rows hold anything)
-                const f2 q = fall<E, decltype(is_small)::value>(mul2(s, g.a)), v = square(q), u = mul2(g.x, get2(in + j * kTile));
-                a[j] = decay(q);
+                const f2 q = fall<E, kSimple>(mul2(s, g.a)), v = square<kSimple>(q), u = mul2(g.x, get2(in + j * kTile));
+                a[j] = decay<kSimple>(q);
                 // (v of 0 or below the normal numbers: beta is 0)
                 w[j] = kSimple ? mul2(mul2(v, each(v, [](float z) { return Fn<E>::inverse_root(fmaxf(z, 1.2e-38f)); })), u)
                                : mul2(mul2(v, inverse_root<E>(v)), u);
@@ -418,13 +427,11 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
             }
             share.P = !kSimple && docs ? both(0.f) : clamp(share.P);
         };
-        int mode = docs == 0 && t + kTokens <= p.T && c_tile + kTile <= p.C ? kSimpleTile : kDocumentTile;
-        if (mode == kDocumentTile) make(Mode<kDocumentTile>{}, std::false_type{});
-        else if (small) make(Mode<kSimpleTile>{}, std::true_type{});
-        else make(Mode<kSimpleTile>{}, std::false_type{});
+        int mode = small && docs == 0 && t + kTokens <= p.T && c_tile + kTile <= p.C ? kSimpleTile : kDocumentTile;
+        if (mode == kSimpleTile) make(Mode<kSimpleTile>{}); else make(Mode<kDocumentTile>{});
         if (__any_sync(0xffffffffu, live && least.below(kLeast))) {
             mode = kExtremeTile;
-            make(Mode<kExtremeTile>{}, std::false_type{});
+            make(Mode<kExtremeTile>{});
         }
         shares[buf][warp][lane] = make_ulonglong2(share.P, share.H);
         const bool cuts = __syncthreads_or(docs != 0);   // (a buffer is written again two rounds on, behind the next barrier)
@@ -518,7 +525,7 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
         // per token: 1 - a, 1 / beta, and w = beta u, which makes room for h before the token
         f2 q[kTokens], inv[kTokens], w[kTokens], P, H, Q;
         Pair<E> least(0.f);
-        auto make = [&](auto mode, auto is_small) {
+        auto make = [&](auto mode) {
             constexpr bool kSimple = decltype(mode)::value == kSimpleTile, kExtreme = decltype(mode)::value == kExtremeTile;
             P = both(1.f);
             H = Q = both(0.f);
@@ -527,35 +534,33 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
                 const Pair<E> vgx(in + kPart + j * kTile), vga(in + 2 * kPart + j * kTile);
                 const Gates<E, kExtreme> g(vga.get(), vgx.get());
                 if (!kExtreme && (kSimple || t + j < p.T)) least.least(vga), least.least(vgx);   // (other rows hold anything)
-                q[j] = fall<E, decltype(is_small)::value>(mul2(s, g.a));
-                const f2 v = square(q[j]), u = mul2(g.x, get2(in + j * kTile));
+                q[j] = fall<E, kSimple>(mul2(s, g.a));
+                const f2 v = square<kSimple>(q[j]), u = mul2(g.x, get2(in + j * kTile));
                 inv[j] = inverse_root<E>(v);
                 w[j] = mul2(mul2(v, inv[j]), u);
                 if (!kSimple) {
                     if (docs >> j & 1) q[j] = both(1.f), inv[j] = both(0.f), w[j] = u;
                     if (t + j >= p.T) q[j] = both(0.f), w[j] = both(0.f);
                 }
-                const f2 a = decay(q[j]);
+                const f2 a = decay<kSimple>(q[j]);
                 H = !kSimple && docs >> j & 1 ? w[j] : fma2(a, H, w[j]);
                 P = mul2(P, a);
             }
 #pragma unroll
             for (int j = kTokens - 1; j >= 0; --j) {
                 if (kSimple) {
-                    Q = mul2(decay(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
+                    Q = mul2(decay<kSimple>(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
                 } else if (t + j < p.T) {
-                    Q = docs >> j & 1 ? both(0.f) : mul2(decay(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
+                    Q = docs >> j & 1 ? both(0.f) : mul2(decay<kSimple>(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
                 }
             }
             P = !kSimple && docs ? both(0.f) : clamp(P);
         };
-        int mode = docs == 0 && t + kTokens <= p.T && c_tile + kTile <= p.C ? kSimpleTile : kDocumentTile;
-        if (mode == kDocumentTile) make(Mode<kDocumentTile>{}, std::false_type{});
-        else if (small) make(Mode<kSimpleTile>{}, std::true_type{});
-        else make(Mode<kSimpleTile>{}, std::false_type{});
+        int mode = small && docs == 0 && t + kTokens <= p.T && c_tile + kTile <= p.C ? kSimpleTile : kDocumentTile;
+        if (mode == kSimpleTile) make(Mode<kSimpleTile>{}); else make(Mode<kDocumentTile>{});
         if (__any_sync(0xffffffffu, live && least.below(kLeast))) {
             mode = kExtremeTile;
-            make(Mode<kExtremeTile>{}, std::false_type{});
+            make(Mode<kExtremeTile>{});
         }
         shares[buf][warp][lane] = make_ulonglong2(P, Q);
         forward[buf][warp][lane] = H;
@@ -576,7 +581,7 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
 #pragma unroll
             for (int j = 0; j < kTokens; ++j) {
                 const f2 before = h;
-                h = !kSimple && docs >> j & 1 ? w[j] : fma2(decay(q[j]), h, w[j]);
+                h = !kSimple && docs >> j & 1 ? w[j] : fma2(decay<kSimple>(q[j]), h, w[j]);
                 w[j] = before;
             }
             const i64 at = (i64)t * p.C;
@@ -586,8 +591,8 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
                 if (!kSimple && t + j >= p.T) continue;
                 const bool doc = !kSimple && docs >> j & 1;
                 const Gates<E, kExtreme> g(get2(in + 2 * kPart + j * kTile), get2(in + kPart + j * kTile));
-                const f2 vx = get2(in + j * kTile), a = decay(q[j]), G = add2(get2(in + 3 * kPart + j * kTile), e);
-                const f2 beta = doc ? both(1.f) : mul2(square(q[j]), inv[j]);
+                const f2 vx = get2(in + j * kTile), a = decay<kSimple>(q[j]), G = add2(get2(in + 3 * kPart + j * kTile), e);
+                const f2 beta = doc ? both(1.f) : mul2(square<kSimple>(q[j]), inv[j]);
                 const f2 ox = mul2(mul2(G, beta), g.x), og = mul2(mul2(ox, vx), g.rest_x());
                 e = mul2(a, G);
                 const f2 slope = fma2(w[j], both(-1.f), mul2(mul2(mul2(g.x, vx), a), inv[j]));
@@ -683,8 +688,8 @@ __global__ void __launch_bounds__(kUpdateThreads) scan_update_kernel(int B, int 
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const Gates<E, true> g(both(to_f(rga.e[i])), both(to_f(rgx.e[i])));
-            const f2 fallen = fall<E, false>(mul2(both(sc.e[i]), g.a)), v = square(fallen);
-            h.e[i] = fmaf(lo(decay(fallen)), h.e[i], lo(mul2(v, inverse_root<E>(v))) * (lo(g.x) * to_f(rx.e[i])));
+            const f2 fallen = fall<E, false>(mul2(both(sc.e[i]), g.a)), v = square<false>(fallen);
+            h.e[i] = fmaf(lo(decay<false>(fallen)), h.e[i], lo(mul2(v, inverse_root<E>(v))) * (lo(g.x) * to_f(rx.e[i])));
             out.e[i] = from_f<E>(h.e[i]);
         }
         *reinterpret_cast<Row*>(y + (i64)q * C + c) = out;

@@ -21,6 +21,7 @@ struct Divisor {
 // what the kernels write into the status word of their device
 constexpr int kBadPage = 1;      // a page number outside of the pool
 constexpr int kBadLength = 2;    // a length beyond what a row of the table holds
+constexpr int kTimeout = 3;      // a wait for a copy ran out
 
 int paged_append_error(int clear);      // the last code of the current device, or -1; clear: sets it to 0
 int paged_attention_error(int clear);

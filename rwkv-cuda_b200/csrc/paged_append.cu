@@ -94,7 +94,8 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs p) {
         if (working && group < p.Hkv) load(p.k, p.Hkv, group, k);
         if (v_working && v_group < p.Hkv) load_v(v_group, v);
     }
-    int b = m, nth = 0;
+    int b = m;
+    i64 nth = 0;
     if (p.cu != nullptr) {
         int lo = 0, hi = p.B;   // the last b with cu[b] <= m
         while (hi - lo > 1) {
@@ -102,12 +103,12 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs p) {
             if (p.cu[mid] <= m) lo = mid; else hi = mid;
         }
         b = lo;
-        nth = m - p.cu[b];
+        nth = (i64)m - p.cu[b];
         if (nth < 0 || m >= p.cu[p.B]) return;   // a row that belongs to no sequence
     }
     const int before = p.lengths[b];
     if (before < 0) return;                      // a row that only pads the batch
-    const i64 position = (i64)before + nth;
+    const i64 position = before + nth;
     const bool in_table = position < (i64)p.width * p.page.d;
     const uint32_t col = in_table ? p.page.quotient((uint32_t)position) : 0;
     const int id = in_table ? p.table[(i64)b * p.width + col] : -1;

@@ -120,7 +120,6 @@ __device__ __forceinline__ Start find_start(const AttentionArgs& p, int index, i
 enum { kTma, kPieces, kElements };
 // LONE: a cluster of blocks has a unit of its own and nothing is left for a second kernel (launch_steps has the rule).
 constexpr int kMaxCluster = 8;
-constexpr int kTimeout = 3;       // a wait for a copy ran out
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -972,14 +971,14 @@ int launch_steps(AttentionArgs& p, const Maps& maps, cudaStream_t st) {
     static_assert(Way::kWarpBytes >= HEADS * NP * 4, "a warp's sums fit its slots");
     p.blocks = (p.group + HEADS - 1) / HEADS;
     p.tile_bits = sizeof(E) == 2 ? 6 : 5;
-    // Units of which no block of a cluster gets more than kLoneTokens go to clusters of their own as long as all clusters are there at
-    // once: one launch instead of two, and no share of the work has to be found out (1000 tokens of 12 heads, bf16: 9.9 and
-    // 11.6 us; 8 sequences of up to 1024 tokens, 32 heads on 8: 12.9 and 16.7).  Beyond that equal shares are better (128 sequences of up
-    // to 4096 tokens: 261 and 198 us).
+    // Units of which no block of a cluster gets more than kLoneTokens go to clusters of their own, of up to four blocks or, as long as
+    // all clusters are there at once, eight: one launch instead of two, and no share of the work has to be found out (32 heads on 8 of
+    // 128: 8 sequences of up to 1024 tokens 12.8 us instead of 16.7, 64 of up to 2048 70.7 and 77.1; 128 of up to 2048 127 and 120).
+    // Longer ones are better shared equally (128 sequences of up to 4096 tokens: 261 and 198 us).
     const i64 units = (i64)p.B * p.Hkv * p.blocks, capacity = (i64)p.width * p.page.d, most = p.window > 0 && p.window < capacity ? p.window : capacity;
     int K = 1;
     while (K < kMaxCluster && (most > (i64)K * kLoneTokens || (units * K * 2 <= 2 * sm_count() && most > K * 64))) K *= 2;
-    if (TMA && most <= (i64)K * kLoneTokens && units * K <= run_blocks()) {
+    if (TMA && most <= (i64)K * kLoneTokens && (K <= 4 || units * K <= run_blocks()) && units * K <= 0x7fffffff) {
         constexpr auto kernel = steps_kernel<E, NP, HEADS, MODE, TMA>();
         if (allow_smem<kernel>(smem) != cudaSuccess) return check_launch("paged_attention");
         cudaLaunchConfig_t config{};

@@ -64,6 +64,42 @@ def test_lengths_and_channels(dtype, B, T, C):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,T,C,docs", [(8, 300, 2048, False), (5, 129, 2046, True), (4, 200, 1024, True), (3, 333, 1500, False), (1, 2500, 192, True),
+                                        (150, 1, 64, False), (160, 70, 8, True)])
+def test_blocks_and_clusters(dtype, B, T, C, docs):
+    """Launches of a block per channel tile (from 149 of them on) and of clusters of 2, 4 and 8 blocks, over several rounds."""
+    check(inputs(B, T, C, dtype, seed=T, docs=docs))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("C", [64, 2048])
+def test_large_decays(dtype, C):
+    """s up to 30: beyond L = 1 the decays come from the exponential, down to exp(-30)."""
+    d = inputs(1, 100, C, dtype, seed=1, docs=True)
+    d["s"] = torch.linspace(0, 30, C, device="cuda")
+    d["s"][:2] = 1.0 + torch.tensor([0.0, 1e-6])
+    T = 100
+    ins = [d[n] for n in ("x", "gx", "ga", "s", "h0", "first")]
+    y64, _ = M.gated_scan(*ins)
+    ybar, _ = M.gated_scan(*ins, bar=True)
+    want, bars = M.gated_scan_gradients(*ins, d["dy"], d["dhT"])
+    more = 1 + d["s"].max().item()   # a unit of the exponent counts as often as the exponent is large
+    for got, w, bar, name in zip((forward(d)[0], *train(d)[1]), (y64, *want), (ybar, *bars), ("y", "dx", "dgx", "dga", "ds", "dh0")):
+        within(got, w, M.scan_bound(T, bar * more, w, got.dtype), name)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("C", [64, 130])
+def test_without_decay(dtype, C):
+    """s = 0: the state stays, the gradient through beta is taken as 0, and ds is that of the decay alone."""
+    d = inputs(1, 70, C, dtype, seed=1)
+    d["s"] = torch.zeros(C, device="cuda")
+    y, hT = forward(d)
+    assert torch.equal(hT, d["h0"]) and torch.equal(y, d["h0"].to(dtype)[:, None].expand_as(y))
+    check(d)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("scale", [8.0, 15.0])
 def test_gates_that_saturate(dtype, scale):
     """Gates from sigmoid(-60) to sigmoid(60): decays of 1 - 1e-27 to exp(-s)."""
@@ -269,6 +305,33 @@ def test_update_slots():
     assert y2[40].isnan().all() and y2[41].isnan().all() and torch.equal(again, mine)
     y2[40:42] = 7.0
     assert torch.equal(y, y2)
+
+
+def test_update_many_channels():
+    """Four channels a thread: shared slots, padding rows and a bad slot there too."""
+    import rwkv_cuda_b200 as R
+    from rwkv_cuda_b200 import _lib
+    L = _lib.lib()
+    for dtype in (BF, F32):
+        B, C, pool = 200, 516, 150
+        d = inputs(B, 1, C, dtype, seed=4)
+        x, gx, ga = (d[n][:, 0].contiguous() for n in ("x", "gx", "ga"))
+        state = Hh.randn(Hh.gen(2), pool, C).cuda()
+        slots = [(b * 7) % pool for b in range(B)]   # 50 slots twice
+        slots[3], slots[199], slots[100] = -1, -7, pool
+        L.rwkvb200_device_status_clear()
+        mine, y = state.clone(), torch.full((B, C), 7.0, dtype=dtype, device="cuda")
+        R.ops.gated_scan_update(mine, x, gx, ga, d["s"], y, slots=torch.tensor(slots, dtype=torch.int32, device="cuda"))
+        assert L.rwkvb200_device_status() == 121
+        L.rwkvb200_device_status_clear()
+        want, rows = step(state, x, gx, ga, d["s"], slots)
+        size = torch.tensor(16.0, device="cuda")
+        within(mine, want, M.scan_bound(2, size, want, F32), "state")
+        for b in range(B):
+            if b in rows:
+                within(y[b], rows[b], M.scan_bound(2, size, rows[b], dtype), "y")
+            else:
+                assert y[b].isnan().all() if slots[b] == pool else (y[b] == 7.0).all()
 
 
 def test_update_is_the_scan():

@@ -75,6 +75,40 @@ def test_lengths(dtype, lengths):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lengths", [[5000] + [i % 40 - 1 for i in range(299)], [9000, 0, 1, 8999, 4096, 4097, -1, 63], [20000] * 5, [6000, 100] * 40])
+@pytest.mark.parametrize("Hq,Hkv,N", [(8, 2, 128), (3, 3, 64), (20, 1, 72)])
+def test_shared_work(dtype, lengths, Hq, Hkv, N):
+    """Tables of more than 4096 tokens: the work is shared equally and units that lie in several runs are joined; more sequences than a block has threads."""
+    check(lengths, Hq, Hkv, N, 16, dtype, seed=7)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("most,B", [(500, 3), (1000, 40), (2000, 100), (4000, 2), (64, 300), (16, 1)])
+@pytest.mark.parametrize("Hq,Hkv,N", [(8, 2, 128), (6, 6, 64), (32, 2, 64)])
+def test_lone_sequences(dtype, most, B, Hq, Hkv, N):
+    """Short tables: clusters of 1 to 8 blocks with a sequence's head each, for sequences of all lengths."""
+    check([(i * 37) % (most + 1) if i else most for i in range(B)], Hq, Hkv, N, 16, dtype, seed=8)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("lengths", [[1, 0, 130, -1, 63, 64, 65, 17], [9000, 5, 300]])
+@pytest.mark.parametrize("N", [64, 128])
+def test_without_tensor_maps(dtype, lengths, N):
+    """Where the driver makes no tensor maps, rows are copied in pieces; results are the same bits (the products see the same tiles)
+    but for tables that are then not given to clusters."""
+    from rwkv_cuda_b200 import _lib
+    L = _lib.lib()
+    with_maps = check(lengths, 8, 2, N, 16, dtype, seed=9)
+    L.rwkvb200_test_disable_tensor_maps(1)
+    try:
+        without = check(lengths, 8, 2, N, 16, dtype, seed=9)
+    finally:
+        L.rwkvb200_test_disable_tensor_maps(0)
+    if max(lengths) > 4096:
+        assert torch.equal(with_maps[0], without[0]) and torch.equal(with_maps[1], without[1])
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("k", [dict(cap=30.0), dict(cap=0.5), dict(window=1), dict(window=100), dict(window=5000), dict(slopes=True), dict(scale=0.0),
                                dict(scale=-0.3), dict(scale=3.0), dict(cap=20.0, window=700, slopes=True)])
 @pytest.mark.parametrize("Hq,Hkv,N", [(8, 2, 128), (3, 1, 40)])
@@ -293,6 +327,60 @@ def test_append(dtype, Hq, Hkv, N, R_, interleaved, page):
                 assert torch.equal(a, b2) and (a[untouched] == 7.0).all()
         if ragged and q is not None:
             assert (outs[0][0][:lead] == 7.0).all() and (outs[0][0][-3:] == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("Hq,Hkv,N,R_,interleaved,page", [(4, 2, 64, 64, False, 16), (33, 5, 64, 32, True, 16), (8, 1, 128, 32, False, 5), (1, 9, 80, 16, True, 48), (0, 2, 128, 0, False, 16)])
+def test_append_many(dtype, Hq, Hkv, N, R_, interleaved, page):
+    """Thousands of tokens: a warp does a token."""
+    import rwkv_cuda_b200 as R
+    g = Hh.gen(N)
+    counts = torch.tensor([1500, 1, 0, 1203, 700])
+    lengths = torch.tensor([10, 0, 5, 1, 4000])
+    B, lead, total = len(counts), 3, int(counts.sum()) + 3 + 5
+    cu = torch.cat([torch.zeros(1, dtype=torch.long), counts.cumsum(0)]) + lead
+    need = -(-(lengths + counts) // page)
+    first = torch.cat([torch.zeros(1, dtype=torch.long), need.cumsum(0)])
+    pages = int(first[-1])
+    order = torch.randperm(pages, generator=g)
+    table = torch.full((B, int(need.max())), -1)
+    for b in range(B):
+        table[b, :need[b]] = order[first[b]:first[b + 1]]
+    k, v = (Hh.randn(g, total, Hkv, N).to(dtype).cuda() for _ in range(2))
+    q = Hh.randn(g, total, Hq, N).to(dtype).cuda() if Hq else None
+    q_out = torch.full_like(q, 7.0) if Hq else None
+    pools = [torch.full((pages, Hkv, page, N), 7.0, dtype=dtype, device="cuda") for _ in range(2)]
+    inv = (10000.0 ** (-torch.arange(0, R_, 2) / max(R_, 1))).cuda() if R_ else None
+    R.ops.paged_append(k, v, *pools, table.int().cuda(), lengths.int().cuda(), cu_seqlens=cu.int().cuda(), q=q, q_out=q_out, inv_freq=inv, interleaved=interleaved)
+    m = torch.arange(lead, total - 5)
+    seq = torch.searchsorted(cu[1:], m, right=True)
+    pos = lengths[seq] + m - cu[seq]
+    where = (table[seq, pos // page].cuda(), slice(None), (pos % page).cuda())
+    m, pos = m.cuda(), pos.cuda()
+    for got, x in ((pools[0][where], k[m]), (q_out[m] if Hq else None, q[m] if Hq else None)):
+        if got is not None:
+            want = M.rotated(x, pos, inv, interleaved, 1.0) if R_ else x.double()
+            within(got, want, M.half_step(dtype) * want.abs() + (16 * M.UNIT * 2 * x.double().abs().max() if R_ else 0.0), "rotated")
+    assert torch.equal(pools[1][where], v[m])
+    for p in pools:
+        p[where] = 7.0
+        assert (p == 7.0).all()
+    assert not Hq or (q_out[:lead] == 7.0).all() and (q_out[-5:] == 7.0).all()
+
+
+def test_sequences_that_make_no_sense():
+    """cu_seqlens and lengths of any values write to no other place than a token's page."""
+    import rwkv_cuda_b200 as R
+    from rwkv_cuda_b200 import _lib
+    x = Hh.randn(Hh.gen(1), 12, 2, 64).cuda()
+    table = torch.zeros(3, 2, dtype=torch.int32, device="cuda")
+    for cu in ([0, -5, 12, 12], [-2 ** 31, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1], [5, 4, 3, 2], [2 ** 31 - 1] * 4, [-2 ** 31] * 4):
+        for lengths in ([0, 0, 0], [2 ** 31 - 1, -2 ** 31, 31]):
+            pools = [torch.full((3, 2, 16, 64), 7.0, device="cuda") for _ in range(2)]
+            R.ops.paged_append(x, x, *pools, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), cu_seqlens=torch.tensor(cu, dtype=torch.int32, device="cuda"))
+            torch.cuda.synchronize()
+            assert (pools[0][1:] == 7.0).all() and (pools[1][1:] == 7.0).all()
+    _lib.lib().rwkvb200_device_status_clear()
 
 
 def test_far_positions():
