@@ -387,6 +387,10 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, q = lane & 3;
     const int units = p.Hkv * p.blocks, N = TMA ? NP : p.N;
     unsigned char* mine = staged + warp * Way::kWarpBytes;
+    if (TMA && threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.keys) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.values) : "memory");
+    }
     Way way(p, maps, bars[warp], mine, lane);
     Start start{0, 1, 0, 0, 0};
     if (!LONE) {
@@ -636,6 +640,10 @@ __global__ void __launch_bounds__(kThreads, 3) attention_fp32_kernel(const Atten
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, t = lane & 7, part = lane >> 3;
     const int units = p.Hkv * p.blocks;
     unsigned char* mine = staged + warp * Way::kWarpBytes;
+    if (TMA && threadIdx.x == 0) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.keys) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.values) : "memory");
+    }
     Way way(p, maps, bars[warp], mine, lane);
     Start start{0, 1, 0, 0, 0};
     if (!LONE) {
