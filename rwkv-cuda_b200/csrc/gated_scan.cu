@@ -355,8 +355,9 @@ constexpr int kBwdStages = 2;
 template <typename E> constexpr int fwd_smem() { return kFwdStages * kWarps * 3 * kFwdTokens<E> * kTile * (int)sizeof(E); }
 template <typename E> constexpr int bwd_smem() { return kBwdStages * kWarps * 4 * kBwdTokens * kTile * (int)sizeof(E); }
 
-// A warp's tile: all tokens and channels are there, no document begins and s <= 1; or not; or some gate is out of range (found on the way)
-enum { kSimpleTile, kDocumentTile, kExtremeTile };
+// A warp's tile: all tokens and channels are there, no document begins and s <= 1; only s <= 1; not even that; or some gate is out of
+// range (found on the way)
+enum { kSimpleTile, kDocumentTile, kLargeTile, kExtremeTile };
 template <int M> using Mode = std::integral_constant<int, M>;
 
 template <typename E, bool WIDE, bool CLUSTER>
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
         Share share;
         Pair<E> least(0.f);
         auto make = [&](auto mode) {
-            constexpr bool kSimple = decltype(mode)::value == kSimpleTile, kExtreme = decltype(mode)::value == kExtremeTile;
+            constexpr bool kSimple = decltype(mode)::value == kSimpleTile, kExtreme = decltype(mode)::value == kExtremeTile, kSmall = decltype(mode)::value <= kDocumentTile;
             share.P = both(1.f);
             share.H = both(0.f);
 #pragma unroll
@@ -413,8 +414,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
                 const Pair<E> vgx(in + kPart + j * kTile), vga(in + 2 * kPart + j * kTile);
                 const Gates<E, kExtreme> g(vga.get(), vgx.get());
                 if (!kExtreme && (kSimple || t + j < p.T)) least.least(vga), least.least(vgx);   // (other rows hold anything)
-                const f2 q = fall<E, kSimple>(mul2(s, g.a)), v = square<kSimple>(q), u = mul2(g.x, get2(in + j * kTile));
-                a[j] = decay<kSimple>(q);
+                const f2 q = fall<E, kSmall>(mul2(s, g.a)), v = square<kSmall>(q), u = mul2(g.x, get2(in + j * kTile));
+                a[j] = decay<kSmall>(q);
                 // (v of 0 or below the normal numbers: beta is 0)
                 w[j] = kSimple ? mul2(mul2(v, each(v, [](float z) { return Fn<E>::inverse_root(fmaxf(z, 1.2e-38f)); })), u)
                                : mul2(mul2(v, inverse_root<E>(v)), u);
@@ -427,8 +428,10 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
             }
             share.P = !kSimple && docs ? both(0.f) : clamp(share.P);
         };
-        int mode = small && docs == 0 && t + kTokens <= p.T && c_tile + kTile <= p.C ? kSimpleTile : kDocumentTile;
-        if (mode == kSimpleTile) make(Mode<kSimpleTile>{}); else make(Mode<kDocumentTile>{});
+        int mode = !small ? kLargeTile : docs == 0 && t + kTokens <= p.T && c_tile + kTile <= p.C ? kSimpleTile : kDocumentTile;
+        if (mode == kSimpleTile) make(Mode<kSimpleTile>{});
+        else if (mode == kDocumentTile) make(Mode<kDocumentTile>{});
+        else make(Mode<kLargeTile>{});
         if (__any_sync(0xffffffffu, live && least.below(kLeast))) {
             mode = kExtremeTile;
             make(Mode<kExtremeTile>{});
@@ -526,7 +529,7 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
         f2 q[kTokens], inv[kTokens], w[kTokens], P, H, Q;
         Pair<E> least(0.f);
         auto make = [&](auto mode) {
-            constexpr bool kSimple = decltype(mode)::value == kSimpleTile, kExtreme = decltype(mode)::value == kExtremeTile;
+            constexpr bool kSimple = decltype(mode)::value == kSimpleTile, kExtreme = decltype(mode)::value == kExtremeTile, kSmall = decltype(mode)::value <= kDocumentTile;
             P = both(1.f);
             H = Q = both(0.f);
 #pragma unroll
@@ -534,30 +537,32 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
                 const Pair<E> vgx(in + kPart + j * kTile), vga(in + 2 * kPart + j * kTile);
                 const Gates<E, kExtreme> g(vga.get(), vgx.get());
                 if (!kExtreme && (kSimple || t + j < p.T)) least.least(vga), least.least(vgx);   // (other rows hold anything)
-                q[j] = fall<E, kSimple>(mul2(s, g.a));
-                const f2 v = square<kSimple>(q[j]), u = mul2(g.x, get2(in + j * kTile));
+                q[j] = fall<E, kSmall>(mul2(s, g.a));
+                const f2 v = square<kSmall>(q[j]), u = mul2(g.x, get2(in + j * kTile));
                 inv[j] = inverse_root<E>(v);
                 w[j] = mul2(mul2(v, inv[j]), u);
                 if (!kSimple) {
                     if (docs >> j & 1) q[j] = both(1.f), inv[j] = both(0.f), w[j] = u;
                     if (t + j >= p.T) q[j] = both(0.f), w[j] = both(0.f);
                 }
-                const f2 a = decay<kSimple>(q[j]);
+                const f2 a = decay<kSmall>(q[j]);
                 H = !kSimple && docs >> j & 1 ? w[j] : fma2(a, H, w[j]);
                 P = mul2(P, a);
             }
 #pragma unroll
             for (int j = kTokens - 1; j >= 0; --j) {
                 if (kSimple) {
-                    Q = mul2(decay<kSimple>(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
+                    Q = mul2(decay<kSmall>(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
                 } else if (t + j < p.T) {
-                    Q = docs >> j & 1 ? both(0.f) : mul2(decay<kSimple>(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
+                    Q = docs >> j & 1 ? both(0.f) : mul2(decay<kSmall>(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
                 }
             }
             P = !kSimple && docs ? both(0.f) : clamp(P);
         };
-        int mode = small && docs == 0 && t + kTokens <= p.T && c_tile + kTile <= p.C ? kSimpleTile : kDocumentTile;
-        if (mode == kSimpleTile) make(Mode<kSimpleTile>{}); else make(Mode<kDocumentTile>{});
+        int mode = !small ? kLargeTile : docs == 0 && t + kTokens <= p.T && c_tile + kTile <= p.C ? kSimpleTile : kDocumentTile;
+        if (mode == kSimpleTile) make(Mode<kSimpleTile>{});
+        else if (mode == kDocumentTile) make(Mode<kDocumentTile>{});
+        else make(Mode<kLargeTile>{});
         if (__any_sync(0xffffffffu, live && least.below(kLeast))) {
             mode = kExtremeTile;
             make(Mode<kExtremeTile>{});
@@ -577,11 +582,11 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
             }
         }
         auto walk = [&](auto mode) {
-            constexpr bool kSimple = decltype(mode)::value == kSimpleTile, kExtreme = decltype(mode)::value == kExtremeTile;
+            constexpr bool kSimple = decltype(mode)::value == kSimpleTile, kExtreme = decltype(mode)::value == kExtremeTile, kSmall = decltype(mode)::value <= kDocumentTile;
 #pragma unroll
             for (int j = 0; j < kTokens; ++j) {
                 const f2 before = h;
-                h = !kSimple && docs >> j & 1 ? w[j] : fma2(decay<kSimple>(q[j]), h, w[j]);
+                h = !kSimple && docs >> j & 1 ? w[j] : fma2(decay<kSmall>(q[j]), h, w[j]);
                 w[j] = before;
             }
             const i64 at = (i64)t * p.C;
@@ -591,8 +596,8 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
                 if (!kSimple && t + j >= p.T) continue;
                 const bool doc = !kSimple && docs >> j & 1;
                 const Gates<E, kExtreme> g(get2(in + 2 * kPart + j * kTile), get2(in + kPart + j * kTile));
-                const f2 vx = get2(in + j * kTile), a = decay<kSimple>(q[j]), G = add2(get2(in + 3 * kPart + j * kTile), e);
-                const f2 beta = doc ? both(1.f) : mul2(square<kSimple>(q[j]), inv[j]);
+                const f2 vx = get2(in + j * kTile), a = decay<kSmall>(q[j]), G = add2(get2(in + 3 * kPart + j * kTile), e);
+                const f2 beta = doc ? both(1.f) : mul2(square<kSmall>(q[j]), inv[j]);
                 const f2 ox = mul2(mul2(G, beta), g.x), og = mul2(mul2(ox, vx), g.rest_x());
                 e = mul2(a, G);
                 const f2 slope = fma2(w[j], both(-1.f), mul2(mul2(mul2(g.x, vx), a), inv[j]));
@@ -609,6 +614,7 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
         };
         if (mode == kSimpleTile) walk(Mode<kSimpleTile>{});
         else if (mode == kDocumentTile) walk(Mode<kDocumentTile>{});
+        else if (mode == kLargeTile) walk(Mode<kLargeTile>{});
         else walk(Mode<kExtremeTile>{});
         if (!CLUSTER && warp == 0) ends[buf][lane] = e;
         stage = stage == S - 1 ? 0 : stage + 1;
