@@ -105,7 +105,7 @@ def attention(q, k, v, scale, cap=0.0, slopes=None, window=0):
     k, v = k.repeat_interleave(Hq // Hkv, 1), v.repeat_interleave(Hq // Hkv, 1)
     z = torch.einsum("hn,thn->ht", q, k) * scale
     bar = torch.einsum("hn,thn->ht", q.abs(), k.abs()) * abs(scale)
-    if cap > 0:
+    if 0 < cap < math.inf:
         z = cap * torch.tanh(z / cap)
     off = 2 * (N + 2) * UNIT * bar + 8 * UNIT * z.abs()
     if slopes is not None:

@@ -83,6 +83,14 @@ def test_shared_work(dtype, lengths, Hq, Hkv, N):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("Hq,N", [(1, 1), (2, 1), (3, 2), (1, 3)])
+def test_more_runs_than_elements(dtype, Hq, N):
+    """One long sequence of tiny heads: hundreds of runs of which each block joins an element or none."""
+    check([60000], Hq, 1, N, 16, dtype, seed=5)
+    check([40000, 3], Hq, 1, N, 16, dtype, seed=5, cap=math.inf)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("most,B", [(500, 3), (1000, 40), (2000, 100), (4000, 2), (64, 300), (16, 1)])
 @pytest.mark.parametrize("Hq,Hkv,N", [(8, 2, 128), (6, 6, 64), (32, 2, 64)])
 def test_lone_sequences(dtype, most, B, Hq, Hkv, N):
