@@ -199,6 +199,42 @@ def test_values_that_are_not_finite(bad):
     assert torch.equal(grads[4], clean_grads[4])
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("C", [64, 2048])
+def test_gates_that_are_not_finite(dtype, C):
+    """A NaN in one gate does not go into the other: with gx NaN (or infinite) the decay stays, so that gradients of earlier tokens stay, and with ga NaN
+    the gradient comes to nothing before it only.  Infinite gates are 0 and 1."""
+    d = inputs(1, 200, C, dtype, seed=6)
+    ins = [d[n] for n in ("x", "gx", "ga", "s", "h0", "first")]
+    y64, _ = M.gated_scan(*ins)
+    ybar, _ = M.gated_scan(*ins, bar=True)
+    want, bars = M.gated_scan_gradients(*ins, d["dy"], d["dhT"])
+    others = [c for c in range(C) if c != 5]
+    for name, bad in (("gx", float("nan")), ("gx", float("inf")), ("gx", float("-inf")), ("ga", float("nan")), ("ga", float("-inf"))):
+        g = d[name].clone()
+        g[0, 100, 5] = bad
+        (y, hT), grads, _ = train({**d, name: g})
+        # What the gate does not reach stays within the bound of the inputs without it; a tile that holds it divides for each gate on
+        # its own, so that its neighbours are rounded in other places and are not the same bits.
+        bound = M.scan_bound(200, ybar, y64, dtype)
+        within(y[:, :100], y64[:, :100], bound[:, :100], "y before")
+        within(y[..., others], y64[..., others], bound[..., others], "y beside")
+        for got, w, bar in list(zip(grads, want, bars))[:3]:
+            bound = M.scan_bound(200, bar, w, dtype)
+            within(got[..., others], w[..., others], bound[..., others], "gradient beside")
+            if name == "gx" and bad != bad:
+                within(got[0, :99, 5], w[0, :99, 5], bound[0, :99, 5], "gradient before")
+        if bad != bad:
+            assert y[0, 100:, 5].isnan().all() and hT[0, 5].isnan()
+            if name == "ga":
+                assert grads[0][0, :100, 5].isnan().all()
+        else:
+            same = {**d, name: g.nan_to_num(posinf=300.0, neginf=-300.0)}   # exp(-300) is 0 in fp32, as of an infinity
+            check(same)
+            y2, hT2 = forward(same)
+            assert torch.equal(y, y2) and torch.equal(hT, hT2)
+
+
 def test_autograd():
     """Walked twice; only one output used; no state; through torch.autograd.Function."""
     import rwkv_cuda_b200 as R
