@@ -6,9 +6,11 @@
 // decoding step and about 100 us for a training step.  Here a call checks its tensors, allocates its outputs and enters the
 // C ABI of librwkvb200.so without coming back to the interpreter.
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -131,7 +133,20 @@ struct OpNode : torch::autograd::Node {
         for (auto& x : kept) x.reset_data();
         released = true;
     }
+    // A leaf that an older graph still holds gets its gradient on the stream of that graph.  The default stream cannot be part of a capture,
+    // and an engine that waits for one on it ends the process.
+    void check_capture() const {
+        if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+        for (uint32_t i = 0; i < num_outputs(); ++i) {
+            const auto& to = next_edge(i).function;
+            if (to == nullptr || !task_should_compute_output(i) || dynamic_cast<torch::autograd::AccumulateGrad*>(to.get()) == nullptr) continue;
+            const auto stream = to->stream();
+            TORCH_CHECK(!stream || c10::cuda::CUDAStream(*stream) != c10::cuda::getDefaultCUDAStream(stream->device_index()), op,
+                        ": captured into a graph while a graph of the default stream holds the same leaf (delete its outputs first)");
+        }
+    }
     variable_list apply(variable_list&& grads) override {
+        check_capture();
         Saved s;
         {
             std::lock_guard<std::mutex> lock(mutex_);

@@ -281,6 +281,46 @@ def test_captured_training_step():
     assert all(torch.equal(a, b) for a, b in zip((*out, *grads), (*want_out, *want)))
 
 
+def test_capture_beside_a_living_graph():
+    """A leaf that a graph of the default stream holds gets its gradient on that stream, which no capture can have: refused.  Once that graph
+    is gone the step is captured."""
+    import rwkv_cuda_b200 as R
+    d = inputs(2, 200, 64, BF, seed=11)
+    want_out, want, leaves = train(d)
+    run = lambda: R.functions.GATED_SCAN.apply(*leaves, None)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        run()
+    torch.cuda.synchronize()
+    alive = run()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="holds the same leaf"):
+        with torch.cuda.graph(graph):
+            out = run()
+            torch.autograd.grad(out, leaves, (d["dy"], d["dhT"]))
+    del alive, out, want_out
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+        grads = torch.autograd.grad(out, leaves, (d["dy"], d["dhT"]))
+    for g in grads:
+        g.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+def test_gradients_that_are_not_contiguous():
+    """A sum's gradient is one element in all places."""
+    import rwkv_cuda_b200 as R
+    d = inputs(2, 70, 64, F32, seed=12)
+    d["dy"], d["dhT"] = torch.ones_like(d["dy"]), torch.ones_like(d["dhT"])
+    want, leaves = train(d)[1:]
+    y, hT = R.functions.GATED_SCAN.apply(*leaves, None)
+    (y.sum() + hT.sum()).backward()
+    assert all(torch.equal(leaf.grad, w) for leaf, w in zip(leaves, want))
+
+
 # ---- one token -----------------------------------------------------------------------------------------------------
 def step(state, x, gx, ga, s, slots):
     """fp64, row after row"""
