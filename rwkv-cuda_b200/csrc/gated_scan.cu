@@ -167,6 +167,11 @@ template <> struct Pair<bf16> {
     __nv_bfloat162 v;
     __device__ __forceinline__ explicit Pair(const bf16* p) : v(*reinterpret_cast<const __nv_bfloat162*>(p)) {}
     __device__ __forceinline__ explicit Pair(float x) : v(__floats2bfloat162_rn(x, x)) {}
+    static __device__ __forceinline__ Pair of(uint32_t w) {
+        Pair p(0.f);
+        p.v = *reinterpret_cast<const __nv_bfloat162*>(&w);
+        return p;
+    }
     __device__ __forceinline__ f2 get() const {
         const uint32_t w = *reinterpret_cast<const uint32_t*>(&v);
         return pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
@@ -187,7 +192,6 @@ template <> struct Pair<float> {
     __device__ __forceinline__ void least(const Pair& o) { v.x = min_nan(v.x, o.v.x), v.y = min_nan(v.y, o.v.y); }
     __device__ __forceinline__ bool all_from(float x) const { return v.x >= x && v.y >= x; }
 };
-template <typename E> __device__ __forceinline__ f2 get2(const E* p) { return Pair<E>(p).get(); }
 // ... to global memory: as one word, or one after the other where C is odd or a tensor starts between two words
 template <bool WORD>
 __device__ __forceinline__ void put2(bf16* p, f2 v, bool second) {
@@ -214,7 +218,7 @@ template <typename E>
 __device__ __forceinline__ E* rows_on(E* p, uint32_t row_bytes, int j) { return reinterpret_cast<E*>(reinterpret_cast<char*>(p) + (uint64_t)row_bytes * (uint32_t)j); }
 
 struct Args {
-    int T, C, tiles, rounds, saves;   // channel tiles, rounds of the kernel, of the backward
+    int B, T, C, tiles, rounds, saves;   // channel tiles, rounds of the kernel, of the backward
     const float* h0;
     const void *x, *gx, *ga;
     const float* s;
@@ -238,31 +242,50 @@ __device__ __forceinline__ uint32_t firsts(const uint8_t* first, int t, int T, i
     return __ballot_sync(0xffffffffu, f);
 }
 
-// Tiles of N tensors, [L][kTile] each, from token t on: to shared memory, without waiting.  WIDE: every row of C starts on a 16-byte
-// boundary, and a piece of 16 bytes is asked for at a time; else element by element, at once.  What lies outside is left alone.
-template <typename E, bool WIDE, int L, int N>
+// How rows of C elements lie in memory: each starts on a 16-byte boundary; on one of a pair of channels (C is even); anywhere.
+enum { kWideRows, kPairRows, kAnyRows };
+// In shared memory a row is kTile elements, or, bf16 anywhere, the 33 words that hold them.
+template <typename E, int ROWS> constexpr int kPitch = sizeof(E) == 2 && ROWS == kAnyRows ? kTile + 2 : kTile;
+
+// Tiles of N tensors, L rows each, from token t on: to shared memory, without waiting.  A lane asks for pieces of 16 bytes, for its pair
+// of each row, or, anywhere, for single words: there is no asynchronous copy of two bytes, so that bf16 rows come with what shares a
+// word with their ends, and are shifted when they are read.  B8 T4096: C4096 238 and 485 us, C4095
+// 532 and 841.  (Element by element, without waiting ahead, a training step of B4 T1761 C2474 took 1310 us instead of 284.)
+// What lies outside is left alone.
+template <typename E, int ROWS, int L, int N>
 struct Fetch {
     static constexpr int n = 16 / sizeof(E), kRow = kTile / n, kRows = 32 / kRow;   // elements of a piece, pieces of a row, rows at a time
+    static constexpr int kPart = L * kPitch<E, ROWS>, kPitchBytes = kPitch<E, ROWS> * (int)sizeof(E), kWords = kTile / 2 + 1;
+    static constexpr bool kShifted = sizeof(E) == 2 && ROWS == kAnyRows;
     const E* from[N];
-    int T, C, row, lane;
-    i64 at;        // of this lane's first piece
-    bool inside;   // its channels
-    __device__ __forceinline__ Fetch(int T, int C, int c_tile, int lane) : T(T), C(C), row(lane / kRow), lane(lane) {
-        const int c = lane % kRow * n;
-        at = (i64)row * C + c;
+    uint32_t off = 0, off_odd;   // bits by which even and odd rows are off, in five bits for each tensor (kShifted; tiles begin at even tokens)
+    int T, C, row, lane, channels;
+    i64 at, base, total;   // at: of this lane's first piece
+    bool inside, edge;     // its channels; the first or the last sequence
+    __device__ __forceinline__ Fetch(int T, int C, int c_tile, int lane, i64 base, i64 total, bool edge)
+        : T(T), C(C), row(lane / kRow), lane(lane), channels(min(kTile, C - c_tile)), base(base), total(total), edge(edge) {
+        const int c = ROWS == kWideRows ? lane % kRow * n : lane * 2;
+        at = (ROWS == kWideRows ? (i64)row * C : 0) + c;
         inside = c_tile + c < C;
     }
-    __device__ __forceinline__ void operator()(E* to, int t, int c_tile) const {
-        if (WIDE) {
-            const uint32_t shared = (uint32_t)__cvta_generic_to_shared(to) + lane * 16;
+    __device__ __forceinline__ void tensor(int k, const void* p) {
+        from[k] = static_cast<const E*>(p) + base;
+        off |= (uint32_t)(reinterpret_cast<uintptr_t>(from[k]) & 2) * 8 << 5 * k;
+        off_odd = off ^ (C & 1 ? 0x84210u : 0u);
+    }
+    __device__ __forceinline__ uint32_t shift(int k, int j) const { return (j & 1 ? off_odd : off) >> 5 * k; }   // (its low five bits)
+    __device__ __forceinline__ void operator()(E* to, int t) const {
+        const uint32_t shared = (uint32_t)__cvta_generic_to_shared(to);
+        const bool whole = t + L <= T;
+        if (ROWS == kWideRows) {
             const i64 first = (i64)t * C + at, step = (i64)kRows * C;
-            if (t + L <= T) {
+            if (whole) {
                 if (inside) {
 #pragma unroll
                     for (int k = 0; k < N; ++k) {
                         const E* p = from[k] + first;
 #pragma unroll
-                        for (int i = 0; i < L / kRows; ++i, p += step) copy(shared + (k * L + i * kRows) * kTile * (int)sizeof(E), p);
+                        for (int i = 0; i < L / kRows; ++i, p += step) copy<16>(shared + lane * 16 + (k * L + i * kRows) * kPitchBytes, p);
                     }
                 }
             } else {
@@ -270,19 +293,82 @@ struct Fetch {
                 for (int k = 0; k < N; ++k)
 #pragma unroll
                     for (int i = 0; i < L / kRows; ++i)
-                        if (inside && t + i * kRows + row < T) copy(shared + (k * L + i * kRows) * kTile * (int)sizeof(E), from[k] + first + i * step);
+                        if (inside && t + i * kRows + row < T) copy<16>(shared + lane * 16 + (k * L + i * kRows) * kPitchBytes, from[k] + first + i * step);
+            }
+        } else if (ROWS == kPairRows) {
+            if (!inside) return;
+            const uint32_t mine = shared + lane * 2 * (int)sizeof(E);
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const E* p = from[k] + (i64)t * C + at;
+#pragma unroll
+                for (int j = 0; j < L; ++j, p += C)
+                    if (whole || t + j < T) copy<2 * sizeof(E)>(mine + (k * L + j) * kPitchBytes, p);
+            }
+        } else if (!kShifted) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const E* p = from[k] + (i64)t * C + lane;
+#pragma unroll
+                for (int j = 0; j < L; ++j, p += C)
+                    if (whole || t + j < T) {
+                        if (lane < channels) copy<4>(shared + lane * 4 + (k * L + j) * kPitchBytes, p);
+                        if (lane + 32 < channels) copy<4>(shared + lane * 4 + 128 + (k * L + j) * kPitchBytes, p + 32);
+                    }
             }
         } else {
+            // word i of a row holds its elements 2 i - 1, 2 i or 2 i, 2 i + 1; one at an end of the tensor may be half outside
+            if (whole && !(edge && (t == 0 || t + L == T))) {
 #pragma unroll
-            for (int k = 0; k < N; ++k)
+                for (int k = 0; k < N; ++k) {
+                    const E* p = from[k] + (i64)t * C + lane * 2;
 #pragma unroll 4
-                for (int j = 0; j < L; ++j)
+                    for (int j = 0; j < L; ++j, p += C) {
+                        const int off = (int)(shift(k, j) >> 4 & 1);
+                        if (lane * 2 - off < channels) copy<4>(shared + lane * 4 + (k * L + j) * kPitchBytes, p - off);
+                    }
+                    // (the 33rd word of row `lane`)
+                    if (lane < L && (shift(k, lane) & 16) != 0 && channels == kTile)
+                        copy<4>(shared + 2 * kTile + (k * L + lane) * kPitchBytes, from[k] + (i64)(t + lane) * C + kTile - 1);
+                }
+            } else {
+#pragma unroll 1
+                for (int k = 0; k < N; ++k) {
+                    const E* tensor = from[0];
 #pragma unroll
-                    for (int c = lane; c < kTile; c += 32)
-                        if (t + j < T) to[(k * L + j) * kTile + c] = c_tile + c < C ? from[k][(i64)(t + j) * C + c] : from_f<E>(0.f);
+                    for (int q = 1; q < N; ++q) tensor = k == q ? from[q] : tensor;
+#pragma unroll 1
+                    for (int w = lane; w < L * kWords; w += 32) {
+                        const int j = w / kWords, i = w % kWords * 2 - (int)(shift(k, j) >> 4 & 1);
+                        if (t + j >= T || i >= channels) continue;
+                        const uint32_t word = shared + (k * L + j) * kPitchBytes + w % kWords * 4;
+                        const i64 nth = (i64)(t + j) * C + i;
+                        if (base + nth >= 0 && base + nth + 1 < total) {
+                            copy<4>(word, tensor + nth);
+                        } else {
+                            const int half = base + nth < 0;
+                            const uint16_t v = *reinterpret_cast<const uint16_t*>(tensor + nth + half);
+                            asm volatile("st.shared.u16 [%0], %1;" ::"r"(word + half * 2), "h"(v) : "memory");
+                        }
+                    }
+                }
+            }
         }
     }
-    static __device__ __forceinline__ void copy(uint32_t to, const E* p) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p) : "memory"); }
+    template <int BYTES> static __device__ __forceinline__ void copy(uint32_t to, const E* p) {
+        if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(p), "n"(BYTES) : "memory");
+    }
+    // two channels of row j of tensor k, from those of the tile's first row on; `kept` has the bits of those that are there (kShifted)
+    __device__ __forceinline__ Pair<E> read(const E* in, int k, int j, uint32_t kept) const {
+        const E* p = in + k * kPart + j * kPitch<E, ROWS>;
+        if constexpr (kShifted) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(p);
+            return Pair<E>::of(__funnelshift_r(w[0], w[1], shift(k, j)) & kept);
+        } else {
+            return Pair<E>(p);
+        }
+    }
 };
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void wait_group() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -358,8 +444,8 @@ __device__ __forceinline__ f2 through_cluster(cg::cluster_group& cluster, int K,
 
 constexpr int kFwdStages = 2;
 constexpr int kBwdStages = 2;
-template <typename E> constexpr int fwd_smem() { return kFwdStages * kWarps * 3 * kFwdTokens<E> * kTile * (int)sizeof(E); }
-template <typename E> constexpr int bwd_smem() { return kBwdStages * kWarps * 4 * kBwdTokens * kTile * (int)sizeof(E); }
+template <typename E, int ROWS> constexpr int fwd_smem() { return kFwdStages * kWarps * 3 * kFwdTokens<E> * kPitch<E, ROWS> * (int)sizeof(E); }
+template <typename E, int ROWS> constexpr int bwd_smem() { return kBwdStages * kWarps * 4 * kBwdTokens * kPitch<E, ROWS> * (int)sizeof(E); }
 
 // A warp's tile: all tokens and channels are there, no document begins and s <= 1; only s <= 1; not even that; or some gate is out of
 // range (found on the way)
@@ -369,24 +455,30 @@ template <int M> using Mode = std::integral_constant<int, M>;
 // B8 T4096 C4096 bf16: 238 us, 4.5 TB/s; 176 us without the arithmetic of the gates, 216 without the exchange between the warps.
 // Special functions 52 %, issue slots 54 %, four warps per scheduler: three blocks per SM with 8 tokens per warp are no faster.
 // One sequence of 32768 tokens, 2048 channels (clusters of 8): 162 us, 111 without the exchange.
-template <typename E, bool WIDE, bool CLUSTER>
+template <typename E, int ROWS, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args p) {
     extern __shared__ __align__(16) unsigned char raw[];
     __shared__ ulonglong2 shares[2][kWarps][32], peers[2][CLUSTER ? kMaxCluster : 1][32];
     __shared__ f2 ends[2][32];   // the state behind a round (a lone block's)
-    constexpr int S = kFwdStages, kTokens = kFwdTokens<E>, kRound = kWarps * kTokens, kPart = kTokens * kTile;
+    constexpr int S = kFwdStages, kTokens = kFwdTokens<E>, kRound = kWarps * kTokens, kPart = kTokens * kPitch<E, ROWS>;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     cg::cluster_group cluster = cg::this_cluster();
     const int K = CLUSTER ? (int)cluster.num_blocks() : 1, rank = CLUSTER ? (int)cluster.block_rank() : 0, unit = blockIdx.x / K;
     const int b = unit / p.tiles, c_tile = unit % p.tiles * kTile, c0 = c_tile + lane * 2;
     const bool live = c0 < p.C, second = c0 + 1 < p.C;
     const i64 base = (i64)b * p.T * p.C + c_tile;
-    Fetch<E, WIDE, kTokens, 3> fetch(p.T, p.C, c_tile, lane);
-    fetch.from[0] = static_cast<const E*>(p.x) + base;
-    fetch.from[1] = static_cast<const E*>(p.gx) + base;
-    fetch.from[2] = static_cast<const E*>(p.ga) + base;
+    Fetch<E, ROWS, kTokens, 3> fetch(p.T, p.C, c_tile, lane, base, (i64)p.B * p.T * p.C, b == 0 || b == p.B - 1);
+    fetch.tensor(0, p.x);
+    fetch.tensor(1, p.gx);
+    fetch.tensor(2, p.ga);
     E* y = static_cast<E*>(p.y) + base + lane * 2;
     E* mine = reinterpret_cast<E*>(raw) + warp * 3 * kPart;
+    const uint32_t kept = second ? 0xffffffffu : 0xffffu;
+    if (ROWS == kAnyRows && sizeof(E) == 4) {   // (a last channel's neighbour stays 0)
+        for (int i = lane; i < S * kWarps * 3 * kPart; i += 32)
+            if (i / (3 * kPart) % kWarps == 0) mine[i] = from_f<E>(0.f);
+        __syncwarp();
+    }
     const uint32_t row_bytes = p.C * (uint32_t)sizeof(E);
     const uint8_t* first = p.first ? p.first + (i64)b * p.T : nullptr;
     const f2 s = pack2(live ? p.s[c0] : 0.f, second ? p.s[c0 + 1] : 0.f);
@@ -396,7 +488,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
 
     auto ask = [&](int round, int stage) {
         const int t = round * kRound + warp * kTokens;
-        if (t < p.T) fetch(mine + stage * kWarps * 3 * kPart, t, c_tile);
+        if (t < p.T) fetch(mine + stage * kWarps * 3 * kPart, t);
         commit();
     };
 #pragma unroll
@@ -420,10 +512,10 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
             share.H = both(0.f);
 #pragma unroll
             for (int j = 0; j < kTokens; ++j) {
-                const Pair<E> vgx(in + kPart + j * kTile), vga(in + 2 * kPart + j * kTile);
+                const Pair<E> vgx = fetch.read(in, 1, j, kept), vga = fetch.read(in, 2, j, kept);
                 const Gates<E, kExtreme> g(vga.get(), vgx.get());
                 if (!kExtreme && (kSimple || t + j < p.T)) least.least(vga), least.least(vgx);   // (other rows hold anything)
-                const f2 q = fall<E, kSmall>(mul2(s, g.a)), v = square<kSmall>(q), u = mul2(g.x, get2(in + j * kTile));
+                const f2 q = fall<E, kSmall>(mul2(s, g.a)), v = square<kSmall>(q), u = mul2(g.x, fetch.read(in, 0, j, kept).get());
                 a[j] = decay<kSmall>(q);
                 // (v of 0 or below the normal numbers: beta is 0)
                 w[j] = kSimple ? mul2(mul2(v, each(v, [](float z) { return Fn<E>::inverse_root(fmaxf(z, 1.2e-38f)); })), u)
@@ -459,13 +551,13 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
 #pragma unroll
             for (int j = 0; j < kTokens; ++j) {
                 h = fma2(a[j], h, w[j]);
-                put2<WIDE>(rows_on(to, row_bytes, j), h, second);
+                put2<ROWS != kAnyRows>(rows_on(to, row_bytes, j), h, second);
             }
         } else {
 #pragma unroll
             for (int j = 0; j < kTokens; ++j) {
                 h = docs >> j & 1 ? w[j] : fma2(a[j], h, w[j]);
-                if (live && t + j < p.T) put2<WIDE>(rows_on(to, row_bytes, j), h, second);
+                if (live && t + j < p.T) put2<ROWS != kAnyRows>(rows_on(to, row_bytes, j), h, second);
             }
         }
         if (!CLUSTER && warp == kWarps - 1) ends[buf][lane] = h;
@@ -486,25 +578,31 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
 // the forward, with the same products of decays.  h before each token is made again from the saved states, and so are the gates
 // in the last walk: keeping them would take more registers than two blocks per SM have.  B8 T4096 C4096 bf16: 487 us, 3.9 TB/s; 419
 // without the exchange, 358 without the arithmetic of the last walk, 325 without that and the gates'.  T32768 C2048: 330, and 220.
-template <typename E, bool WIDE, bool CLUSTER>
+template <typename E, int ROWS, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_backward_kernel(const Args p) {
     extern __shared__ __align__(16) unsigned char raw[];
     __shared__ ulonglong2 shares[2][kWarps][32], peers[2][CLUSTER ? kMaxCluster : 1][32];
     __shared__ f2 forward[2][kWarps][32], ends[2][32];
-    constexpr int S = kBwdStages, kTokens = kBwdTokens, kRound = kWarps * kTokens, kPart = kTokens * kTile;
+    constexpr int S = kBwdStages, kTokens = kBwdTokens, kRound = kWarps * kTokens, kPart = kTokens * kPitch<E, ROWS>;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     cg::cluster_group cluster = cg::this_cluster();
     const int K = CLUSTER ? (int)cluster.num_blocks() : 1, rank = CLUSTER ? (int)cluster.block_rank() : 0, unit = blockIdx.x / K;
     const int b = unit / p.tiles, c_tile = unit % p.tiles * kTile, c0 = c_tile + lane * 2;
     const bool live = c0 < p.C, second = c0 + 1 < p.C;
     const i64 base = (i64)b * p.T * p.C + c_tile;
-    Fetch<E, WIDE, kTokens, 4> fetch(p.T, p.C, c_tile, lane);
-    fetch.from[0] = static_cast<const E*>(p.x) + base;
-    fetch.from[1] = static_cast<const E*>(p.gx) + base;
-    fetch.from[2] = static_cast<const E*>(p.ga) + base;
-    fetch.from[3] = static_cast<const E*>(p.dy) + base;
+    Fetch<E, ROWS, kTokens, 4> fetch(p.T, p.C, c_tile, lane, base, (i64)p.B * p.T * p.C, b == 0 || b == p.B - 1);
+    fetch.tensor(0, p.x);
+    fetch.tensor(1, p.gx);
+    fetch.tensor(2, p.ga);
+    fetch.tensor(3, p.dy);
     E *dx = static_cast<E*>(p.dx) + base + lane * 2, *dgx = static_cast<E*>(p.dgx) + base + lane * 2, *dga = static_cast<E*>(p.dga) + base + lane * 2;
     E* mine = reinterpret_cast<E*>(raw) + warp * 4 * kPart;
+    const uint32_t kept = second ? 0xffffffffu : 0xffffu;
+    if (ROWS == kAnyRows && sizeof(E) == 4) {   // (a last channel's neighbour stays 0)
+        for (int i = lane; i < S * kWarps * 4 * kPart; i += 32)
+            if (i / (4 * kPart) % kWarps == 0) mine[i] = from_f<E>(0.f);
+        __syncwarp();
+    }
     const uint32_t row_bytes = p.C * (uint32_t)sizeof(E);
     const uint8_t* first = p.first ? p.first + (i64)b * p.T : nullptr;
     const f2 s = pack2(live ? p.s[c0] : 0.f, second ? p.s[c0 + 1] : 0.f);
@@ -514,7 +612,7 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
 
     auto ask = [&](int round, int stage) {
         const int t = round * kRound + warp * kTokens;
-        if (round >= 0 && t < p.T) fetch(mine + stage * kWarps * 4 * kPart, t, c_tile);
+        if (round >= 0 && t < p.T) fetch(mine + stage * kWarps * 4 * kPart, t);
         commit();
     };
     const int turns = (p.rounds + K - 1) / K;
@@ -544,11 +642,11 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
             H = Q = both(0.f);
 #pragma unroll
             for (int j = 0; j < kTokens; ++j) {
-                const Pair<E> vgx(in + kPart + j * kTile), vga(in + 2 * kPart + j * kTile);
+                const Pair<E> vgx = fetch.read(in, 1, j, kept), vga = fetch.read(in, 2, j, kept);
                 const Gates<E, kExtreme> g(vga.get(), vgx.get());
                 if (!kExtreme && (kSimple || t + j < p.T)) least.least(vga), least.least(vgx);   // (other rows hold anything)
                 q[j] = fall<E, kSmall>(mul2(s, g.a));
-                const f2 v = square<kSmall>(q[j]), u = mul2(g.x, get2(in + j * kTile));
+                const f2 v = square<kSmall>(q[j]), u = mul2(g.x, fetch.read(in, 0, j, kept).get());
                 inv[j] = inverse_root<E>(v);
                 w[j] = mul2(mul2(v, inv[j]), u);
                 if (!kSimple) {
@@ -562,9 +660,9 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
 #pragma unroll
             for (int j = kTokens - 1; j >= 0; --j) {
                 if (kSimple) {
-                    Q = mul2(decay<kSmall>(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
+                    Q = mul2(decay<kSmall>(q[j]), add2(fetch.read(in, 3, j, kept).get(), Q));
                 } else if (t + j < p.T) {
-                    Q = docs >> j & 1 ? both(0.f) : mul2(decay<kSmall>(q[j]), add2(get2(in + 3 * kPart + j * kTile), Q));
+                    Q = docs >> j & 1 ? both(0.f) : mul2(decay<kSmall>(q[j]), add2(fetch.read(in, 3, j, kept).get(), Q));
                 }
             }
             P = !kSimple && docs ? both(0.f) : clamp(P);
@@ -605,8 +703,8 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
             for (int j = kTokens - 1; j >= 0; --j) {
                 if (!kSimple && t + j >= p.T) continue;
                 const bool doc = !kSimple && docs >> j & 1;
-                const Gates<E, kExtreme> g(get2(in + 2 * kPart + j * kTile), get2(in + kPart + j * kTile));
-                const f2 vx = get2(in + j * kTile), a = decay<kSmall>(q[j]), G = add2(get2(in + 3 * kPart + j * kTile), e);
+                const Gates<E, kExtreme> g(fetch.read(in, 2, j, kept).get(), fetch.read(in, 1, j, kept).get());
+                const f2 vx = fetch.read(in, 0, j, kept).get(), a = decay<kSmall>(q[j]), G = add2(fetch.read(in, 3, j, kept).get(), e);
                 const f2 beta = doc ? both(1.f) : mul2(square<kSmall>(q[j]), inv[j]);
                 const f2 ox = mul2(mul2(G, beta), g.x), og = mul2(mul2(ox, vx), g.rest_x());
                 e = mul2(a, G);
@@ -616,9 +714,9 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
                 const f2 oa = mul2(mul2(dL, mul2(s, g.a)), g.rest_a());
                 ds = fma2(dL, g.a, ds);
                 if (kSimple || live) {
-                    put2<WIDE>(rows_on(px, row_bytes, j), ox, second);
-                    put2<WIDE>(rows_on(pgx, row_bytes, j), og, second);
-                    put2<WIDE>(rows_on(pga, row_bytes, j), oa, second);
+                    put2<ROWS != kAnyRows>(rows_on(px, row_bytes, j), ox, second);
+                    put2<ROWS != kAnyRows>(rows_on(pgx, row_bytes, j), og, second);
+                    put2<ROWS != kAnyRows>(rows_on(pga, row_bytes, j), oa, second);
                 }
             }
         };
@@ -722,10 +820,10 @@ __global__ void __launch_bounds__(kUpdateThreads) scan_update_kernel(int B, int 
     *reinterpret_cast<Wide*>(home) = h;
 }
 
-bool aligned(std::initializer_list<const void*> ps) {
+bool aligned(std::initializer_list<const void*> ps, size_t bytes) {
     uintptr_t all = 0;
     for (const void* p : ps) all |= reinterpret_cast<uintptr_t>(p);
-    return all % 16 == 0;
+    return all % bytes == 0;
 }
 
 int check(const char* what, int dtype, int B, int T, int C) {
@@ -745,10 +843,10 @@ int cluster_size(int units, int rounds) {
 }
 
 template <auto Kernel>
-int launch(const char* what, const Args& p, int B, int K, int smem, cudaStream_t st) {
+int launch(const char* what, const Args& p, int K, int smem, cudaStream_t st) {
     if (allow_smem<Kernel>(smem) != cudaSuccess) return check_launch(what);
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3((unsigned)(B * p.tiles * K));
+    config.gridDim = dim3((unsigned)(p.B * p.tiles * K));
     config.blockDim = dim3(32 * kWarps);
     config.dynamicSmemBytes = smem;
     config.stream = st;
@@ -762,21 +860,31 @@ int launch(const char* what, const Args& p, int B, int K, int smem, cudaStream_t
     return check_launch(what);
 }
 template <typename E>
-int run_forward(const Args& p, int B, int K, cudaStream_t st) {
+int rows_of(int C, std::initializer_list<const void*> ps) {
+    if (C % (16 / sizeof(E)) == 0 && aligned(ps, 16)) return kWideRows;
+    return C % 2 == 0 && aligned(ps, 2 * sizeof(E)) ? kPairRows : kAnyRows;
+}
+template <typename E, int ROWS>
+int run_forward(const Args& p, int K, cudaStream_t st) {
     const char* what = "gated_scan_forward";
-    // 16 bytes a copy where every row starts on such a boundary; else element by element
-    const bool wide = p.C % (16 / sizeof(E)) == 0 && aligned({p.x, p.gx, p.ga, p.y});
-    constexpr int smem = fwd_smem<E>();
-    if (wide) return K > 1 ? launch<scan_forward_kernel<E, true, true>>(what, p, B, K, smem, st) : launch<scan_forward_kernel<E, true, false>>(what, p, B, 1, smem, st);
-    return K > 1 ? launch<scan_forward_kernel<E, false, true>>(what, p, B, K, smem, st) : launch<scan_forward_kernel<E, false, false>>(what, p, B, 1, smem, st);
+    constexpr int smem = fwd_smem<E, ROWS>();
+    return K > 1 ? launch<scan_forward_kernel<E, ROWS, true>>(what, p, K, smem, st) : launch<scan_forward_kernel<E, ROWS, false>>(what, p, 1, smem, st);
 }
 template <typename E>
-int run_backward(const Args& p, int B, int K, cudaStream_t st) {
+int run_forward(const Args& p, int K, cudaStream_t st) {
+    const int rows = rows_of<E>(p.C, {p.x, p.gx, p.ga, p.y});
+    return rows == kWideRows ? run_forward<E, kWideRows>(p, K, st) : rows == kPairRows ? run_forward<E, kPairRows>(p, K, st) : run_forward<E, kAnyRows>(p, K, st);
+}
+template <typename E, int ROWS>
+int run_backward(const Args& p, int K, cudaStream_t st) {
     const char* what = "gated_scan_backward";
-    const bool wide = p.C % (16 / sizeof(E)) == 0 && aligned({p.x, p.gx, p.ga, p.dy, p.dx, p.dgx, p.dga});
-    constexpr int smem = bwd_smem<E>();
-    if (wide) return K > 1 ? launch<scan_backward_kernel<E, true, true>>(what, p, B, K, smem, st) : launch<scan_backward_kernel<E, true, false>>(what, p, B, 1, smem, st);
-    return K > 1 ? launch<scan_backward_kernel<E, false, true>>(what, p, B, K, smem, st) : launch<scan_backward_kernel<E, false, false>>(what, p, B, 1, smem, st);
+    constexpr int smem = bwd_smem<E, ROWS>();
+    return K > 1 ? launch<scan_backward_kernel<E, ROWS, true>>(what, p, K, smem, st) : launch<scan_backward_kernel<E, ROWS, false>>(what, p, 1, smem, st);
+}
+template <typename E>
+int run_backward(const Args& p, int K, cudaStream_t st) {
+    const int rows = rows_of<E>(p.C, {p.x, p.gx, p.ga, p.dy, p.dx, p.dgx, p.dga});
+    return rows == kWideRows ? run_backward<E, kWideRows>(p, K, st) : rows == kPairRows ? run_backward<E, kPairRows>(p, K, st) : run_backward<E, kAnyRows>(p, K, st);
 }
 
 }  // namespace
@@ -805,12 +913,12 @@ extern "C" int rwkvb200_gated_scan_forward(int dtype, int B, int T, int C, const
     if (int e = check("gated_scan_forward", dtype, B, T, C)) return e;
     RWKV_NOTNULL(x); RWKV_NOTNULL(gx); RWKV_NOTNULL(ga); RWKV_NOTNULL(s); RWKV_NOTNULL(y);
     Args p{};
-    p.T = T; p.C = C; p.tiles = (C + kTile - 1) / kTile; p.saves = (T + kSaved - 1) / kSaved; const int round = kWarps * (dtype == RWKVB200_BF16 ? kFwdTokens<bf16> : kFwdTokens<float>);
+    p.B = B; p.T = T; p.C = C; p.tiles = (C + kTile - 1) / kTile; p.saves = (T + kSaved - 1) / kSaved; const int round = kWarps * (dtype == RWKVB200_BF16 ? kFwdTokens<bf16> : kFwdTokens<float>);
     p.rounds = (T + round - 1) / round;
     p.h0 = h0; p.x = x; p.gx = gx; p.ga = ga; p.s = s; p.first = first; p.y = y; p.hT = hT; p.saved = static_cast<float*>(saved);
     const cudaStream_t st = as_stream(stream);
     const int K = cluster_size(B * p.tiles, p.rounds);
-    return dtype == RWKVB200_BF16 ? run_forward<bf16>(p, B, K, st) : run_forward<float>(p, B, K, st);
+    return dtype == RWKVB200_BF16 ? run_forward<bf16>(p, K, st) : run_forward<float>(p, K, st);
 }
 
 extern "C" int rwkvb200_gated_scan_backward(int dtype, int B, int T, int C, const void* x, const void* gx, const void* ga, const float* s,
@@ -820,12 +928,12 @@ extern "C" int rwkvb200_gated_scan_backward(int dtype, int B, int T, int C, cons
     RWKV_NOTNULL(x); RWKV_NOTNULL(gx); RWKV_NOTNULL(ga); RWKV_NOTNULL(s); RWKV_NOTNULL(saved); RWKV_NOTNULL(dy);
     RWKV_NOTNULL(dx); RWKV_NOTNULL(dgx); RWKV_NOTNULL(dga); RWKV_NOTNULL(ds); RWKV_NOTNULL(work);
     Args p{};
-    p.T = T; p.C = C; p.tiles = (C + kTile - 1) / kTile; p.rounds = p.saves = (T + kSaved - 1) / kSaved;
+    p.B = B; p.T = T; p.C = C; p.tiles = (C + kTile - 1) / kTile; p.rounds = p.saves = (T + kSaved - 1) / kSaved;
     p.x = x; p.gx = gx; p.ga = ga; p.s = s; p.first = first; p.saved = static_cast<float*>(const_cast<void*>(saved));
     p.dy = dy; p.dhT = dhT; p.dh0 = dh0; p.dx = dx; p.dgx = dgx; p.dga = dga; p.ds = static_cast<float*>(work);
     const cudaStream_t st = as_stream(stream);
     const int K = cluster_size(B * p.tiles, p.rounds);
-    const int rc = dtype == RWKVB200_BF16 ? run_backward<bf16>(p, B, K, st) : run_backward<float>(p, B, K, st);
+    const int rc = dtype == RWKVB200_BF16 ? run_backward<bf16>(p, K, st) : run_backward<float>(p, K, st);
     return rc != RWKVB200_OK ? rc : sum_rows(RWKVB200_F32, (i64)B * K, C, p.ds, ds, st);
 }
 
@@ -836,7 +944,7 @@ extern "C" int rwkvb200_gated_scan_update(int dtype, int B, int C, int pool, flo
     RWKV_REQUIRE(B <= 65535, RWKVB200_EINVAL, "gated_scan_update: B=%d exceeds 65535", B);
     RWKV_NOTNULL(state); RWKV_NOTNULL(x); RWKV_NOTNULL(gx); RWKV_NOTNULL(ga); RWKV_NOTNULL(s); RWKV_NOTNULL(y);
     // four channels a thread where that leaves every SM a block and all rows start on their boundaries
-    const bool wide = C % 4 == 0 && (i64)B * C >= 4ll * kUpdateThreads * sm_count() && aligned({state, x, gx, ga, s, y});
+    const bool wide = C % 4 == 0 && (i64)B * C >= 4ll * kUpdateThreads * sm_count() && aligned({state, x, gx, ga, s, y}, 16);
     const int per = wide ? 4 : 1;
     const dim3 grid((C + kUpdateThreads * per - 1) / (kUpdateThreads * per), B);
     const cudaStream_t st = as_stream(stream);

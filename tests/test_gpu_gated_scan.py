@@ -151,6 +151,41 @@ def test_unaligned_and_strided():
         assert torch.equal(out[0], y) and torch.equal(out[1], hT)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,T,C,docs", [(2, 80, 129, False), (1, 16, 128, False), (3, 37, 65, True), (1, 8, 1, False), (2, 150, 2047, False), (2, 33, 66, True)])
+@pytest.mark.parametrize("starts", [(0, 0, 0, 0), (1, 0, 1, 1), (0, 1, 1, 0), (1, 1, 1, 1), (2, 3, 0, 1)])
+def test_rows_anywhere(dtype, B, T, C, docs, starts):
+    """Each tensor begins at an element of its own behind a 16-byte boundary, with NaN before and behind it, which stays."""
+    import rwkv_cuda_b200 as R
+    d = inputs(B, T, C, dtype, seed=C, docs=docs)
+    n = B * T * C
+    wants = [d[m] for m in ("x", "gx", "ga", "dy")]
+    room = [torch.full((n + 16,), float("nan"), device="cuda", dtype=dtype) for _ in range(8)]
+    where = [r[8 + o:8 + o + n].view(B, T, C) for r, o in zip(room, starts + starts[::-1])]
+    for to, want in zip(where, wants):
+        to.copy_(want)
+    x, gx, ga, dy, y, dx, dgx, dga = where
+    f, p = dict(device="cuda"), lambda t: t.data_ptr() if t is not None else 0
+    hT, ds, dh0 = torch.empty(B, C, **f), torch.empty(C, **f), torch.empty(B, C, **f)
+    lib, e = R._lib.lib(), 1 if dtype == BF else 0
+    saved = torch.empty(lib.rwkvb200_gated_scan_saved_bytes(B, T, C), dtype=torch.uint8, **f)
+    work = torch.empty(lib.rwkvb200_gated_scan_work_bytes(B, T, C), dtype=torch.uint8, **f)
+    first, stream = d["first"], torch.cuda.current_stream().cuda_stream
+    assert lib.rwkvb200_gated_scan_forward(e, B, T, C, p(d["h0"]), p(x), p(gx), p(ga), p(d["s"]), p(first), p(y), p(hT), p(saved), stream) == 0
+    assert lib.rwkvb200_gated_scan_backward(e, B, T, C, p(x), p(gx), p(ga), p(d["s"]), p(first), p(saved), p(dy), p(d["dhT"]), p(dh0), p(dx), p(dgx), p(dga),
+                                            p(ds), p(work), stream) == 0
+    for r, o in zip(room, starts + starts[::-1]):
+        assert r[:8 + o].isnan().all() and r[8 + o + n:].isnan().all()
+    ins = [d[m] for m in ("x", "gx", "ga", "s", "h0", "first")]
+    y64, hT64 = M.gated_scan(*ins)
+    ybar, hbar = M.gated_scan(*ins, bar=True)
+    within(y, y64, M.scan_bound(T, ybar, y64, dtype), "y")
+    within(hT, hT64, M.scan_bound(T, hbar, hT64, F32), "hT")
+    want, bars = M.gated_scan_gradients(*ins, d["dy"], d["dhT"])
+    for got, w, bar, name in zip((dx, dgx, dga, ds, dh0), want, bars, ("dx", "dgx", "dga", "ds", "dh0")):
+        within(got, w, M.scan_bound(T, bar, w, got.dtype), name)
+
+
 def test_pieces_are_the_whole():
     """A prompt in pieces of any length through the state (in place) is the prompt at once, to rounding."""
     d = inputs(2, 333, 64, F32, seed=4, docs=True)
