@@ -30,7 +30,17 @@ struct AppendArgs {
 };
 
 // VEC elements as they lie in memory
-template <typename E, int VEC> struct Vec;
+template <typename E, int VEC> struct alignas(sizeof(E) * VEC) Vec {
+    E w[VEC];
+    __device__ __forceinline__ void get(float (&f)[VEC]) const {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) f[i] = to_f(w[i]);
+    }
+    __device__ __forceinline__ void set(const float (&f)[VEC]) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) w[i] = from_f<E>(f[i]);
+    }
+};
 template <> struct Vec<bf16, 8> {
     uint4 w;
     __device__ __forceinline__ void get(float (&f)[8]) const {
@@ -53,11 +63,6 @@ template <> struct Vec<float, 4> {
     __device__ __forceinline__ void get(float (&f)[4]) const { f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w; }
     __device__ __forceinline__ void set(const float (&f)[4]) { w = make_float4(f[0], f[1], f[2], f[3]); }
 };
-template <typename E> struct Vec<E, 1> {
-    E w;
-    __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_f(w); }
-    __device__ __forceinline__ void set(const float (&f)[1]) { w = from_f<E>(f[0]); }
-};
 
 // Items of a head of q or k: first the rotated ones: a vector x of the first half and z of the second (half layout), a vector of pairs
 // (interleaved), or (interleaved, VEC = 1) a pair's two elements; then the vectors behind R.
@@ -65,7 +70,7 @@ template <typename E, int VEC, int TEAM>
 __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs p) {
     using V = Vec<E, VEC>;
     constexpr bool kBlock = TEAM == kThreads;
-    constexpr int kAtOnce = kBlock ? 1 : 4;   // heads that a thread has in hand
+    constexpr int kAtOnce = kBlock && VEC > 1 ? 1 : 4;   // heads that a thread has in hand
     __shared__ float cosine[kThreads / TEAM][RWKVB200_MAX_HEAD_SIZE / 2], sine[kThreads / TEAM][RWKVB200_MAX_HEAD_SIZE / 2];
     const int team = threadIdx.x / TEAM, thread = threadIdx.x % TEAM, m = blockIdx.x * (kThreads / TEAM) + team, half = p.R / 2;
     if (m >= p.M) return;   // (a warp of its own: a block's token always is)
@@ -163,7 +168,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs p) {
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u) {
                 const int h = h0 + u * groups;
-                if (kBlock && h0 == group) i[u] = first;
+                if (kBlock && u == 0 && h0 == group) i[u] = first;
                 else if (h < H) load(from, H, h, i[u]);
             }
 #pragma unroll
@@ -187,7 +192,7 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs p) {
 #pragma unroll
             for (int u = 0; u < kAtOnce; ++u) {
                 const int h = h0 + u * v_groups;
-                if (kBlock && h0 == v_group) i[u] = v;
+                if (kBlock && u == 0 && h0 == v_group) i[u] = v;
                 else if (h < p.Hkv) load_v(h, i[u]);
             }
 #pragma unroll
@@ -199,19 +204,28 @@ __global__ void __launch_bounds__(kThreads) append_kernel(const AppendArgs p) {
     }
 }
 
+template <typename E, int VEC>
+void launch(const AppendArgs& p, cudaStream_t st) {
+    // a warp a token where that gives every SM sixteen of them, and a head's items are no more than its lanes
+    if (p.M >= 16 * sm_count() && p.N / VEC <= 32) {
+        constexpr int kPerBlock = kThreads / 32;
+        append_kernel<E, VEC, 32><<<(unsigned)((p.M + kPerBlock - 1) / kPerBlock), kThreads, 0, st>>>(p);
+    } else {
+        append_kernel<E, VEC, kThreads><<<p.M, kThreads, 0, st>>>(p);
+    }
+}
 template <typename E>
 int launch(const AppendArgs& p, cudaStream_t st) {
-    constexpr int VEC = 16 / sizeof(E);
-    uintptr_t all = 0;
-    for (const void* x : {p.q, p.k, p.v, (const void*)p.q_out, (const void*)p.k_pages, (const void*)p.v_pages}) all |= reinterpret_cast<uintptr_t>(x);
-    // 16 bytes a vector where heads and the rotated part (a half of it in the half layout) are whole numbers of them
-    const bool wide = all % 16 == 0 && p.N % VEC == 0 && (p.interleaved ? p.R : p.R / 2) % VEC == 0;
-    // a warp a token where that gives every SM sixteen of them, and a head's items are no more than its lanes
-    const bool warps = wide && p.M >= 16 * sm_count();
-    constexpr int kPerBlock = kThreads / 32;
-    if (warps) append_kernel<E, VEC, 32><<<(unsigned)((p.M + kPerBlock - 1) / kPerBlock), kThreads, 0, st>>>(p);
-    else if (wide) append_kernel<E, VEC, kThreads><<<p.M, kThreads, 0, st>>>(p);
-    else append_kernel<E, 1, kThreads><<<p.M, kThreads, 0, st>>>(p);
+    // The widest vectors, up to 16 bytes, of which heads and the rotated part (a half of it in the half layout) are whole numbers and on whose
+    // boundaries all tensors begin.  (5000 tokens of 48 heads of 80 with 40 rotated elements, by elements and by four: 65 and 40 us.)
+    uintptr_t bytes = 0;
+    for (const void* x : {p.q, p.k, p.v, (const void*)p.q_out, (const void*)p.k_pages, (const void*)p.v_pages}) bytes |= reinterpret_cast<uintptr_t>(x);
+    const int elements = p.N | (p.interleaved ? p.R : p.R / 2);
+    auto fits = [&](int vec) { return elements % vec == 0 && bytes % (vec * sizeof(E)) == 0; };
+    if (sizeof(E) == 2 && fits(8)) launch<E, 16 / sizeof(E)>(p, st);
+    else if (fits(4)) launch<E, 4>(p, st);
+    else if (fits(2)) launch<E, 2>(p, st);
+    else launch<E, 1>(p, st);
     return check_launch("paged_append");
 }
 

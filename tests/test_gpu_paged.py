@@ -282,7 +282,7 @@ def test_offsets_beyond_32_bits():
 @pytest.mark.parametrize("Hq,Hkv,N,R_,interleaved,page", [(4, 2, 64, 64, False, 16), (4, 2, 64, 64, True, 16), (8, 1, 128, 32, False, 5), (8, 1, 128, 32, True, 5),
                                                           (3, 3, 33, 32, False, 7), (3, 3, 33, 10, True, 7), (2, 2, 80, 24, False, 48),
                                                           (2, 2, 80, 20, True, 48), (1, 1, 2, 2, False, 1), (5, 5, 64, 0, False, 16), (0, 2, 64, 64, False, 16),
-                                                          (32, 8, 128, 128, False, 16)])
+                                                          (32, 8, 128, 128, False, 16), (3, 2, 66, 12, False, 7), (2, 3, 66, 22, True, 16)])
 def test_append(dtype, Hq, Hkv, N, R_, interleaved, page):
     import rwkv_cuda_b200 as R
     g = Hh.gen(N + R_)
@@ -338,7 +338,8 @@ def test_append(dtype, Hq, Hkv, N, R_, interleaved, page):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("Hq,Hkv,N,R_,interleaved,page", [(4, 2, 64, 64, False, 16), (33, 5, 64, 32, True, 16), (8, 1, 128, 32, False, 5), (1, 9, 80, 16, True, 48), (0, 2, 128, 0, False, 16)])
+@pytest.mark.parametrize("Hq,Hkv,N,R_,interleaved,page", [(4, 2, 64, 64, False, 16), (33, 5, 64, 32, True, 16), (8, 1, 128, 32, False, 5), (1, 9, 80, 16, True, 48), (0, 2, 128, 0, False, 16),
+                                                          (5, 2, 80, 40, False, 16), (3, 1, 66, 10, True, 16), (2, 2, 30, 14, False, 16), (2, 3, 31, 10, True, 7), (2, 1, 33, 16, False, 16)])
 def test_append_many(dtype, Hq, Hkv, N, R_, interleaved, page):
     """Thousands of tokens: a warp does a token."""
     import rwkv_cuda_b200 as R
