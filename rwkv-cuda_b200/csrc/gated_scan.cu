@@ -21,6 +21,7 @@
 // barrier.  What bounds the kernels is in front of each.
 #include "packed.cuh"
 #include <cooperative_groups.h>
+#include <atomic>
 #include <initializer_list>
 #include <type_traits>
 
@@ -834,12 +835,52 @@ int check(const char* what, int dtype, int B, int T, int C) {
     return RWKVB200_OK;
 }
 
-// How many blocks share a (sequence, channel tile): as many as leave two blocks for every SM, up to what a cluster may have.  (Training
-// step, blocks per tile 1 / 2 / 4 / 8: T32768 C2048, 32 tiles 2344 / 1531 / 846 / 586 us; B8 T1024 C4096, 512 tiles 211 / 239 / 262 / 323.)
-int cluster_size(int units, int rounds) {
-    int K = 1;
-    while (K < kMaxCluster && 2 * K <= rounds && (i64)units * K * 2 <= 2 * sm_count()) K *= 2;
-    return K;
+cudaLaunchAttribute cluster_of(int K) {
+    cudaLaunchAttribute a;
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = K;
+    a.val.clusterDim.y = a.val.clusterDim.z = 1;
+    return a;
+}
+// How many clusters of K blocks of a kernel the current device holds at once (a cluster does not go over the border of a group of SMs, and
+// the groups differ in size).  Asked for once per device.
+template <auto Kernel>
+int clusters_at_once(int K, int smem) {
+    static std::atomic<int> known[64][kMaxCluster + 1];   // + 1
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || allow_smem<Kernel>(smem) != cudaSuccess) return 0;
+    if (dev < 64 && (n = known[dev][K].load(std::memory_order_relaxed)) > 0) return n - 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(K);
+    config.blockDim = dim3(32 * kWarps);
+    config.dynamicSmemBytes = smem;
+    cudaLaunchAttribute cluster = cluster_of(K);
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, Kernel, &config) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    if (dev < 64) known[dev][K].store(n + 1, std::memory_order_relaxed);
+    return n;
+}
+// How many blocks share a (sequence, channel tile): as many as are all there at once, one on every SM (the fp32 backward has that many) or two
+// (where the kernel has two): two side by side take 1.38 times the time of one.  B1 T8192 bf16, training step, K = 1 to 8: 20
+// tiles 454 / 316 / 222 / 166 / 141 / 123 / 151 / 130 us (6 are there one by one), 40 tiles 455 / 315 / 224 / 232 / 198 / 177 / 241 /
+// 232 (of 7 not all at once), 60 tiles 452 / 318 / 311 / 244 / 310.
+int cluster_size(int units, int rounds, bool two) {
+    auto most = [&](auto at_once) {
+        int K = kMaxCluster;
+        while (K > 1 && (units > 2 * sm_count() / K || at_once(K) < units)) --K;
+        return K;
+    };
+    int K = most([](int K) { return clusters_at_once<scan_backward_kernel<float, kWideRows, true>>(K, bwd_smem<float, kWideRows>()); });
+    if (two) {
+        const int other = most([](int K) { return clusters_at_once<scan_forward_kernel<bf16, kWideRows, true>>(K, fwd_smem<bf16, kWideRows>()); });
+        if (other * 100 > K * 138) K = other;
+    }
+    const int turns = (rounds + K - 1) / K;
+    return (rounds + turns - 1) / turns;   // (no block without a round)
 }
 
 template <auto Kernel>
@@ -850,10 +891,7 @@ int launch(const char* what, const Args& p, int K, int smem, cudaStream_t st) {
     config.blockDim = dim3(32 * kWarps);
     config.dynamicSmemBytes = smem;
     config.stream = st;
-    cudaLaunchAttribute cluster;
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = K;
-    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cudaLaunchAttribute cluster = cluster_of(K);
     config.attrs = &cluster;
     config.numAttrs = 1;
     cudaLaunchKernelEx(&config, Kernel, p);
@@ -917,7 +955,7 @@ extern "C" int rwkvb200_gated_scan_forward(int dtype, int B, int T, int C, const
     p.rounds = (T + round - 1) / round;
     p.h0 = h0; p.x = x; p.gx = gx; p.ga = ga; p.s = s; p.first = first; p.y = y; p.hT = hT; p.saved = static_cast<float*>(saved);
     const cudaStream_t st = as_stream(stream);
-    const int K = cluster_size(B * p.tiles, p.rounds);
+    const int K = cluster_size(B * p.tiles, p.rounds, true);
     return dtype == RWKVB200_BF16 ? run_forward<bf16>(p, K, st) : run_forward<float>(p, K, st);
 }
 
@@ -932,7 +970,7 @@ extern "C" int rwkvb200_gated_scan_backward(int dtype, int B, int T, int C, cons
     p.x = x; p.gx = gx; p.ga = ga; p.s = s; p.first = first; p.saved = static_cast<float*>(const_cast<void*>(saved));
     p.dy = dy; p.dhT = dhT; p.dh0 = dh0; p.dx = dx; p.dgx = dgx; p.dga = dga; p.ds = static_cast<float*>(work);
     const cudaStream_t st = as_stream(stream);
-    const int K = cluster_size(B * p.tiles, p.rounds);
+    const int K = cluster_size(B * p.tiles, p.rounds, dtype == RWKVB200_BF16);
     const int rc = dtype == RWKVB200_BF16 ? run_backward<bf16>(p, K, st) : run_backward<float>(p, K, st);
     return rc != RWKVB200_OK ? rc : sum_rows(RWKVB200_F32, (i64)B * K, C, p.ds, ds, st);
 }

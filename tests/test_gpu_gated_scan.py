@@ -72,6 +72,13 @@ def test_blocks_and_clusters(dtype, B, T, C, docs):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,T,C,docs", [(1, 900, 1280, True), (1, 1000, 2304, False), (2, 700, 2880, True), (1, 1030, 3456, False), (4, 333, 833, False), (1, 400, 2560, True)])
+def test_clusters_of_any_size(dtype, B, T, C, docs):
+    """20 to 108 channel tiles: clusters of 2 to 7 blocks, whose last turn has rounds for some of them only."""
+    check(inputs(B, T, C, dtype, seed=T, docs=docs))
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("C", [64, 2048])
 def test_large_decays(dtype, C):
     """s up to 30: beyond L = 1 the decays come from the exponential, down to exp(-30)."""
