@@ -250,8 +250,8 @@ template <typename E, int ROWS> constexpr int kPitch = sizeof(E) == 2 && ROWS ==
 
 // Tiles of N tensors, L rows each, from token t on: to shared memory, without waiting.  A lane asks for pieces of 16 bytes, for its pair
 // of each row, or, anywhere, for single words: there is no asynchronous copy of two bytes, so that bf16 rows come with what shares a
-// word with their ends, and are shifted when they are read.  B8 T4096: C4096 238 and 485 us, C4095
-// 532 and 841.  (Element by element, without waiting ahead, a training step of B4 T1761 C2474 took 1310 us instead of 284.)
+// word with their ends, and are shifted when they are read.  bf16, B8 T4096: C4096 238 and 485 us,
+// C4094 435 and 675, C4095 545 and 817.  (Element by element, without running ahead, a step of B4 T1761 C2474 took 1310 us instead of 262.)
 // What lies outside is left alone.
 template <typename E, int ROWS, int L, int N>
 struct Fetch {
@@ -299,12 +299,18 @@ struct Fetch {
         } else if (ROWS == kPairRows) {
             if (!inside) return;
             const uint32_t mine = shared + lane * 2 * (int)sizeof(E);
+            const uint32_t row_bytes = C * (uint32_t)sizeof(E);
+            const int rows = whole ? L : T - t;
 #pragma unroll
             for (int k = 0; k < N; ++k) {
                 const E* p = from[k] + (i64)t * C + at;
+                if (whole) {
 #pragma unroll
-                for (int j = 0; j < L; ++j, p += C)
-                    if (whole || t + j < T) copy<2 * sizeof(E)>(mine + (k * L + j) * kPitchBytes, p);
+                    for (int j = 0; j < L; ++j) copy<2 * sizeof(E)>(mine + (k * L + j) * kPitchBytes, rows_on(const_cast<E*>(p), row_bytes, j));
+                } else {
+#pragma unroll 1
+                    for (int j = 0; j < rows; ++j) copy<2 * sizeof(E)>(mine + (k * L + j) * kPitchBytes, rows_on(const_cast<E*>(p), row_bytes, j));
+                }
             }
         } else if (!kShifted) {
 #pragma unroll
@@ -320,13 +326,17 @@ struct Fetch {
         } else {
             // word i of a row holds its elements 2 i - 1, 2 i or 2 i, 2 i + 1; one at an end of the tensor may be half outside
             if (whole && !(edge && (t == 0 || t + L == T))) {
+                const uint32_t row_bytes = C * (uint32_t)sizeof(E);
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
                     const E* p = from[k] + (i64)t * C + lane * 2;
+                    if (lane * 2 < channels) {   // (with one before it or not)
 #pragma unroll 4
-                    for (int j = 0; j < L; ++j, p += C) {
-                        const int off = (int)(shift(k, j) >> 4 & 1);
-                        if (lane * 2 - off < channels) copy<4>(shared + lane * 4 + (k * L + j) * kPitchBytes, p - off);
+                        for (int j = 0; j < L; ++j) copy<4>(shared + lane * 4 + (k * L + j) * kPitchBytes, rows_on(const_cast<E*>(p), row_bytes, j) - (shift(k, j) >> 4 & 1));
+                    } else if (lane * 2 == channels) {   // (an even row's last channel is in the word before, an odd one's may be here)
+#pragma unroll 1
+                        for (int j = 0; j < L; ++j)
+                            if ((shift(k, j) & 16) != 0) copy<4>(shared + lane * 4 + (k * L + j) * kPitchBytes, rows_on(const_cast<E*>(p), row_bytes, j) - 1);
                     }
                     // (the 33rd word of row `lane`)
                     if (lane < L && (shift(k, lane) & 16) != 0 && channels == kTile)
