@@ -134,7 +134,7 @@ struct OpNode : torch::autograd::Node {
         released = true;
     }
     // A leaf that an older graph still holds gets its gradient on the stream of that graph.  The default stream cannot be part of a capture,
-    // and an engine that waits for one on it ends the process.
+    // and the engine, which lets it wait for the captured one, breaks the capture or ends the process.
     void check_capture() const {
         if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
         for (uint32_t i = 0; i < num_outputs(); ++i) {
