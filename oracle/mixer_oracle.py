@@ -93,7 +93,7 @@ def attention(q, k, v, scale, cap=0.0, slopes=None, window=0):
 
     A score is a sum of N products: N + 2 units of the sum of their absolute values (the tensor core drops what does not fit instead
     of rounding: twice that), and 8 units of its own size for the cap and the bias.  A weight is off by as much as its
-    exponent, twice (its own and the largest score), and 2^-16 relative where it is kept as two bf16 numbers; the sums over the
+    exponent, twice (its own and the largest score), and 2^-22 relative where it is kept as three bf16 numbers; the sums over the
     tokens add 2^-20."""
     n, Hkv = k.shape[:2]
     Hq, N = q.shape
@@ -122,4 +122,4 @@ def attention(q, k, v, scale, cap=0.0, slopes=None, window=0):
     out = torch.einsum("ht,htn->hn", p, used)
     lse = torch.where(empty[:, 0], -math.inf, m + torch.log(total))
     sizes = torch.einsum("ht,htn->hn", p, used.abs())
-    return out, lse, (2 * off[:, None] + 2.0 ** -16 + 2.0 ** -20) * sizes, off + 2.0 ** -20 + 4 * UNIT * lse.abs()
+    return out, lse, (2 * off[:, None] + 2.0 ** -22 + 2.0 ** -20) * sizes, off + 2.0 ** -20 + 4 * UNIT * lse.abs()

@@ -155,6 +155,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&t);
 }
+// the upper digits of v > 0 as a bf16 number, short of all of it: the rest is 2^-12 to 2^-6.9 of v and exact
+__device__ __forceinline__ float upper_half(float v) { return __uint_as_float(__float_as_uint(v * (1.f - 1.f / 4096.f)) & 0xffff0000u); }
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int BYTES>
 __device__ __forceinline__ void copy_or_zero(uint32_t shared, const void* from, bool there) {
@@ -374,8 +376,9 @@ __device__ __forceinline__ void write_from_cluster(const AttentionArgs& p, float
 // bf16: products on mma.sync m16n8k16 with the tokens in the rows, S^T = K q^T and O^T = V^T P^T, for up to 8 HT query heads that share
 // the keys.  Eight heads make 52 TFLOP/s at the full rate of memory, which mma.sync does with a seventh of its time: the tiles
 // are too narrow for tensor memory to give anything.  Each warp keeps its own maxima and sums.  Both first operands come out of
-// shared memory by ldmatrix (the values transposed).  Weights are taken into the second product as the sum of two bf16
-// numbers (2^-16 relative; one would double the output's rounding), both above 0, so that an infinite value stays one.
+// shared memory by ldmatrix (the values transposed).  Weights are taken into the second product as the sum of three bf16
+// numbers (2^-22 relative, as good as fp32; two leave 2^-16, which shows where values cancel), all above 0, so that an
+// infinite value stays one.
 // 128 sequences of up to 4096 tokens, 32 heads on 8 of 128: 189 us, 5.7 TB/s (87 % of the copy rate); one of 131001 tokens 92 us,
 // 5.8 TB/s.  Short sequences spend their time at the ends of units: 64 of up to 2048 tokens 3.9 TB/s, heads of 64 3.4.
 template <int NP, int HT, int MODE, bool LONE>
@@ -570,21 +573,24 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
                 __syncwarp();
             }
             // weights, and as the second operand of the second product
-            uint32_t high[HT][2], low[HT][2];
+            uint32_t high[HT][2], middle[HT][2], low[HT][2];
 #pragma unroll
             for (int h = 0; h < HT; ++h) {
-                float x[4], y[4];
+                float x[4], y[4], r[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const float top = m[h][e & 1], w = ex2(z[h][e] - (top == -INFINITY ? 0.f : top));
                     l[h][e & 1] += w;
-                    x[e] = __uint_as_float(__float_as_uint(w * (1.f - 1.f / 4096.f)) & 0xffff0000u);
-                    y[e] = w - x[e];
+                    const float least = w > 0.f ? 0x1p-126f : 0.f;   // (parts of a small weight would be 0)
+                    x[e] = upper_half(w);
+                    y[e] = fmaxf(upper_half(w - x[e]), least);
+                    r[e] = fmaxf(w - x[e] - y[e], least);
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     high[h][i] = transposed(pack_bf16(x[2 * i], x[2 * i + 1]));
-                    low[h][i] = transposed(pack_bf16(y[2 * i], y[2 * i + 1]));
+                    middle[h][i] = transposed(pack_bf16(y[2 * i], y[2 * i + 1]));
+                    low[h][i] = transposed(pack_bf16(r[2 * i], r[2 * i + 1]));
                 }
             }
             const uint32_t in = way.values(step) + value_row;
@@ -595,6 +601,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
 #pragma unroll
                 for (int h = 0; h < HT; ++h) {
                     mma(o[h][i], a[0], a[1], a[2], a[3], high[h][0], high[h][1]);
+                    mma(o[h][i], a[0], a[1], a[2], a[3], middle[h][0], middle[h][1]);
                     mma(o[h][i], a[0], a[1], a[2], a[3], low[h][0], low[h][1]);
                 }
             }

@@ -176,6 +176,41 @@ def test_values_that_are_not_finite(dtype, N):
     assert out[4, 2:].isnan().all() and torch.isfinite(out[4, :2]).all() and torch.isfinite(lse[4]).all()
 
 
+@pytest.mark.parametrize("Hq,Hkv,N,page,extra", [(8, 2, 128, 16, 1), (8, 2, 64, 16, 300), (32, 2, 128, 16, 1), (40, 2, 64, 16, 300), (6, 2, 40, 7, 1), (3, 1, 33, 16, 1)])
+def test_weights_keep_their_digits(Hq, Hkv, N, page, extra):
+    """bf16, values of +1 and -1 in turn under nearly equal weights: what is left of them is 1e-3 to 1e-5, so that the rounding of the result hides nothing
+    of the weights' own.  (Weights of 2^-17 relative are several times the bound off.)"""
+    lengths = [2] * 30 + [4, 64, 100]
+    pools, table, kept = paged(lengths, Hkv, N, page, BF, seed=6, extra=extra)
+    for b, n in enumerate(lengths):
+        for j in range(n):
+            at = int(table[b, j // page]), slice(None), j % page
+            kept[b][0][j] = pools[0][at] = kept[b][0][j] * (j % 2) * 2.0 ** -11   # (an even token's score is 0)
+            kept[b][1][j] = pools[1][at] = 1.0 - 2 * (j % 2)
+    q = Hh.randn(Hh.gen(7), len(lengths), Hq, N).to(BF).cuda()
+    out, lse = attend(q, pools, table, lengths)
+    for b, n in enumerate(lengths):
+        o, l, ob, lb = M.attention(q[b], *kept[b], N ** -0.5)
+        within(out[b], o, ob + M.half_step(BF) * o.abs(), f"out {b}")
+        within(lse[b], l, lb, f"lse {b}")
+
+
+def test_small_weights_of_infinite_values():
+    """A weight down to 2^-120 makes an infinite value of the other head's token infinite and not NaN; without weight it is nothing."""
+    for N, Hq in ((64, 2), (128, 12), (40, 2)):
+        for power in (20, 100, 120):
+            pools, table, kept = paged([20], 1, N, 16, BF, seed=2)
+            q = torch.zeros(1, Hq, N, dtype=BF, device="cuda")
+            q[:, :, 0] = 1.0
+            keys, values = (torch.zeros(20, 1, N, dtype=BF, device="cuda") for _ in range(2))
+            keys[:, :, 0], keys[3, :, 0] = 1.0, 1.0 - power
+            values[:], values[3, :, 5] = 0.5, math.inf
+            for j in range(20):
+                pools[0][int(table[0, j // 16]), :, j % 16], pools[1][int(table[0, j // 16]), :, j % 16] = keys[j], values[j]
+            out, _ = attend(q, pools, table, [20], scale=math.log(2))
+            assert (out[0, :, 5] == math.inf).all() and torch.isfinite(out[0, :, :5]).all() and torch.isfinite(out[0, :, 6:]).all()
+
+
 def test_unaligned_tensors():
     """Pools, queries and outputs that start at an odd element."""
     import rwkv_cuda_b200 as R
