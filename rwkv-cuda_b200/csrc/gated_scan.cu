@@ -116,6 +116,8 @@ __device__ __forceinline__ f2 fall(f2 L) {
     if (SMALL) return q;
     return each(L, q, [](float l, float p) { return l <= 1.f ? p : -Fn<E>::exp_minus(l); });
 }
+// s as it is read: -0 becomes 0, as -0 times a gate would come out of the polynomial with the sign of the other form
+__device__ __forceinline__ float rate(float s) { return s + 0.f; }
 // a and 1 - a^2 = (1 - a) (2 - (1 - a)) of what fall has made
 template <bool SMALL>
 __device__ __forceinline__ f2 decay(f2 q) {
@@ -492,7 +494,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
     }
     const uint32_t row_bytes = p.C * (uint32_t)sizeof(E);
     const uint8_t* first = p.first ? p.first + (i64)b * p.T : nullptr;
-    const f2 s = pack2(live ? p.s[c0] : 0.f, second ? p.s[c0 + 1] : 0.f);
+    const f2 s = pack2(live ? rate(p.s[c0]) : 0.f, second ? rate(p.s[c0 + 1]) : 0.f);
     const i64 row = (i64)b * p.C + c0;
     f2 carry = pack2(live && p.h0 ? p.h0[row] : 0.f, second && p.h0 ? p.h0[row + 1] : 0.f);
     const bool small = __all_sync(0xffffffffu, lo(s) <= 1.f && hi(s) <= 1.f);
@@ -616,7 +618,7 @@ __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_back
     }
     const uint32_t row_bytes = p.C * (uint32_t)sizeof(E);
     const uint8_t* first = p.first ? p.first + (i64)b * p.T : nullptr;
-    const f2 s = pack2(live ? p.s[c0] : 0.f, second ? p.s[c0 + 1] : 0.f);
+    const f2 s = pack2(live ? rate(p.s[c0]) : 0.f, second ? rate(p.s[c0 + 1]) : 0.f);
     const i64 row = (i64)b * p.C + c0;
     f2 carry = pack2(live && p.dhT ? p.dhT[row] : 0.f, second && p.dhT ? p.dhT[row + 1] : 0.f), ds = both(0.f);
     const bool small = __all_sync(0xffffffffu, lo(s) <= 1.f && hi(s) <= 1.f);
@@ -814,7 +816,7 @@ __global__ void __launch_bounds__(kUpdateThreads) scan_update_kernel(int B, int 
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const Gates<E, true> g(both(to_f(rga.e[i])), both(to_f(rgx.e[i])));
-            const f2 fallen = fall<E, false>(mul2(both(sc.e[i]), g.a)), v = square<false>(fallen);
+            const f2 fallen = fall<E, false>(mul2(both(rate(sc.e[i])), g.a)), v = square<false>(fallen);
             h.e[i] = fmaf(lo(decay<false>(fallen)), h.e[i], lo(mul2(v, inverse_root<E>(v))) * (lo(g.x) * to_f(rx.e[i])));
             out.e[i] = from_f<E>(h.e[i]);
         }

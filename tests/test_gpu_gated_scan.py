@@ -107,6 +107,57 @@ def test_without_decay(dtype, C):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("C", [64, 130, 2048])
+@pytest.mark.parametrize("beside", [None, 1.0, 1.5, 20.0, "gates"])
+def test_without_decay_beside_others(dtype, C, beside):
+    """s of -0.0 is s of 0.0, which -8 log(1) and a saturated logsigmoid make: alone, beside channels with larger s, and beside gates out of range; also
+    token by token."""
+    import rwkv_cuda_b200 as R
+    d = inputs(2, 70, C, dtype, seed=3, docs=C == 130)
+    none = torch.zeros(C, dtype=torch.bool, device="cuda")
+    none[::3] = True
+    s = torch.full((C,), 0.3 if beside in (None, "gates") else beside, device="cuda")
+    if beside == "gates":
+        d["ga"][:, 5:60:9, 1] = -50.0
+    if beside is None:
+        none[:] = True
+    outs = []
+    for zero in (0.0, -0.0):
+        d["s"] = torch.where(none, zero, s)
+        (y, hT), grads, _ = train(d)
+        outs.append((y, hT, *grads, *forward(d)))
+    assert torch.signbit(d["s"][0])
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    if d["first"] is None:
+        assert torch.equal(outs[1][1][:, none], d["h0"][:, none])
+        assert torch.equal(outs[1][0][..., none], d["h0"].to(dtype)[:, None, none].expand(-1, 70, -1))
+    ins = [d[n] for n in ("x", "gx", "ga", "s", "h0", "first")]
+    want, bars = M.gated_scan_gradients(*ins, d["dy"], d["dhT"])
+    y64, ybar = M.gated_scan(*ins)[0], M.gated_scan(*ins, bar=True)[0]
+    more = 1 + s.max().item()   # a unit of the exponent counts as often as the exponent is large
+    for got, w, bar, name in zip((outs[1][0], *outs[1][2:7]), (y64, *want), (ybar, *bars), ("y", "dx", "dgx", "dga", "ds", "dh0")):
+        within(got, w, M.scan_bound(70, bar * more, w, got.dtype), name)
+    state, y = d["h0"].clone(), torch.empty_like(d["x"][:, 0])
+    for t in range(5):
+        R.ops.gated_scan_update(state, *(d[n][:, t].contiguous() for n in ("x", "gx", "ga")), d["s"], y)
+        assert torch.equal(state[:, none], d["h0"][:, none]) and torch.equal(y[:, none], d["h0"].to(dtype)[:, none])
+
+
+def test_update_without_decay_in_wide_rows():
+    """The same where four channels go to a thread."""
+    import rwkv_cuda_b200 as R
+    for dtype in (BF, F32):
+        d = inputs(100, 1, 1024, dtype, seed=3)
+        d["s"][::2] = -0.0
+        x, gx, ga = (d[n][:, 0].contiguous() for n in ("x", "gx", "ga"))
+        state, y = d["h0"].clone(), torch.empty_like(x)
+        R.ops.gated_scan_update(state, x, gx, ga, d["s"], y)
+        assert torch.equal(state[:, ::2], d["h0"][:, ::2]) and torch.equal(y[:, ::2], d["h0"].to(dtype)[:, ::2])
+        assert (state[:, 1::2] != d["h0"][:, 1::2]).any()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("scale", [8.0, 15.0])
 def test_gates_that_saturate(dtype, scale):
     """Gates from sigmoid(-60) to sigmoid(60): decays of 1 - 1e-27 to exp(-s)."""
