@@ -842,6 +842,9 @@ bool aligned(std::initializer_list<const void*> ps, size_t bytes) {
 int check(const char* what, int dtype, int B, int T, int C) {
     RWKV_REQUIRE(dtype == RWKVB200_F32 || dtype == RWKVB200_BF16, RWKVB200_EINVAL, "%s: unknown dtype %d", what, dtype);
     RWKV_REQUIRE(B > 0 && T > 0 && C > 0, RWKVB200_EINVAL, "%s: B=%d T=%d C=%d must be positive", what, B, T, C);
+    RWKV_REQUIRE(C <= 0x7fffffff - 65536, RWKVB200_EINVAL, "%s: C=%d is too wide", what, C);
+    // (the scan counts the bytes of a row in 32 bits)
+    RWKV_REQUIRE(T == 1 || (i64)C * (dtype == RWKVB200_BF16 ? 2 : 4) <= 0xffffffffll, RWKVB200_EINVAL, "%s: C=%d: rows of 4 GiB", what, C);
     RWKV_REQUIRE((i64)B * ((C + kTile - 1) / kTile) <= 0x7fffffff / kMaxCluster, RWKVB200_EINVAL, "%s: B=%d C=%d: too many blocks", what, B, C);
     RWKV_REQUIRE(T <= 0x7fffffff - 65536, RWKVB200_EINVAL, "%s: T=%d is too long", what, T);
     return RWKVB200_OK;

@@ -83,6 +83,17 @@ def test_status_codes_without_launch():
     assert attend(width=2 ** 27, page=16) == -1 and b"2^31" in err()
 
 
+def test_rows_too_wide_are_refused():
+    """A row's bytes are counted in 32 bits, its channels in 31 with some to spare."""
+    L = _lib.lib()
+    one, err = ctypes.c_void_p(16), L.rwkvb200_last_error
+    for dtype, C, T, word in ((0, 2 ** 30, 2, b"4 GiB"), (0, 2 ** 31 - 65537, 5, b"4 GiB"), (0, 2 ** 31 - 1, 1, b"too wide"), (1, 2 ** 31 - 1, 2, b"too wide"),
+                              (1, 2 ** 31 - 65536, 2, b"too wide")):
+        assert L.rwkvb200_gated_scan_forward(dtype, 1, T, C, None, one, one, one, one, None, one, None, None, None) == -1 and word in err()
+        assert L.rwkvb200_gated_scan_backward(dtype, 1, T, C, one, one, one, one, None, one, one, None, None, one, one, one, one, one, None) == -1 and word in err()
+    assert L.rwkvb200_gated_scan_update(0, 1, 2 ** 31 - 1, 1, one, None, one, one, one, one, one, None) == -1 and b"too wide" in err()
+
+
 def test_ops_refuse_cpu_tensors():
     x, s = torch.zeros(1, 4, 8), torch.zeros(8)
     with pytest.raises(RuntimeError, match="CUDA device"):
