@@ -954,7 +954,7 @@ using namespace rwkvb200;
 
 extern "C" size_t rwkvb200_gated_scan_saved_bytes(int B, int T, int C) {
     if (B <= 0 || T <= 0 || C <= 0) return 0;
-    return (size_t)B * ((T + kSaved - 1) / kSaved) * C * sizeof(float);
+    return (size_t)B * (((size_t)T + kSaved - 1) / kSaved) * C * sizeof(float);
 }
 extern "C" size_t rwkvb200_gated_scan_work_bytes(int B, int T, int C) {
     if (B <= 0 || T <= 0 || C <= 0) return 0;

@@ -94,6 +94,12 @@ def test_rows_too_wide_are_refused():
     assert L.rwkvb200_gated_scan_update(0, 1, 2 ** 31 - 1, 1, one, None, one, one, one, one, one, None) == -1 and b"too wide" in err()
 
 
+def test_saved_bytes_of_any_length():
+    size = _lib.lib().rwkvb200_gated_scan_saved_bytes
+    for T in (2 ** 31 - 1, 2 ** 31 - 64, 2 ** 31 - 63):
+        assert size(3, T, 5) == 3 * -(-T // 64) * 5 * 4
+
+
 def test_ops_refuse_cpu_tensors():
     x, s = torch.zeros(1, 4, 8), torch.zeros(8)
     with pytest.raises(RuntimeError, match="CUDA device"):
