@@ -209,7 +209,7 @@ void launch(const AppendArgs& p, cudaStream_t st) {
     // a warp a token where that gives every SM sixteen of them, and a head's items are no more than its lanes
     if (p.M >= 16 * sm_count() && p.N / VEC <= 32) {
         constexpr int kPerBlock = kThreads / 32;
-        append_kernel<E, VEC, 32><<<(unsigned)((p.M + kPerBlock - 1) / kPerBlock), kThreads, 0, st>>>(p);
+        append_kernel<E, VEC, 32><<<((unsigned)p.M + kPerBlock - 1) / kPerBlock, kThreads, 0, st>>>(p);
     } else {
         append_kernel<E, VEC, kThreads><<<p.M, kThreads, 0, st>>>(p);
     }

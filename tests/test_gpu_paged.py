@@ -443,6 +443,21 @@ def test_far_positions():
     within(pool[0, 0, pos % page], want[0, 0], 16 * M.UNIT * 2 * q.abs().max().double(), "k")
 
 
+def test_append_of_the_most_tokens():
+    """2^31 - 1 rows, of which the last five belong to a sequence: more than an int holds once it is rounded up to whole blocks."""
+    import rwkv_cuda_b200 as R
+    if torch.cuda.mem_get_info()[0] < 12 << 30:
+        pytest.skip("needs 12 GB")
+    M_ = 2 ** 31 - 1
+    k = torch.zeros(M_, 1, 1, dtype=BF, device="cuda")
+    k[-5:, 0, 0] = torch.arange(1.0, 6.0).to(BF)
+    pools = [torch.zeros(2, 1, 4, 1, dtype=BF, device="cuda") for _ in range(2)]
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    R.ops.paged_append(k, k, *pools, ints([0, 0], [1, 0]), ints(-1, 0), cu_seqlens=ints(0, M_ - 5, M_))
+    for p in pools:
+        assert p.flatten().tolist() == [5.0, 0.0, 0.0, 0.0, 1.0, 2.0, 3.0, 4.0]
+
+
 def test_append_to_pages_that_are_none():
     import rwkv_cuda_b200 as R
     from rwkv_cuda_b200 import _lib
