@@ -12,6 +12,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
@@ -134,9 +135,10 @@ struct OpNode : torch::autograd::Node {
         released = true;
     }
     // A leaf that an older graph still holds gets its gradient on the stream of that graph.  The default stream cannot be part of a capture,
-    // and the engine, which lets it wait for the captured one, breaks the capture or ends the process.
+    // and the engine, which lets it wait for the captured one, breaks the capture or ends the process.  (A program that calls the node itself has
+    // the gradients in hand: there is no engine.)
     void check_capture() const {
-        if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+        if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None || torch::autograd::get_current_graph_task_id() == -1) return;
         for (uint32_t i = 0; i < num_outputs(); ++i) {
             const auto& to = next_edge(i).function;
             if (to == nullptr || !task_should_compute_output(i) || dynamic_cast<torch::autograd::AccumulateGrad*>(to.get()) == nullptr) continue;

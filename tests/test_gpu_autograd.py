@@ -280,3 +280,30 @@ def test_gradients_that_are_not_aligned(name):
     whole = torch.autograd.grad(flat.square().sum(), xs, retain_graph=True)
     for a, b in zip(whole, torch.autograd.grad(ys, xs, [2 * y.detach() for y in ys])):
         Hh.assert_close(a, b.double().cpu(), tol, name)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_node_called_in_a_capture(name):
+    """A program that calls a node itself, beside a living graph of the same leaves: there is no engine whose streams could be in the way."""
+    xs, call = cases()[name]
+    xs = [x.cuda().requires_grad_(True) for x in xs]
+    want = gradients(call, xs)
+    ones = [x.detach().requires_grad_(True) for x in xs]
+    with torch.cuda.stream(torch.cuda.Stream()):
+        call(*ones)
+    torch.cuda.synchronize()
+    alive = call(*xs)
+    cots = cotangents(outputs(alive))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ys = outputs(call(*xs))
+        got = ys[0].grad_fn(*cots)
+    for g in got:
+        if g is not None:
+            g.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    of_leaf = {fn.variable: g for (fn, _), g in zip(ys[0].grad_fn.next_functions, got) if fn is not None}   # (a node has its inputs in an order of its own)
+    for x, w in zip(xs, want):
+        assert torch.equal(of_leaf[x].view(w.shape), w)
