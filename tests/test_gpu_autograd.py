@@ -307,3 +307,34 @@ def test_node_called_in_a_capture(name):
     of_leaf = {fn.variable: g for (fn, _), g in zip(ys[0].grad_fn.next_functions, got) if fn is not None}   # (a node has its inputs in an order of its own)
     for x, w in zip(xs, want):
         assert torch.equal(of_leaf[x].view(w.shape), w)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_capture_beside_a_living_graph(name):
+    """A leaf that a graph of the default stream holds gets its gradient on that stream, which no capture can have: refused, with the program and the
+    stream left usable.  Once that graph is gone the same step is captured."""
+    xs, call = cases()[name]
+    xs = [x.cuda().requires_grad_(True) for x in xs]
+    want = gradients(call, xs)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        call(*xs)
+    torch.cuda.synchronize()
+    alive = call(*xs)
+    cots = cotangents(outputs(alive))
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="holds the same leaf"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ys = outputs(call(*xs))
+            torch.autograd.grad(ys, xs, cots)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(outputs(alive), xs, cots), want))
+    del alive, ys
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ys = outputs(call(*xs))
+        got = torch.autograd.grad(ys, xs, cots)
+    for g in got:
+        g.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
