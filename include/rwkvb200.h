@@ -417,6 +417,10 @@ int rwkvb200_wkv7_test_expire_next_forward(void);
  * load their inputs without TMA (the one-group RWKV-7 forward, the plain-load paths of the backward kernels, the
  * mma.sync RWKV-5/6 forward) run; 0 restores the normal choice.  Process-wide.  No counterpart in the reference. */
 int rwkvb200_test_disable_tensor_maps(int on);
+/* Test hook: how many blocks share a (sequence, channel tile) in a gated-scan forward (or backward) of this size, and how many
+ * such groups the current device holds at once (`at_once`).  rows: 0 on 16-byte boundaries, 1 on those of a pair of channels, 2
+ * anywhere.  Negative: an error.  No counterpart in the reference. */
+int rwkvb200_test_gated_scan_cluster(int dtype, int B, int T, int C, int rows, int backward, int* at_once);
 
 #ifdef __cplusplus
 }

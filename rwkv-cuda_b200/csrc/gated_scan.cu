@@ -880,20 +880,20 @@ int clusters_at_once(int K, int smem) {
     return n;
 }
 // How many blocks share a (sequence, channel tile): as many as are all there at once, one on every SM (the fp32 backward has that many) or two
-// (where the kernel has two): two side by side take 1.38 times the time of one.  B1 T8192 bf16, training step, K = 1 to 8: 20
-// tiles 454 / 316 / 222 / 166 / 141 / 123 / 151 / 130 us (6 are there one by one), 40 tiles 455 / 315 / 224 / 232 / 198 / 177 / 241 /
-// 232 (of 7 not all at once), 60 tiles 452 / 318 / 311 / 244 / 310.
-int cluster_size(int units, int rounds, bool two) {
+// (where the kernel has two: it is asked for itself, as rows on any boundary take more shared memory): two side by side take
+// 1.38 times the time of one.  B1 T8192 bf16, training step, K = 1 to 8: 20 tiles 454 / 316 / 222 / 166 / 141 / 123 / 151 / 130 us
+// (6 are there one by one), 40 tiles 455 / 315 / 224 / 232 / 198 / 177 / 241 / 232 (of 7 not all at once), 60 tiles 452 / 318 / 311 /
+// 244 / 310.
+template <auto Kernel>
+int cluster_size(int units, int rounds, int smem) {
     auto most = [&](auto at_once) {
         int K = kMaxCluster;
         while (K > 1 && (units > 2 * sm_count() / K || at_once(K) < units)) --K;
         return K;
     };
     int K = most([](int K) { return clusters_at_once<scan_backward_kernel<float, kWideRows, true>>(K, bwd_smem<float, kWideRows>()); });
-    if (two) {
-        const int other = most([](int K) { return clusters_at_once<scan_forward_kernel<bf16, kWideRows, true>>(K, fwd_smem<bf16, kWideRows>()); });
-        if (other * 100 > K * 138) K = other;
-    }
+    const int other = most([=](int K) { return clusters_at_once<Kernel>(K, smem); });
+    if (other * 100 > K * 138) K = other;
     const int turns = (rounds + K - 1) / K;
     return (rounds + turns - 1) / turns;   // (no block without a round)
 }
@@ -918,24 +918,31 @@ int rows_of(int C, std::initializer_list<const void*> ps) {
     return C % 2 == 0 && aligned(ps, 2 * sizeof(E)) ? kPairRows : kAnyRows;
 }
 template <typename E, int ROWS>
-int run_forward(const Args& p, int K, cudaStream_t st) {
+int forward_cluster(int units, int rounds) { return cluster_size<scan_forward_kernel<E, ROWS, true>>(units, rounds, fwd_smem<E, ROWS>()); }
+template <typename E, int ROWS>
+int backward_cluster(int units, int rounds) { return cluster_size<scan_backward_kernel<E, ROWS, true>>(units, rounds, bwd_smem<E, ROWS>()); }
+template <typename E, int ROWS>
+int run_forward(const Args& p, cudaStream_t st) {
     const char* what = "gated_scan_forward";
     constexpr int smem = fwd_smem<E, ROWS>();
+    const int K = forward_cluster<E, ROWS>(p.B * p.tiles, p.rounds);
     return K > 1 ? launch<scan_forward_kernel<E, ROWS, true>>(what, p, K, smem, st) : launch<scan_forward_kernel<E, ROWS, false>>(what, p, 1, smem, st);
 }
 template <typename E>
-int run_forward(const Args& p, int K, cudaStream_t st) {
+int run_forward(const Args& p, cudaStream_t st) {
     const int rows = rows_of<E>(p.C, {p.x, p.gx, p.ga, p.y});
-    return rows == kWideRows ? run_forward<E, kWideRows>(p, K, st) : rows == kPairRows ? run_forward<E, kPairRows>(p, K, st) : run_forward<E, kAnyRows>(p, K, st);
+    return rows == kWideRows ? run_forward<E, kWideRows>(p, st) : rows == kPairRows ? run_forward<E, kPairRows>(p, st) : run_forward<E, kAnyRows>(p, st);
 }
+// (leaves B K rows of ds in p.ds)
 template <typename E, int ROWS>
-int run_backward(const Args& p, int K, cudaStream_t st) {
+int run_backward(const Args& p, int& K, cudaStream_t st) {
     const char* what = "gated_scan_backward";
     constexpr int smem = bwd_smem<E, ROWS>();
+    K = backward_cluster<E, ROWS>(p.B * p.tiles, p.rounds);
     return K > 1 ? launch<scan_backward_kernel<E, ROWS, true>>(what, p, K, smem, st) : launch<scan_backward_kernel<E, ROWS, false>>(what, p, 1, smem, st);
 }
 template <typename E>
-int run_backward(const Args& p, int K, cudaStream_t st) {
+int run_backward(const Args& p, int& K, cudaStream_t st) {
     const int rows = rows_of<E>(p.C, {p.x, p.gx, p.ga, p.dy, p.dx, p.dgx, p.dga});
     return rows == kWideRows ? run_backward<E, kWideRows>(p, K, st) : rows == kPairRows ? run_backward<E, kPairRows>(p, K, st) : run_backward<E, kAnyRows>(p, K, st);
 }
@@ -970,8 +977,7 @@ extern "C" int rwkvb200_gated_scan_forward(int dtype, int B, int T, int C, const
     p.rounds = (T + round - 1) / round;
     p.h0 = h0; p.x = x; p.gx = gx; p.ga = ga; p.s = s; p.first = first; p.y = y; p.hT = hT; p.saved = static_cast<float*>(saved);
     const cudaStream_t st = as_stream(stream);
-    const int K = cluster_size(B * p.tiles, p.rounds, true);
-    return dtype == RWKVB200_BF16 ? run_forward<bf16>(p, K, st) : run_forward<float>(p, K, st);
+    return dtype == RWKVB200_BF16 ? run_forward<bf16>(p, st) : run_forward<float>(p, st);
 }
 
 extern "C" int rwkvb200_gated_scan_backward(int dtype, int B, int T, int C, const void* x, const void* gx, const void* ga, const float* s,
@@ -985,7 +991,7 @@ extern "C" int rwkvb200_gated_scan_backward(int dtype, int B, int T, int C, cons
     p.x = x; p.gx = gx; p.ga = ga; p.s = s; p.first = first; p.saved = static_cast<float*>(const_cast<void*>(saved));
     p.dy = dy; p.dhT = dhT; p.dh0 = dh0; p.dx = dx; p.dgx = dgx; p.dga = dga; p.ds = static_cast<float*>(work);
     const cudaStream_t st = as_stream(stream);
-    const int K = cluster_size(B * p.tiles, p.rounds, dtype == RWKVB200_BF16);
+    int K = 1;
     const int rc = dtype == RWKVB200_BF16 ? run_backward<bf16>(p, K, st) : run_backward<float>(p, K, st);
     return rc != RWKVB200_OK ? rc : sum_rows(RWKVB200_F32, (i64)B * K, C, p.ds, ds, st);
 }
@@ -1011,4 +1017,22 @@ extern "C" int rwkvb200_gated_scan_update(int dtype, int B, int C, int pool, flo
         if (wide) run(scan_update_kernel<float, 4>, float()); else run(scan_update_kernel<float, 1>, float());
     }
     return check_launch("gated_scan_update");
+}
+
+extern "C" int rwkvb200_test_gated_scan_cluster(int dtype, int B, int T, int C, int rows, int backward, int* at_once) {
+    const char* what = "test_gated_scan_cluster";
+    if (int e = check(what, dtype, B, T, C)) return e;
+    RWKV_REQUIRE(rows >= kWideRows && rows <= kAnyRows, RWKVB200_EINVAL, "%s: rows=%d", what, rows);
+    RWKV_NOTNULL(at_once);
+    const int units = B * ((C + kTile - 1) / kTile);
+    auto ask = [&](auto element, auto mode) {
+        using E = decltype(element);
+        constexpr int ROWS = decltype(mode)::value, round = kWarps * kFwdTokens<E>;
+        const int K = backward ? backward_cluster<E, ROWS>(units, (T + kSaved - 1) / kSaved) : forward_cluster<E, ROWS>(units, (T + round - 1) / round);
+        *at_once = backward ? clusters_at_once<scan_backward_kernel<E, ROWS, true>>(K, bwd_smem<E, ROWS>())
+                            : clusters_at_once<scan_forward_kernel<E, ROWS, true>>(K, fwd_smem<E, ROWS>());
+        return K;
+    };
+    auto of = [&](auto element) { return rows == kWideRows ? ask(element, Mode<kWideRows>{}) : rows == kPairRows ? ask(element, Mode<kPairRows>{}) : ask(element, Mode<kAnyRows>{}); };
+    return dtype == RWKVB200_BF16 ? of(bf16()) : of(0.f);
 }

@@ -79,6 +79,22 @@ def test_clusters_of_any_size(dtype, B, T, C, docs):
 
 
 @pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows", [0, 1, 2])
+def test_clusters_are_there_at_once(dtype, rows):
+    """Whatever the rows' alignment (it decides how much shared memory a block takes): no cluster waits for another to end."""
+    import ctypes
+    from rwkv_cuda_b200 import _lib
+    L, n = _lib.lib(), ctypes.c_int()
+    sizes = set()
+    for backward in (0, 1):
+        for tiles in range(1, 301):
+            K = L.rwkvb200_test_gated_scan_cluster(1 if dtype == BF else 0, 1, 8192, tiles * 64 - (rows == 2), rows, backward, ctypes.byref(n))
+            assert 1 <= K <= 8 and (K == 1 or tiles <= n.value), f"{tiles} clusters of {K}, {n.value} at once"
+            sizes.add(K)
+    assert {1, 2, 4, 8} <= sizes   # (from one block for every two SMs to more blocks than there is room for)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("C", [64, 2048])
 def test_large_decays(dtype, C):
     """s up to 30: beyond L = 1 the decays come from the exponential, down to exp(-30)."""
