@@ -7,7 +7,10 @@ Bounds.  Every factor and sum of a kernel is off by a few units of fp32 (2^-24 r
 passes at most T products, so a result is off by at most (T + 16) d times the same formula with absolute values (a "bar" below),
 with d the units of one token: exponential 4, multiply-add 1, and what the decay gets from its exponent L, which is at most about 1
 here: sigmoid 5, product 1: 16 units are enough.  The other factors are in the result once: a gate is off by 5 units and by as many
-as its argument is large (60 at most here), beta for bf16 tensors by 58 (its series): less than the 16 d that are added.
+as its argument is large (60 at most here), beta by 20: less than the 16 d that are added.
+
+These bounds grow with T whether or not the decays forget.  scan_errors and gradient_errors follow an error through the recurrence instead,
+token by token, and see what is lost in long sequences too.
 """
 import math
 
@@ -72,6 +75,97 @@ def gated_scan_gradients(x, gx, ga, s, h0, first, dy, dhT):
 def scan_bound(T, bar, value, dtype):
     """What an output of the recurrence (two passes over T tokens for a gradient) may be off by."""
     return half_step(dtype) * value.abs() + (2 * T + 32) * 16 * UNIT * bar + 1e-35
+
+
+def _units(x, gx, ga, s, first, dtype):
+    """The factors of each token in fp64 and what a kernel may have them off by, in units relative to each (the decay: as a value).
+
+    An exponential is off by 4 units (CUDA's expf by 2, the hardware's 2^x by 4) and, where its argument is multiplied by log2 e first (bf16), by as
+    many as the argument is large.  A gate is the inverse (2 units; 4 of the product of two) of 1 + that, taken times the other gate's 1 + that: 8 more,
+    and so is what it lacks of 1.  L is a product: 1.  Up to L = 1, 1 - a = q is a polynomial (3 units) of L and a its difference from 1 (1 unit of
+    a); beyond, a is an exponential.  v = 1 - a^2 = q (2 - q) is off by no more than q and 3, 1 / beta by half of that and 4 for the root, beta = v / beta
+    by one more."""
+    x, gx, ga, s = (t.double() for t in (x, gx, ga, s))
+    doc = torch.zeros(*x.shape[:2], 1, dtype=torch.bool, device=x.device) if first is None else first.bool()[..., None]
+    r, i = sigmoid(ga), sigmoid(gx)
+    wide = 1.0 if dtype == torch.bfloat16 else 0.0
+    er, ei = 14 + wide * ga.abs(), 14 + wide * gx.abs()
+    L = s * r
+    eL = er + 1
+    a, q = torch.exp(-L), -torch.expm1(-L)
+    ea = a * L * eL + torch.where(L <= 1, 3 * q + a, a * (L + 5))
+    ev = eL + 6
+    beta = torch.sqrt(-torch.expm1(-2 * L))
+    eb, einv = ev / 2 + 6, ev / 2 + 5
+    zero = torch.zeros_like(a)
+    a, ea, beta, eb = (torch.where(doc, v, t) for v, t in ((0.0, a), (zero, ea), (1.0, beta), (zero, eb)))
+    return doc, x, r, i, er, ei, L, eL, a, ea, beta, eb, einv
+
+
+def _forward_errors(f, h0):
+    """Per token: h before it and behind it, their bars and errors (in units).  A product with the decay and a sum are a unit each, twice: a kernel makes
+    the state before a block of tokens from products of decays and walks the block from there."""
+    doc, x, r, i, er, ei, L, eL, a, ea, beta, eb, einv = f
+    B, T, C = x.shape
+    h = torch.zeros(B, C, dtype=torch.float64, device=x.device) if h0 is None else h0.double()
+    bar, off = h.abs(), torch.zeros_like(h)
+    w = beta * i * x
+    ew = (eb + ei + 2) * w.abs()
+    outs = []
+    for t in range(T):
+        before = h, bar, off
+        h = a[:, t] * h + w[:, t]
+        new = a[:, t] * bar + w[:, t].abs()
+        off = a[:, t] * off + (ea[:, t] + 2 * a[:, t]) * bar + ew[:, t] + 2 * new
+        bar = new
+        outs.append((*before, h, bar, off))
+    return [torch.stack(o, 1) for o in zip(*outs)]
+
+
+def scan_errors(x, gx, ga, s, h0=None, first=None, dtype=None):
+    """(y, hT) in fp64 and what a kernel for tensors of `dtype` may have each off by."""
+    dtype = dtype or x.dtype
+    *_, h, _, off = _forward_errors(_units(x, gx, ga, s, first, dtype), h0)
+    off = UNIT * off + 1e-35
+    return (h, h[:, -1]), (off + half_step(dtype) * h.abs(), off[:, -1])
+
+
+def gradient_errors(x, gx, ga, s, h0, first, dy, dhT, dtype=None):
+    """What a kernel may have (dx, dgx, dga, ds, dh0) off by, with the same meaning: the errors of the gradient that comes into a token
+    go back through the recurrence as those of the state go forward, and every product of a gradient is a unit."""
+    dtype = dtype or x.dtype
+    f = _units(x, gx, ga, s, first, dtype)
+    doc, x, r, i, er, ei, L, eL, a, ea, beta, eb, einv = f
+    B, T, C = x.shape
+    hb, hbar, hoff = _forward_errors(f, h0)[:3]
+    dy = dy.double()
+    e = dhT.double()
+    ebar, eoff = e.abs(), torch.zeros_like(e)
+    Gs = []
+    for t in reversed(range(T)):
+        G, Gbar = dy[:, t] + e, dy[:, t].abs() + ebar
+        Goff = eoff + 2 * Gbar
+        e, ebar = a[:, t] * G, a[:, t] * Gbar
+        eoff = a[:, t] * Goff + (ea[:, t] + 2 * a[:, t]) * Gbar + 2 * ebar
+        Gs.append((G, Gbar, Goff, e, ebar, eoff))
+    G, Gbar, Goff, eG, eGbar, eGoff = (torch.stack(o[::-1], 1) for o in zip(*Gs))
+    i_rest, r_rest = sigmoid(-gx.double()), sigmoid(-ga.double())
+    inv = torch.where(beta > 0, 1 / beta, 0.0)
+    u = i * x
+    dx, dx_off = G * beta * i, beta * i * Goff + (eb + ei + 3) * Gbar * beta * i
+    dgx, dgx_off = dx * x * i_rest, (x * i_rest).abs() * dx_off + (ei + 4) * (Gbar * beta * u * i_rest).abs()
+    part = (u * a * inv).abs()
+    slope, slope_bar = u * a * inv - hb, part + hbar
+    slope_off = (ei + einv + 4) * part + ea * (u * inv).abs() + hoff + slope_bar
+    dL = torch.where(doc, 0.0, eG * slope)
+    dL_bar = torch.where(doc, 0.0, eGbar * slope_bar)
+    dL_off = torch.where(doc, 0.0, slope_bar * eGoff + eGbar * slope_off + eGbar * slope_bar)
+    dga, dga_off = dL * L * r_rest, L * r_rest * (dL_off + (eL + er + 4) * dL_bar)
+    # ds: each of eight warps sums its tokens, then they and the blocks that shared the tokens, then the sequences
+    ds, ds_off = (dL * r).sum((0, 1)), (r * dL_off + er * r * dL_bar).sum((0, 1)) + (T / 8 + 8 * B + 40) * (r * dL_bar).sum((0, 1))
+    step = half_step(dtype)
+    offs = [UNIT * o + step * v.abs() + 1e-35 for o, v in ((dx_off, dx), (dgx_off, dgx), (dga_off, dga))]
+    return (dx, dgx, dga, ds, e), (*offs, UNIT * ds_off + 1e-35, UNIT * eoff + 1e-35)
 
 
 def rotated(x, position, inv_freq, interleaved, factor):

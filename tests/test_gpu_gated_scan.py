@@ -78,6 +78,32 @@ def test_clusters_of_any_size(dtype, B, T, C, docs):
     check(inputs(B, T, C, dtype, seed=T, docs=docs))
 
 
+def check_digits(d):
+    """Forward, training forward and gradients within the bounds that follow errors through the decays."""
+    ins = [d[n] for n in ("x", "gx", "ga", "s", "h0", "first")]
+    want, bounds = M.scan_errors(*ins)
+    for out in (forward(d), train(d)[0]):
+        for got, w, b, name in zip(out, want, bounds, ("y", "hT")):
+            within(got, w, b, name)
+    grads = train(d)[1]
+    want, bounds = M.gradient_errors(*ins, d["dy"], d["dhT"])
+    for got, w, b, name in zip(grads, want, bounds, ("dx", "dgx", "dga", "ds", "dh0")):
+        within(got, w, b, name)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,T,C,docs", [(1, 1, 64, False), (3, 17, 65, True), (2, 130, 192, False), (1, 1040, 768, True), (2, 1000, 130, False), (8, 512, 1024, True),
+                                        (1, 1999, 1919, False), (1, 2500, 192, False), (1, 6000, 64, True), (150, 70, 64, False)])
+@pytest.mark.parametrize("decays", ["usual", "large"])
+def test_digits_in_long_sequences(dtype, B, T, C, docs, decays):
+    """The bound does not grow with T where the state forgets: what rounds to fewer digits anywhere is seen after thousands of tokens too."""
+    d = inputs(B, T, C, dtype, seed=T, docs=docs)
+    if decays == "large":   # from 0 over the border of the two forms of the decay to exp(-30), all in every tile
+        few = torch.tensor([0.0, -0.0, 1e-6, 0.1, 1.0 - 2 ** -24, 1.0, 1.0 + 2 ** -23, 1.7, 2.5, 8.0, 30.0], device="cuda")
+        d["s"] = few[torch.arange(C, device="cuda") % len(few)].contiguous()
+    check_digits(d)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("rows", [0, 1, 2])
 def test_clusters_are_there_at_once(dtype, rows):
@@ -531,6 +557,29 @@ def test_update_is_the_scan():
         R.ops.gated_scan_forward(x[:, None], gx[:, None], ga[:, None], d["s"], z, h0=b, hT=b)
         torch.testing.assert_close(a, b, rtol=1e-6, atol=1e-6)
         torch.testing.assert_close(y, z[:, 0], rtol=2 ** -7, atol=1e-6)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("B,C", [(3, 130), (100, 1024)])
+def test_update_and_scan_keep_their_digits(dtype, B, C):
+    """Tokens one at a time, each element within its own bound, and the scan over the same tokens within the same: channels without decay, at the border of
+    its two forms, and far beyond it side by side, gates out of the ordinary range among them."""
+    import rwkv_cuda_b200 as R
+    T = 9
+    d = inputs(B, T, C, dtype, seed=C)
+    few = torch.tensor([0.3, -0.0, 0.0, 1.0 - 2 ** -24, 1.0, 1.0 + 2 ** -23, 2.0, 30.0], device="cuda")
+    d["s"] = few[torch.arange(C, device="cuda") % len(few)].contiguous()
+    d["ga"][:, 4, ::5], d["gx"][:, 6, 1::5] = -45.0, 50.0
+    want, bounds = M.scan_errors(*(d[n] for n in ("x", "gx", "ga", "s", "h0")))
+    y, hT = forward(d)
+    within(y, want[0], bounds[0], "y of the scan")
+    within(hT, want[1], bounds[1], "hT of the scan")
+    state = d["h0"].clone()
+    for t in range(T):
+        y = torch.empty(B, C, dtype=dtype, device="cuda")
+        R.ops.gated_scan_update(state, *(d[n][:, t].contiguous() for n in ("x", "gx", "ga")), d["s"], y)
+        within(y, want[0][:, t], bounds[0][:, t], f"y {t}")
+    within(state, want[1], bounds[1], "state")
 
 
 def test_refusals():

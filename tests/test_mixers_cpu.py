@@ -26,6 +26,49 @@ def test_gradient_formulas_are_autograds():
         assert (bar >= a.abs() * (1 - 1e-12)).all()
 
 
+def test_bounds_that_follow_the_decays_see_lost_digits():
+    """The formulas in fp32 stay within the bounds at any length; the same with one intermediate rounded to bf16, or with results rounded to it, do not."""
+    g = Hh.gen(3)
+    B, C = 2, 24
+    s = -8 * torch.log(Hh.rand(g, C, lo=0.9, hi=0.999))
+    for T in (60, 1500):
+        x, gx, ga, dy = (Hh.randn(g, B, T, C) for _ in range(4))
+        h0, dhT, first = Hh.randn(g, B, C), Hh.randn(g, B, C), Hh.rand(g, B, T) < 0.01
+        (y64, hT64), (by, bhT) = M.scan_errors(x, gx, ga, s, h0, first)
+        want, bounds = M.gradient_errors(x, gx, ga, s, h0, first, dy, dhT)
+        for a, b in zip((y64, *want), (M.gated_scan(x, gx, ga, s, h0, first)[0], *M.gated_scan_gradients(x, gx, ga, s, h0, first, dy, dhT)[0])):
+            torch.testing.assert_close(a, b, rtol=1e-11, atol=1e-12)
+        same, short = lambda v: v, lambda v: v.bfloat16().float()
+        for lossy in (None, "a", "beta", "u", "h", "G"):
+            on = lambda name: short if name == lossy else same
+            doc = first[..., None]
+            r, i = torch.sigmoid(ga), torch.sigmoid(gx)
+            L = s * r
+            a = on("a")(torch.exp(-L)).masked_fill(doc, 0.0)
+            beta = on("beta")(torch.sqrt(-torch.expm1(-2 * L))).masked_fill(doc, 1.0)
+            u = on("u")(i * x)
+            h, ys = h0, []
+            for t in range(T):
+                h = on("h")(a[:, t] * h + beta[:, t] * u[:, t])
+                ys.append(h)
+            y = torch.stack(ys, 1)
+            e, Gs = dhT, []
+            for t in reversed(range(T)):
+                Gs.append(on("G")(dy[:, t] + e))
+                e = a[:, t] * Gs[-1]
+            G = torch.stack(Gs[::-1], 1)
+            before = torch.cat([h0[:, None], y[:, :-1]], 1)
+            dL = (G * (u * torch.where(doc, 0.0, a * a / beta) - a * before)).masked_fill(doc, 0.0)
+            got = (G * beta * i, G * beta * u * (1 - i), dL * L * (1 - r), (dL * r).sum((0, 1)), e)
+            inside = [bool(((v.double() - w).abs() <= b).all()) for v, w, b in zip((y, h, *got), (y64, hT64, *want), (by, bhT, *bounds))]
+            if lossy is None:
+                assert all(inside), inside
+                for v, w, b in zip((y, h, *got), (y64, hT64, *want), (by, bhT, *bounds)):
+                    assert ((short(v).double() - w).abs() > b).any()
+            else:
+                assert not all(inside), lossy
+
+
 def test_attention_form():
     g = Hh.gen(2)
     q, k, v = Hh.randn(g, 6, 16), Hh.randn(g, 50, 2, 16), Hh.randn(g, 50, 2, 16)
