@@ -157,6 +157,12 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 }
 // the upper digits of v > 0 as a bf16 number, short of all of it: the rest is 2^-12 to 2^-6.9 of v and exact
 __device__ __forceinline__ float upper_half(float v) { return __uint_as_float(__float_as_uint(v * (1.f - 1.f / 4096.f)) & 0xffff0000u); }
+// ... of a small weight it would come to 0, and 0 times an infinite value to NaN: 2^-126 at least (also of no weight at all)
+__device__ __forceinline__ uint32_t not_zero(uint32_t v) {
+    uint32_t d;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(0x00800080u));
+    return d;
+}
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int BYTES>
 __device__ __forceinline__ void copy_or_zero(uint32_t shared, const void* from, bool there) {
@@ -581,16 +587,16 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
                 for (int e = 0; e < 4; ++e) {
                     const float top = m[h][e & 1], w = ex2(z[h][e] - (top == -INFINITY ? 0.f : top));
                     l[h][e & 1] += w;
-                    const float least = w > 0.f ? 0x1p-126f : 0.f;   // (parts of a small weight would be 0)
                     x[e] = upper_half(w);
-                    y[e] = fmaxf(upper_half(w - x[e]), least);
-                    r[e] = fmaxf(w - x[e] - y[e], least);
+                    r[e] = w - x[e];
+                    y[e] = upper_half(r[e]);
+                    r[e] -= y[e];
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     high[h][i] = transposed(pack_bf16(x[2 * i], x[2 * i + 1]));
-                    middle[h][i] = transposed(pack_bf16(y[2 * i], y[2 * i + 1]));
-                    low[h][i] = transposed(pack_bf16(r[2 * i], r[2 * i + 1]));
+                    middle[h][i] = transposed(not_zero(pack_bf16(y[2 * i], y[2 * i + 1])));
+                    low[h][i] = transposed(not_zero(pack_bf16(r[2 * i], r[2 * i + 1])));
                 }
             }
             const uint32_t in = way.values(step) + value_row;
