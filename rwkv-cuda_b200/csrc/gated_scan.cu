@@ -10,8 +10,8 @@
 //
 // (dL = 0 at a document's first token; where L = 0 the term through beta is taken as 0.)
 //
-// A block owns 32 lanes x 2 channels of one sequence and goes through it in rounds of kWarps x 16 (backward: 8) tokens, a warp
-// owns 16 of them: it makes the gates of its tokens in registers, reduces them to (P, H) (the product of the decays and the end
+// A block owns 32 lanes x 2 channels of one sequence and goes through it in rounds of kWarps x 16 (backward and fp32: 8) tokens, a
+// warp owns 16 (8) of them: it makes the gates of its tokens in registers, reduces them to (P, H) (the product of the decays and the end
 // state from a zero start), all warps fold those of the warps before theirs onto the block's state, and each walks its tokens
 // once more from its own start state.  Every input is read once, y is written once.  Where there are few (sequence, channel)
 // blocks, a cluster of blocks shares the rounds: block k of K takes rounds k, k + K, ..., and the (P, H) of their rounds go
@@ -53,8 +53,9 @@ __device__ __forceinline__ float rsqrt_fast(float x) {
     return y;
 }
 
-// The functions behind the gates: for bf16 tensors the hardware approximations (2e-7 relative: 2^-14 of a step of bf16), for fp32
-// CUDA's exponential and one step of Newton's method behind the others.
+// The functions behind the gates: for bf16 tensors the hardware approximations (2e-7 relative, and for the exponential as many units of
+// 2^-24 as its argument is large, from the product with log2 e: 5e-7 at 10, 1.9e-6 at 41; a step of bf16 is 4e-3), for fp32 CUDA's
+// exponential and one step of Newton's method behind the others.
 constexpr float kLog2e = 1.4426950408889634f;
 template <typename E> struct Fn;
 template <> struct Fn<bf16> {
@@ -101,8 +102,8 @@ template <typename F> __device__ __forceinline__ f2 each(f2 a, F f) { return pac
 template <typename F> __device__ __forceinline__ f2 each(f2 a, f2 b, F f) { return pack2(f(lo(a), lo(b)), f(hi(a), hi(b))); }
 
 // 1 - exp(-L) of two channels, with all its digits where L is small: for L <= 1 as L times a polynomial (interpolation of
-// (1 - exp(-L)) / L at the Chebyshev points of [0, 1]: off by 3e-9, and by one unit of fp32 as it is evaluated), which takes no
-// special function; beyond it -exp(-L), which has the digits of a instead (decay and fallen tell the two apart by the sign).
+// (1 - exp(-L)) / L at the Chebyshev points of [0, 1]: off by 2.4e-8 with its coefficients in fp32, and by 1.4e-7 as it is evaluated),
+// which takes no special function; beyond it -exp(-L), which has the digits of a instead (decay and fallen tell the two apart by the sign).
 // SMALL: s <= 1 in all channels of the warp.
 template <typename E, bool SMALL>
 __device__ __forceinline__ f2 fall(f2 L) {
@@ -466,7 +467,9 @@ enum { kSimpleTile, kDocumentTile, kLargeTile, kExtremeTile };
 template <int M> using Mode = std::integral_constant<int, M>;
 
 // B8 T4096 C4096 bf16: 238 us, 4.5 TB/s; 176 us without the arithmetic of the gates, 216 without the exchange between the warps.
-// Special functions 52 %, issue slots 54 %, four warps per scheduler: three blocks per SM with 8 tokens per warp are no faster.
+// Special functions 52 %, issue slots 54 %, four warps per scheduler: three blocks per SM with 8 tokens per warp are no faster.  Of
+// the 128 registers a few are short: 112 to 156 bytes of spills a thread (rows anywhere 644 to 704).  With s up to 8 in each tile 320 us, with a gate
+// below -41 in each 463.
 // One sequence of 32768 tokens, 2048 channels (clusters of 8): 162 us, 111 without the exchange.
 template <typename E, int ROWS, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args p) {
@@ -591,6 +594,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_forward_kernel(const Args
 // the forward, with the same products of decays.  h before each token is made again from the saved states, and so are the gates
 // in the last walk: keeping them would take more registers than two blocks per SM have.  B8 T4096 C4096 bf16: 487 us, 3.9 TB/s; 419
 // without the exchange, 358 without the arithmetic of the last walk, 325 without that and the gates'.  T32768 C2048: 330, and 220.
+// fp32 takes 198 to 209 registers and 128 KB: one block of eight warps per SM, B8 T512 C1024 46 us for 18 of bytes.
 template <typename E, int ROWS, bool CLUSTER>
 __global__ void __launch_bounds__(32 * kWarps, sizeof(E) == 2 ? 2 : 1) scan_backward_kernel(const Args p) {
     extern __shared__ __align__(16) unsigned char raw[];

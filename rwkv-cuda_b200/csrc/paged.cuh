@@ -8,7 +8,8 @@
 
 namespace rwkvb200 {
 
-// n / d for 0 <= n < 2^31 by a multiplication (d >= 1)
+// n / d for 0 <= n < 2^31 by a multiplication (d >= 1): the high half of n times a 33-bit reciprocal rounded up, whose top bit is the
+// addition of n (Granlund and Montgomery, division by invariant integers)
 struct Divisor {
     uint32_t d, mul, shift;
     explicit Divisor(uint32_t value) : d(value), mul(0), shift(0) {

@@ -3,7 +3,9 @@
 //   z_j = scale q.k_j      z_j = cap tanh(z_j / cap)      z_j += slope_h (j - (len - 1))      max(0, len - window) <= j < len
 //   out = sum_j exp(z_j - m) v_j / sum_j exp(z_j - m)     lse = m + log(sum)                  m = max_j z_j
 //
-// The keys and values of the sequences are read once; memory bounds it.  The work is all tiles (of 64 or 32 tokens) of all units (a
+// The keys and values of the sequences are read once for each block of up to 16 (bf16) or 8 (fp32) query heads that share them, with few
+// sequences out of L2 from the second time on; memory bounds it up to there, the products beyond (128 sequences of up to 4096
+// tokens, 8 key-value heads of 128, bf16: 4 to 8 query heads on each 199 to 252 us, 16 360, 32 685; fp32: 8 468, 16 910, 32 1810).  The work is all tiles (of 64 or 32 tokens) of all units (a
 // sequence, a key-value head, a block of its query heads) behind one another; every block takes an equal run of them, so that
 // one long sequence and many of different lengths both fill the GPU.  A unit that lies in one block's run is finished there; of
 // the others each block leaves (m, sum, sum of exp v) and a second kernel joins them.  A block's run has at most one unit that
@@ -385,8 +387,8 @@ __device__ __forceinline__ void write_from_cluster(const AttentionArgs& p, float
 // shared memory by ldmatrix (the values transposed).  Weights are taken into the second product as the sum of three bf16
 // numbers (2^-22 relative, as good as fp32; two leave 2^-16, which shows where values cancel), all above 0, so that an
 // infinite value stays one.
-// 128 sequences of up to 4096 tokens, 32 heads on 8 of 128: 189 us, 5.7 TB/s (87 % of the copy rate); one of 131001 tokens 92 us,
-// 5.8 TB/s.  Short sequences spend their time at the ends of units: 64 of up to 2048 tokens 3.9 TB/s, heads of 64 3.4.
+// 128 sequences of up to 4096 tokens, 32 heads on 8 of 128: 199 to 203 us with the join, 5.4 TB/s (82 % of the copy rate); one of 131001
+// tokens 101 us, 5.3 TB/s.  Short sequences spend their time at the ends of units: 64 of up to 2048 tokens 3.9 TB/s, heads of 64 3.4.
 template <int NP, int HT, int MODE, bool LONE>
 __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const AttentionArgs p, const __grid_constant__ Maps maps) {
     using Way = Steps<bf16, NP, MODE>;
@@ -642,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
 
 // fp32: packed multiply-adds, for up to HB query heads that share the keys.  Scores: lane (part, t) takes a quarter of key t
 // times all queries (which lie in shared memory, scaled), and the quarters are added so that lane (part, t) ends with the scores of
-// HB / 4 heads.  Sums: a lane has NP / 32 elements of every head, the weights of a token come out of shared memory.  One sequence of
+// HB / 4 heads (q times the scale is rounded once more than q: half a unit of the score).  Sums: a lane has NP / 32 elements of every head, the weights of a token come out of shared memory.  One sequence of
 // 100000 tokens, 64 heads on 8 of 128: 5.7 TB/s; 32 of up to 2048 tokens, 32 heads on 8: 4.0.
 template <int NP, int HB, int MODE, bool LONE>
 __global__ void __launch_bounds__(kThreads, 3) attention_fp32_kernel(const AttentionArgs p, const __grid_constant__ Maps maps) {
