@@ -349,7 +349,8 @@ int rwkvb200_wkv7_select_form(int form);
  *   x, gx, ga, y, dy, dx, dgx, dga (B,T,C) in `dtype`; s, ds (C), h0, hT, dhT, dh0 (B,C) fp32; first (B,T) bytes.
  *   L = s[c] sigmoid(ga)    a = exp(-L)    beta = sqrt(1 - a^2)    h_t = a h_{t-1} + beta sigmoid(gx) x    y_t = h_t
  *   Where first != 0 a document begins: a = 0 and beta = 1, and nothing of the tokens before (infinities and NaN too) reaches it.
- *   s >= 0 (softplus of a parameter, times a constant, by the caller).  Where L = 0 the gradient through beta is taken as 0.
+ *   s >= 0 (softplus of a parameter, times a constant, by the caller).  Where L = 0 the gradient through beta is taken as 0; where
+ *   1 - a^2 is below the normal numbers of fp32 (gates below -87), beta, 1e-19 at most, counts as 0 too.
  *   h0 (zeros), hT, first, saved, dhT (zeros) and dh0 may be NULL; hT may be h0.
  * The forward of a training step leaves states in `saved` (rwkvb200_gated_scan_saved_bytes(B,T,C) bytes) for the backward, which
  * needs `work` (rwkvb200_gated_scan_work_bytes(B,T,C) bytes; free after the call); ds is summed in a fixed order.
