@@ -159,10 +159,16 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 }
 // the upper digits of v > 0 as a bf16 number, short of all of it: the rest is 2^-12 to 2^-6.9 of v and exact
 __device__ __forceinline__ float upper_half(float v) { return __uint_as_float(__float_as_uint(v * (1.f - 1.f / 4096.f)) & 0xffff0000u); }
-// ... of a small weight it would come to 0, and 0 times an infinite value to NaN: 2^-126 at least (also of no weight at all)
-__device__ __forceinline__ uint32_t not_zero(uint32_t v) {
+// ... of a small weight it would come to 0, and 0 times an infinite value to NaN.  Two weights: their lower parts are the smallest number
+// there is (2^-133) at least, but 0 where the upper part, and with it the weight, is 0.
+__device__ __forceinline__ uint32_t least_part(uint32_t upper) {
     uint32_t d;
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(0x00800080u));
+    asm("min.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(upper), "r"(0x00010001u));
+    return d;
+}
+__device__ __forceinline__ uint32_t at_least(uint32_t v, uint32_t least) {
+    uint32_t d;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(v), "r"(least));
     return d;
 }
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -596,9 +602,10 @@ __global__ void __launch_bounds__(kThreads, 3) attention_mma_kernel(const Attent
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    high[h][i] = transposed(pack_bf16(x[2 * i], x[2 * i + 1]));
-                    middle[h][i] = transposed(not_zero(pack_bf16(y[2 * i], y[2 * i + 1])));
-                    low[h][i] = transposed(not_zero(pack_bf16(r[2 * i], r[2 * i + 1])));
+                    const uint32_t upper = pack_bf16(x[2 * i], x[2 * i + 1]), least = least_part(upper);
+                    high[h][i] = transposed(upper);
+                    middle[h][i] = transposed(at_least(pack_bf16(y[2 * i], y[2 * i + 1]), least));
+                    low[h][i] = transposed(at_least(pack_bf16(r[2 * i], r[2 * i + 1]), least));
                 }
             }
             const uint32_t in = way.values(step) + value_row;

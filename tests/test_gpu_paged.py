@@ -211,6 +211,29 @@ def test_small_weights_of_infinite_values():
             assert (out[0, :, 5] == math.inf).all() and torch.isfinite(out[0, :, :5]).all() and torch.isfinite(out[0, :, 6:]).all()
 
 
+def test_large_values_without_weight():
+    """The largest values there are, under weights that are 0 in fp32 or nearly so, in some heads or all of them: nothing is left of them."""
+    for dtype in (BF, F32):
+        for N, Hq in ((64, 2), (128, 12), (40, 2)):
+            pools, table, kept = paged([70], 1, N, 16, dtype, seed=2)
+            top = torch.finfo(BF).max
+            q = torch.zeros(1, Hq, N, dtype=dtype, device="cuda")
+            q[:, :, 0] = 1.0
+            q[:, ::2, 1] = 1.0      # (odd heads give token 9 its full weight)
+            keys, values = (torch.zeros(70, 1, N, dtype=dtype, device="cuda") for _ in range(2))
+            keys[3, :, 0], values[3, :, 5] = -1000.0, top
+            keys[60, :, 0], values[60, :, 6] = -150.0, -top    # 2^-150 top = 2^-22
+            keys[9, :, 1], values[9, :, 7] = -500.0, 2.0 ** 100
+            for j in range(70):
+                at = int(table[0, j // 16]), slice(None), j % 16
+                pools[0][at], pools[1][at] = keys[j], values[j]
+            out, _ = attend(q, pools, table, [70], scale=math.log(2))
+            assert (out[0, :, :5] == 0).all() and (out[0, :, 5] == 0).all() and (out[0, :, 8:] == 0).all()
+            assert (out[0, :, 6].abs() <= 2.0 ** -22).all()   # (weights below 2^-126 are 0)
+            assert (out[0, ::2, 7] == 0).all()
+            torch.testing.assert_close(out[0, 1::2, 7].double(), torch.full((Hq // 2,), 2.0 ** 100 / 68, dtype=torch.float64, device="cuda"), rtol=2 ** -8, atol=0)
+
+
 def test_unaligned_tensors():
     """Pools, queries and outputs that start at an odd element."""
     import rwkv_cuda_b200 as R
