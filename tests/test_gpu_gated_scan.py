@@ -104,6 +104,33 @@ def test_digits_in_long_sequences(dtype, B, T, C, docs, decays):
     check_digits(d)
 
 
+@pytest.mark.parametrize("B,T,C", [(1, 34, 2 ** 26 + 8), (1, 2_200_003, 1000), (3, 1_100_001, 667)])
+def test_more_elements_than_32_bits(B, T, C):
+    """Tensors of 2.2e9 bf16 elements, wide or long: parts at their ends against fp64.  s of 0.5 and more forgets 1000 tokens to less than 1e-100."""
+    import rwkv_cuda_b200 as R
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    g = torch.Generator("cuda").manual_seed(1)
+    x, gx, ga, dy = (torch.empty(B, T, C, dtype=BF, device="cuda").normal_(generator=g) for _ in range(4))
+    s = 0.5 + torch.rand(C, device="cuda", generator=g)
+    leaves = [t.requires_grad_(True) for t in (x, gx, ga, s)]
+    y, hT = R.functions.GATED_SCAN.apply(*leaves)
+    dx, dgx, dga, _ = torch.autograd.grad(y, leaves, dy)
+    n = min(T, 1200)
+    for c in (slice(0, 40), slice(C - 40, C)):
+        part = lambda t, at: t.detach()[:, at, c].contiguous()
+        first, last = slice(0, n), slice(T - n, T)
+        w, b = M.scan_errors(*(part(t, last) for t in (x, gx, ga)), s[c].detach())
+        kept = slice(max(0, n - 100), n)
+        within(part(y, last)[:, kept], w[0][:, kept], b[0][:, kept], "y")
+        within(hT.detach()[:, c], w[1], b[1], "hT")
+        for at, kept in ((first, slice(0, min(n, 100))), (last, slice(max(0, n - 100), n) if n < T else slice(0, n))):
+            h0 = torch.zeros(B, 40, device="cuda")
+            w, b = M.gradient_errors(*(part(t, at) for t in (x, gx, ga)), s[c].detach(), h0, None, part(dy, at), h0)
+            for got, ww, bb, name in zip((dx, dgx, dga), w, b, ("dx", "dgx", "dga")):
+                within(part(got, at)[:, kept], ww[:, kept], bb[:, kept], name)
+
+
 @pytest.mark.parametrize("dtype", [BF, F32])
 @pytest.mark.parametrize("rows", [0, 1, 2])
 def test_clusters_are_there_at_once(dtype, rows):
